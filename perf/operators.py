@@ -78,7 +78,7 @@ def draw(rng):
     passes = 1 if op == "top_k" else 3
     rows = _spread(rng, 1, max(1, min(4096, MOST_BYTES // (SIZES[kind] * passes * max(classes, stride)))))
     case = {"op": op, "type": kind, "classes": classes, "stride": stride, "rows": rows,
-            "temperature": rng.choice([1.0, 1.0, 2.0, 4.0, 0.7]), "norm": rng.random() < 0.5}
+            "temperature": rng.choice([1.0, 1.0, 2.0, 4.0, 0.75]), "norm": rng.random() < 0.5}
     if op == "top_k":
         case.update(k=_spread(rng, 1, 512), masked=rng.choice([0.0, 0.0, 0.5, 0.99]))
     else:
