@@ -30,7 +30,8 @@ def _as_arg(a):
 
 
 def call(name: str, *args, cfg: Optional[KernelConfig] = None, stream: Optional[int] = None):
-    """Invoke entry point `name`; `args` are everything before (cfg, stream)."""
+    """Invoke entry point `name`; `args` are everything before (cfg, stream).  Returns what the entry point returns:
+    None, or for those that can refuse their arguments 0 or an error code (nothing is enqueued then)."""
     lib = load()
     restype, argtypes, names = lib.prototypes[name]
     if len(args) != len(argtypes) - 2:
@@ -39,7 +40,7 @@ def call(name: str, *args, cfg: Optional[KernelConfig] = None, stream: Optional[
         cfg = DEFAULT_CONFIG
     if stream is None:
         stream = torch.cuda.current_stream().cuda_stream
-    lib.symbol(name)(*[_as_arg(a) for a in args], ctypes.byref(cfg), ctypes.c_void_p(stream))
+    return lib.symbol(name)(*[_as_arg(a) for a in args], ctypes.byref(cfg), ctypes.c_void_p(stream))
 
 
 def take_last_error() -> int:

@@ -279,6 +279,66 @@ void anode_gpu_softmax_nd_cat_nll_ignore_packed_f32(uint32_t prefix_dim, uint32_
 void anode_gpu_softmax_nd_cat_nll_bwd_ignore_packed_f32(uint32_t prefix_dim, uint32_t dim0, uint32_t dim1, const float *dy, const float *softmax, const uint32_t *cat_data, float *dx, ANODE_LAUNCH_TAIL);
 void anode_gpu_softmax_nd_cat_nll_bwd_ignore_packed_accumulate_f32(uint32_t prefix_dim, uint32_t dim0, uint32_t dim1, const float *dy, const float *softmax, const uint32_t *cat_data, float *dx, ANODE_LAUNCH_TAIL);
 
+/* ---- rows of many classes: a teacher's top logits, distillation from them, verification of drafted tokens.  No
+ *      counterpart in the reference; they stand beside the row form of softmax, NLL and arg-max above.
+ *
+ * Logits and gradients are float, bfloat16 or half (the 16-bit types as uint16_t); everything else is float or
+ * uint32_t.  Row r of a [dim0 classes, dim1 rows] array of logits starts r * stride elements into it (a padded
+ * vocabulary; what lies between dim0 and stride is neither read nor written); stride = 0 means rows without padding.
+ * dim0 * dim1 may pass 2^32 here.  Per-row arrays of k slots are packed, slots first.  0xffffffff stands for "no class".
+ * These entry points check their arguments before they touch the device: they return 0, or hipErrorInvalidValue
+ * (1), also recorded for anode_gpu_take_last_error(), with the reason on stderr and nothing enqueued.  Refused are
+ * stride < dim0 (unless 0), k > 1024, a temperature that is not positive and finite (or so small that its
+ * reciprocal is not), missing arrays and 16-bit or float arrays that are not aligned to their type. ---- */
+
+/* The k largest values of every row, largest first, and their classes: [k, dim1] each.  Of equal values (-0 equals +0)
+ * the lower class comes first; NaN and -inf are never taken, as in anode_gpu_arg_max_packed_u32, and slots left over
+ * hold -inf and 0xffffffff.  log_norm (may be null) gets ln sum_k exp(x[k] / temperature) of the whole row: -inf where
+ * the row holds -inf only, NaN where it holds a NaN or +inf.  The temperature serves log_norm alone. */
+int anode_gpu_top_k_rows_f32(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *x, float *value, uint32_t *index, float *log_norm, ANODE_LAUNCH_TAIL);
+int anode_gpu_top_k_rows_bf16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const uint16_t *x, float *value, uint32_t *index, float *log_norm, ANODE_LAUNCH_TAIL);
+int anode_gpu_top_k_rows_f16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const uint16_t *x, float *value, uint32_t *index, float *log_norm, ANODE_LAUNCH_TAIL);
+/* Distillation: the loss of each row of student logits x against the k largest logits of a teacher, as the entry point
+ * above writes them (teacher_value, teacher_index: [k, dim1], in any order).  A slot whose class is >= dim0, or whose
+ * value is -inf or NaN, is absent.  With t = temperature:
+ *   p_k  = exp(teacher_value[k] / t) / sum over the row's slots         where teacher_log_norm is null,
+ *   p_k  = exp(teacher_value[k] / t - teacher_log_norm[row])            otherwise (log_norm at the same temperature);
+ *   q    = softmax(x / t), row_max = max x, row_sum = sum exp((x - row_max) / t);
+ *   loss = sum_k p_k (ln p_k - ln q[teacher_index[k]]), a term with p_k = 0 being 0.
+ * A row without a slot has loss 0 whatever x holds (ignored positions).  A row of x that holds NaN or +inf, or -inf
+ * only, gives NaN as its softmax does.  One slot holding the label is softmax_cat_nll. */
+int anode_gpu_softmax_distill_rows_f32(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, float *loss, float *row_max, float *row_sum, ANODE_LAUNCH_TAIL);
+int anode_gpu_softmax_distill_rows_bf16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, float *loss, float *row_max, float *row_sum, ANODE_LAUNCH_TAIL);
+int anode_gpu_softmax_distill_rows_f16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, float *loss, float *row_max, float *row_sum, ANODE_LAUNCH_TAIL);
+/* Its gradient, from the row_max and row_sum of the forward pass: dx[j] = dy[row] / t * (P q[j] - sum of the p_k whose
+ * class is j), P = sum_k p_k (1 where teacher_log_norm is null).  Slots may name a class more than once.  dx lies as
+ * x does (same stride) and may be x itself.  A row without a slot has dx = 0. */
+int anode_gpu_softmax_distill_bwd_rows_f32(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *dy, const float *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *row_max, const float *row_sum, float *dx, ANODE_LAUNCH_TAIL);
+int anode_gpu_softmax_distill_bwd_rows_bf16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *dy, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *row_max, const float *row_sum, uint16_t *dx, ANODE_LAUNCH_TAIL);
+int anode_gpu_softmax_distill_bwd_rows_f16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *dy, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *row_max, const float *row_sum, uint16_t *dx, ANODE_LAUNCH_TAIL);
+/* dx += ..., added in 32 bits or more and rounded once; dx may not be x.  A row without a slot is left as it is. */
+int anode_gpu_softmax_distill_bwd_rows_accumulate_f32(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *dy, const float *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *row_max, const float *row_sum, float *dx, ANODE_LAUNCH_TAIL);
+int anode_gpu_softmax_distill_bwd_rows_accumulate_bf16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *dy, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *row_max, const float *row_sum, uint16_t *dx, ANODE_LAUNCH_TAIL);
+int anode_gpu_softmax_distill_bwd_rows_accumulate_f16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *dy, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *row_max, const float *row_sum, uint16_t *dx, ANODE_LAUNCH_TAIL);
+/* Loss and gradient in one call, for a dy that is known before the forward pass (e.g. 1 / rows): the row is read once.
+ * dx may be x itself. */
+int anode_gpu_softmax_distill_fused_fwd_bwd_rows_f32(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *dy, float *loss, float *row_max, float *row_sum, float *dx, ANODE_LAUNCH_TAIL);
+int anode_gpu_softmax_distill_fused_fwd_bwd_rows_bf16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *dy, float *loss, float *row_max, float *row_sum, uint16_t *dx, ANODE_LAUNCH_TAIL);
+int anode_gpu_softmax_distill_fused_fwd_bwd_rows_f16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *dy, float *loss, float *row_max, float *row_sum, uint16_t *dx, ANODE_LAUNCH_TAIL);
+/* Verification of drafted tokens (speculative decoding) against the target's probabilities, from given random numbers
+ * in [0, 1).  Arrays, first index fastest: target [dim0 classes, dim1 + 1, dim2 sequences]; draft [dim0, dim1, dim2];
+ * draft_token, accept [dim1, dim2]; draft_length, pick, accepted [dim2]; token [dim1 + 1, dim2].  Sequence b holds
+ * min(draft_length[b], dim1) drafted tokens (draft_length null: dim1 each).  Token i is taken while
+ *   accept[i] * draft[token_i, i] < target[token_i, i]         (a class >= dim0 is never taken);
+ * accepted[b] is how many are.  One more token is then drawn: after a refusal at i from max(0, target[., i] -
+ * draft[., i]) -- from target[., i] where nothing is left of that -- and after the last from target[., draft_length];
+ * drawn is the smallest class whose running sum of weights exceeds pick times their total, in 64 bits.  (A pick
+ * of 1 or more, or NaN, draws the last class that weighs; weights that are not greater than zero, NaN among them, do not
+ * weigh; where none weighs the token is 0xffffffff.)  draft may be null: each drafted token is then a point mass (it was
+ * looked up, or chosen greedily), taken with probability target[token].  token[., b] gets the taken tokens, the drawn one
+ * and 0xffffffff behind it.  dim1 = 0 draws one token of each target row. */
+int anode_gpu_verify_draft_packed_f32(uint32_t dim0, uint32_t dim1, uint32_t dim2, const float *target, const float *draft, const uint32_t *draft_token, const uint32_t *draft_length, const float *accept, const float *pick, uint32_t *token, uint32_t *accepted, ANODE_LAUNCH_TAIL);
+
 /* ---- the neighbours anode takes from its sibling library gpudevicemem (source not part of the reference tree) ----
  * Signatures follow the call sites in src/ops_gpu.rs; the arithmetic is the closed form those call sites imply.
  * Exported under this library's prefix; the five that anode calls directly over FFI are repeated below under
