@@ -107,6 +107,27 @@ struct RowGroups {
   }
 };
 
+// 16-byte groups through a buffer descriptor: one offset register serves every group of a thread (the rest of the address
+// is scalar), a group past the end loads zeros and stores nothing.  The memory has to be 4-byte aligned and shorter than
+// 4 GiB.  NT: kNtStore as in store_stream(), kNtLoad as in load_stream().
+struct GroupBuffer {
+  __amdgpu_buffer_rsrc_t rsrc;
+  template <typename T>
+  __device__ GroupBuffer(const T *p, uint32_t groups)
+      : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(p), 0, int(groups * 16u), 0x00027000)) {}
+  template <int NT>
+  __device__ u32x4 load(uint32_t thread_bytes, uint32_t bytes) const {
+    return __builtin_amdgcn_raw_buffer_load_b128(rsrc, int(thread_bytes), int(bytes), (NT & kNtLoad) != 0 ? 2 : 0);
+  }
+  template <int NT>
+  __device__ void store(u32x4 v, uint32_t thread_bytes, uint32_t bytes) const {
+    __builtin_amdgcn_raw_buffer_store_b128(v, rsrc, int(thread_bytes), int(bytes), (NT & kNtStore) != 0 ? 18 : 0);
+    // A write to the data registers of such a store right behind it has changed the stored value here; the compiler, which
+    // keeps the distance after other stores of more than 8 bytes, takes none to be needed where the offset is scalar.
+    asm volatile("s_nop 1" ::"v"(v) : "memory");
+  }
+};
+
 // The values of group g; those that are not the row's are `fill` and are not read.
 template <typename T, int NT>
 __device__ inline void load_group(const RowGroups<T> &rg, const T *row, uint32_t g, float fill, float (&v)[Group<T>::W]) {
@@ -119,50 +140,81 @@ __device__ inline void load_group(const RowGroups<T> &rg, const T *row, uint32_t
   }
 }
 
-// A whole group to where the row has it, at any element.
-template <int ALIGN, typename V>
-__device__ inline void store_unaligned(void *p, V v) {
-  typedef V VU __attribute__((aligned(ALIGN)));
-  *reinterpret_cast<VU *>(p) = v;
+// A whole group to where the row has it; NT (kNtStore): past the caches, for groups that lie on 16-byte boundaries.
+template <int NT, int ALIGN, typename V>
+__device__ inline void store_group(void *p, V v) {
+  if constexpr ((NT & kNtStore) != 0) {
+    store_stream<NT>(static_cast<V *>(p), v);
+  } else {
+    typedef V VU __attribute__((aligned(ALIGN)));
+    *reinterpret_cast<VU *>(p) = v;
+  }
 }
 
-// Maximum m and sum s of exp2((x - m) * c) over what has been seen; c = log2(e) / temperature.  The difference is
-// taken before the product: values up to the type's largest and lowest neither overflow nor cancel.  Nothing seen,
-// or -inf only: m = -inf and s = 0.  A NaN is ignored by m and makes s NaN; so does +inf.
+// ---- statistics of a row: its maximum m and S = sum of exp((x - m) / T) = sum of exp2((x - m) * c) ----
+//
+// The fast form spends one fused multiply-add on a value's exponent: exp2(x * c - R) with R = fl(b * c) for a running
+// reference b >= the values seen.  R's rounding is a factor common to all terms, which row_stats() takes out again at the
+// end.  b starts at -limit, limit = 65536 / c: while it stays inside (-limit, limit) R is off by less than 2^-8 and
+// nothing overflows, whatever single values hold (-inf and the lowest value of a type add 0, a NaN shows in S).  A
+// row whose maximum lies outside -- nothing but -inf or a mask's lowest values, +inf, or values without measure --
+// is summed again in the plain form, exp2((x - m) * c).  Rows in earnest never do.
+struct Scale {
+  float c, limit;
+};
+static inline Scale scale_for(float temperature) {
+  const double c = 1.4426950408889634 / double(temperature);
+  const double limit = 65536.0 / c;
+  return Scale{float(c), float(limit < 1e38 ? limit : 1e38)};
+}
+
 struct SoftmaxSum {
   float m, s;
 };
-__device__ inline float exp_scaled(float x, float m, float c) { return __builtin_amdgcn_exp2f((x - m) * c); }
-// exp2((m - to) * c) with 0 for a sum that holds nothing yet
-__device__ inline float rescale(float m, float to, float c) { return m == kMinusInf ? 0.0f : exp_scaled(m, to, c); }
+
+// max(a, b, c) in one instruction; a NaN operand yields the others.  (fmaxf() costs two more instructions a value to
+// quiet signalling NaNs, which the maximum ignores here either way.)
+__device__ inline float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+template <int COUNT>
+__device__ inline float max_of(float m, const float (&v)[COUNT]) {
+  static_assert(COUNT % 2 == 0, "values are taken two at a time");
+#pragma unroll
+  for (int j = 0; j < COUNT; j += 2) m = max3(m, v[j], v[j + 1]);
+  return m;
+}
+
+
+// The fast form.
+template <int COUNT>
+__device__ inline void fold(SoftmaxSum &t, const float (&v)[COUNT], float c) {
+  const float m = max_of(t.m, v);
+  const float shift = m * c;
+  if (m > t.m) {
+    t.s *= __builtin_amdgcn_exp2f(t.m * c - shift);
+    t.m = m;
+  }
+  float s[2] = {0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < COUNT; ++j) s[j & 1] += __builtin_amdgcn_exp2f(fmaf(v[j], c, -shift));
+  t.s += s[0] + s[1];
+}
+__device__ inline void fold_one(SoftmaxSum &t, float x, float c) {
+  const float v[2] = {x, kMinusInf};
+  fold(t, v, c);
+}
 __device__ inline SoftmaxSum merge(SoftmaxSum a, SoftmaxSum b, float c) {
   SoftmaxSum r;
   r.m = fmaxf(a.m, b.m);
-  r.s = a.s * rescale(a.m, r.m, c) + b.s * rescale(b.m, r.m, c);
+  const float shift = r.m * c;
+  r.s = a.s * __builtin_amdgcn_exp2f(a.m * c - shift) + b.s * __builtin_amdgcn_exp2f(b.m * c - shift);
   return r;
 }
-
-// Folds `count` values into the running maximum and sum.
-template <int COUNT>
-__device__ inline void fold(SoftmaxSum &t, const float (&v)[COUNT], float c) {
-  float m = t.m;
-#pragma unroll
-  for (int j = 0; j < COUNT; ++j) m = fmaxf(m, v[j]);
-  if (m != t.m) {
-    t.s *= rescale(t.m, m, c);
-    t.m = m;
-  }
-  const float about = m == kMinusInf ? 0.0f : m;  // (-inf minus 0 stays -inf and adds nothing; a NaN still shows)
-  float s = 0.0f;
-#pragma unroll
-  for (int j = 0; j < COUNT; ++j) s += exp_scaled(v[j], about, c);
-  t.s += s;
-}
-
-// Every thread of the workgroup gets the merged maximum and sum, merged in a fixed order: butterflies in the wave, then
-// the waves in turn.  `lds` holds one entry a wave; the call ends with a barrier.
-template <int WAVES>
-__device__ inline SoftmaxSum block_merge(SoftmaxSum t, float c, SoftmaxSum *lds) {
+// The same in every lane of the wave, merged in a fixed order.
+__device__ inline SoftmaxSum wave_merge(SoftmaxSum t, float c) {
 #pragma unroll
   for (int off = kWave / 2; off > 0; off >>= 1) {
     SoftmaxSum o;
@@ -170,13 +222,170 @@ __device__ inline SoftmaxSum block_merge(SoftmaxSum t, float c, SoftmaxSum *lds)
     o.s = __shfl_xor(t.s, off, kWave);
     t = merge(t, o, c);
   }
-  if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = t;
-  __syncthreads();
-  t = lds[0];
+  return t;
+}
+// COUNT <= 16 entries in LDS merged, the same in every lane.
+template <int COUNT>
+__device__ inline SoftmaxSum lane_merge(const SoftmaxSum *lds, float c) {
+  static_assert(COUNT <= 16, "an entry a lane of a row of sixteen");
+  const uint32_t lane = threadIdx.x & 15u;
+  SoftmaxSum t = lds[lane < uint32_t(COUNT) ? lane : 0u];
+  if (lane >= uint32_t(COUNT)) t.s = 0.0f;  // (an entry again, of which nothing is added)
 #pragma unroll
-  for (int w = 1; w < WAVES; ++w) t = merge(t, lds[w], c);
+  for (int off = 8; off > 0; off >>= 1) {
+    SoftmaxSum o;
+    o.m = __shfl_xor(t.m, off, kWave);
+    o.s = __shfl_xor(t.s, off, kWave);
+    t = merge(t, o, c);
+  }
+  return t;
+}
+// The same in every thread of the workgroup; `lds` holds one entry a wave.  Ends with a barrier.
+template <int WAVES>
+__device__ inline SoftmaxSum block_merge(SoftmaxSum t, float c, SoftmaxSum *lds) {
+  t = wave_merge(t, c);
+  if constexpr (WAVES > 1) {
+    if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = t;
+    __syncthreads();
+    t = lane_merge<WAVES>(lds, c);
+  }
   __syncthreads();
   return t;
+}
+// Whether the fast form holds for a row of this maximum.
+__device__ inline bool measured(float m, Scale sc) { return fabsf(m) < sc.limit; }
+// The reference's rounding taken out: S about m itself.
+__device__ inline float true_sum(SoftmaxSum t, float c) { return t.s * __builtin_amdgcn_exp2f(fmaf(-t.m, c, t.m * c)); }
+
+// The plain form, for rows that the fast one does not measure: two passes, one value at a time.  -inf only (or
+// nothing): m = -inf, S = 0.  A NaN is ignored by m and makes S NaN; so does +inf.
+template <typename T, int THREADS>
+__device__ inline SoftmaxSum plain_stats(const T *row, uint32_t n, float c, float *lds) {
+  SoftmaxSum t = {kMinusInf, 0.0f};
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    const float about = t.m == kMinusInf ? 0.0f : t.m;
+    float v = pass == 0 ? kMinusInf : 0.0f;
+#pragma unroll 1
+    for (uint64_t i = threadIdx.x; i < n; i += THREADS) {
+      const float x = float(row[i]);
+      v = pass == 0 ? fmaxf(v, x) : v + __builtin_amdgcn_exp2f((x - about) * c);
+    }
+#pragma unroll 1
+    for (int off = kWave / 2; off > 0; off >>= 1) {
+      const float o = __shfl_xor(v, off, kWave);
+      v = pass == 0 ? fmaxf(v, o) : v + o;
+    }
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll 1
+    for (int w = 1; w < THREADS / kWave; ++w) v = pass == 0 ? fmaxf(v, lds[w]) : v + lds[w];
+    if (pass == 0) {
+      t.m = v;
+    } else {
+      t.s = v;
+    }
+  }
+  __syncthreads();
+  return t;
+}
+
+// A row, or a part of one, as it is streamed: `head` single values, `groups` 16-byte groups, `tail` single values.  The
+// single values are taken one a thread.  head = 0 for kernels that only read (a 16-byte load may start at any
+// element); a kernel that stores takes as many as bring its groups to a 128-byte line of the output.
+template <typename T>
+struct RowSpan {
+  static constexpr int W = Group<T>::W;
+  uint32_t head, groups, tail;
+  __device__ RowSpan(uint32_t n, uint32_t head_) : head(head_ < n ? head_ : n) {
+    groups = (n - head) / uint32_t(W);
+    tail = n - head - groups * uint32_t(W);
+  }
+  __device__ bool single(uint32_t thread) const { return thread < head + tail; }
+  // the place of the thread's single value; 0 (any place) for a thread that has none
+  __device__ uint32_t single_at(uint32_t thread) const {
+    return thread < head ? thread : single(thread) ? thread + groups * uint32_t(W) : 0u;
+  }
+  __device__ uint32_t first(uint32_t g) const { return head + g * uint32_t(W); }
+};
+
+// Values from the start of `p` to the next 128-byte line.
+template <typename T>
+__device__ inline uint32_t values_to_line(const T *p) {
+  return uint32_t((128u - (reinterpret_cast<uintptr_t>(p) & 127u)) & 127u) / uint32_t(sizeof(T));
+}
+
+// Makes the compiler forget what it knows of a group held in registers: values unpacked from it before would otherwise
+// be kept beside it until they are asked for again.
+__device__ inline void forget(u32x4 &q) { asm volatile("" : "+v"(q)); }
+
+// U groups of a thread: g, g + THREADS, ...  A group past the end reads the last one again (a branch round each load
+// would make every load wait for the one before); `inside` says which count.  There is at least one group.
+template <typename T, int THREADS, int U, int NT>
+__device__ inline void load_tile(const RowSpan<T> &span, const T *row, uint32_t g, u32x4 (&q)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t at = min(g + uint32_t(u) * uint32_t(THREADS), span.groups - 1u);
+    q[u] = load_stream<NT, int(sizeof(T))>(reinterpret_cast<const u32x4 *>(row + size_t(span.first(at))));
+  }
+}
+template <typename T, int U>
+__device__ inline void unpack_tile(const u32x4 (&q)[U], float (&v)[U * Group<T>::W]) {
+  constexpr int W = Group<T>::W;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float w[W];
+    unpack(q[u], w, static_cast<const T *>(nullptr));
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[u * W + j] = w[j];
+  }
+}
+template <typename T, int THREADS, int U>
+__device__ inline void mask_tile(const RowSpan<T> &span, uint32_t g, float fill, float (&v)[U * Group<T>::W]) {
+  constexpr int W = Group<T>::W;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const bool in = g + uint32_t(u) * uint32_t(THREADS) < span.groups;
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[u * W + j] = in ? v[u * W + j] : fill;
+  }
+}
+
+// A thread's running reference and sum over its part of a row (merge them with block_merge): tiles of U groups a thread,
+// the next tile on its way while one is folded.
+template <typename T, int THREADS, int U, int NT>
+__device__ inline SoftmaxSum stream_stats(const RowSpan<T> &span, const T *row, Scale sc) {
+  constexpr uint32_t kTile = uint32_t(THREADS) * uint32_t(U);
+  SoftmaxSum st = {-sc.limit, 0.0f};
+  // (the head can hold more values than a small workgroup has threads)
+  for (uint32_t i = threadIdx.x; span.single(i); i += THREADS) fold_one(st, float(row[span.single_at(i)]), sc.c);
+  if (span.groups != 0u) {
+    u32x4 q[U];
+    load_tile<T, THREADS, U, NT>(span, row, threadIdx.x, q);
+    for (uint32_t base = 0;; base += kTile) {
+      float v[U * Group<T>::W];
+      u32x4 next[U];
+      const bool more = span.groups - base > kTile;
+      if (more) load_tile<T, THREADS, U, NT>(span, row, base + kTile + threadIdx.x, next);
+      unpack_tile<T, U>(q, v);
+      if (!more) mask_tile<T, THREADS, U>(span, base + threadIdx.x, kMinusInf, v);
+      fold(st, v, sc.c);
+      if (!more) break;
+#pragma unroll
+      for (int u = 0; u < U; ++u) q[u] = next[u];
+    }
+  }
+  return st;
+}
+
+// A row's statistics from its threads' parts, by the whole workgroup.
+template <typename T, int THREADS>
+__device__ inline SoftmaxSum finish_stats(SoftmaxSum t, const T *row, uint32_t n, Scale sc, SoftmaxSum *lds) {
+  t = block_merge<THREADS / kWave>(t, sc.c, lds);
+  if (measured(t.m, sc)) return SoftmaxSum{t.m, true_sum(t, sc.c)};
+  return plain_stats<T, THREADS>(row, n, sc.c, reinterpret_cast<float *>(lds));
 }
 
 #endif  // __HIPCC__

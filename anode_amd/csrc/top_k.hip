@@ -59,7 +59,7 @@ __device__ inline void sort_entries(uint64_t *e, uint32_t size) {
 // One workgroup a row: the k-th largest key is found digit by digit (8 bits a pass over the row, counted in LDS), then
 // the larger ones are collected, and of those that equal it the first classes in order; the k entries are sorted.
 template <typename T>
-__global__ __launch_bounds__(kTopThreads) void top_k_radix_kernel(uint32_t n, uint32_t rows, size_t stride, uint32_t k, float c,
+__global__ __launch_bounds__(kTopThreads) void top_k_radix_kernel(uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc,
                                                                   double inv_t, const T *__restrict__ x, float *__restrict__ value,
                                                                   uint32_t *__restrict__ index, float *__restrict__ log_norm) {
   constexpr int W = Group<T>::W;
@@ -73,13 +73,8 @@ __global__ __launch_bounds__(kTopThreads) void top_k_radix_kernel(uint32_t n, ui
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T *xr = x + r * stride;
     if (log_norm != nullptr) {
-      SoftmaxSum st = {kMinusInf, 0.0f};
-      for (uint32_t g = threadIdx.x; g < rg.groups; g += kTopThreads) {
-        float v[W];
-        load_group<T, 0>(rg, xr, g, kMinusInf, v);
-        fold(st, v, c);
-      }
-      st = block_merge<kTopWaves>(st, c, lds);
+      const SoftmaxSum st = finish_stats<T, kTopThreads>(
+          stream_stats<T, kTopThreads, 4, 0>(RowSpan<T>(n, 0u), xr, sc), xr, n, sc, lds);
       if (threadIdx.x == 0) log_norm[r] = float(double(st.m) * inv_t + log(double(st.s)));
     }
     uint32_t prefix = 0u, known = 0u, need = k;
@@ -205,8 +200,7 @@ int top_k(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, uin
   if (k != 0u && (value == nullptr || index == nullptr)) return refuse(symbol, "an array is missing");
   const uint32_t grid = dim1 < (1u << 24) ? dim1 : (1u << 24);
   top_k_radix_kernel<T><<<grid, kTopThreads, 0, as_stream(stream)>>>(
-      dim0, dim1, size_t(stride != 0u ? stride : dim0), k, float(1.4426950408889634 / double(temperature)),
-      1.0 / double(temperature), x, value, index, log_norm);
+      dim0, dim1, size_t(stride != 0u ? stride : dim0), k, scale_for(temperature), 1.0 / double(temperature), x, value, index, log_norm);
   note_launch(symbol);
   return 0;
 }

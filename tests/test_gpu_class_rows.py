@@ -197,11 +197,11 @@ def test_top_k_of_one_is_arg_max():
 # ---- distillation ----
 
 
-def run_distill(kind, x, value, index, t, dy, log_norm, mode, stride=0, offset=0, in_place=False, old=None):
+def run_distill(kind, x, value, index, t, dy, log_norm, mode, stride=0, offset=0, in_place=False, old=None, apart=0):
     """loss, row_max, row_sum, dx of one of the ways to get them."""
     rows, n = x.shape
     k = value.shape[1]
-    xd = Rows(x, kind, stride, offset)
+    xd = Rows(x, kind, stride, offset + apart)
     tv, ti = dev(value) if value.size else torch.zeros(1, device="cuda"), u32(index) if index.size else torch.zeros(
         1, dtype=torch.int32, device="cuda")
     tn = None if log_norm is None else dev(np.asarray(log_norm, F32))
@@ -229,11 +229,11 @@ def run_distill(kind, x, value, index, t, dy, log_norm, mode, stride=0, offset=0
     return host(loss[0]), host(top[0]), host(total[0]), dx.get()
 
 
-def check_distill(kind, x, value, index, t, dy, log_norm, mode, stride=0, offset=0, in_place=False, what=""):
+def check_distill(kind, x, value, index, t, dy, log_norm, mode, stride=0, offset=0, in_place=False, what="", apart=0):
     rows, n = x.shape
     t = float(F32(t))  # the entry point's argument has 32 bits
     old = rounded(np.random.default_rng(9).standard_normal((rows, n)), kind) if mode == "accumulate" else None
-    loss, top, total, dx = run_distill(kind, x, value, index, t, dy, log_norm, mode, stride, offset, in_place, old)
+    loss, top, total, dx = run_distill(kind, x, value, index, t, dy, log_norm, mode, stride, offset, in_place, old, apart)
     want_loss, want_top, want_total = ref.distill(x, value, index, t, log_norm)
     want_dx, q, p = ref.distill_grad(x, value, index, t, dy, log_norm)
     assert np.array_equal(top.astype(np.float64), want_top), what
@@ -283,6 +283,17 @@ def check_distill(kind, x, value, index, t, dy, log_norm, mode, stride=0, offset
         good = np.where(np.abs(want) + bound >= edge, good | (dx[r] == np.copysign(np.inf, want)), good)
         bad = np.flatnonzero(~good)
         assert bad.size == 0, (where, bad[:5], dx[r][bad[:5]], want[bad[:5]], bound[bad[:5]])
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("apart", [1, 2, 5])
+def test_distill_of_arrays_that_lie_unlike_each_other(kind, apart):
+    g = np.random.default_rng(apart)
+    for n in (130, 9001):
+        x = logits(g, 5, n, kind)
+        value, index = slots(g, 5, n, 9)
+        for mode in ("fused", "apart", "accumulate"):
+            check_distill(kind, x, value, index, 1.0, g.standard_normal(5).astype(F32), None, mode, n + 3, 1, what="unlike", apart=apart)
 
 
 SHAPES = [(1, 3, 1), (2, 5, 3), (7, 4, 7), (8, 3, 2), (9, 2, 9), (63, 5, 10), (255, 3, 64), (257, 2, 0), (1000, 40, 10), (1000, 2, 700),
