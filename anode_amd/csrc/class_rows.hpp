@@ -172,21 +172,21 @@ struct SoftmaxSum {
   float m, s;
 };
 
-// max(a, b, c) in one instruction; a NaN operand yields the others.  (fmaxf() costs two more instructions a value to
-// quiet signalling NaNs, which the maximum ignores here either way.)
-__device__ inline float max3(float a, float b, float c) {
-  float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
-  return r;
-}
+// The largest of m and the values, two values an instruction; a NaN is passed over.  (fmaxf() costs two more instructions a
+// value to quiet signalling NaNs, which the maximum ignores here either way.)
 template <int COUNT>
 __device__ inline float max_of(float m, const float (&v)[COUNT]) {
-  static_assert(COUNT % 2 == 0, "values are taken two at a time");
+  static_assert(COUNT == 2 || COUNT % 4 == 0, "values are taken four at a time");
+  if constexpr (COUNT == 2) {
+    asm("v_max3_f32 %0, %0, %1, %2" : "+v"(m) : "v"(v[0]), "v"(v[1]));
+  } else {
 #pragma unroll
-  for (int j = 0; j < COUNT; j += 2) m = max3(m, v[j], v[j + 1]);
+    for (int j = 0; j < COUNT; j += 4) {
+      asm("v_max3_f32 %0, %0, %1, %2\n\tv_max3_f32 %0, %0, %3, %4" : "+v"(m) : "v"(v[j]), "v"(v[j + 1]), "v"(v[j + 2]), "v"(v[j + 3]));
+    }
+  }
   return m;
 }
-
 
 // The fast form.
 template <int COUNT>
@@ -322,7 +322,8 @@ __device__ inline uint32_t values_to_line(const T *p) {
 __device__ inline void forget(u32x4 &q) { asm volatile("" : "+v"(q)); }
 
 // U groups of a thread: g, g + THREADS, ...  A group past the end reads the last one again (a branch round each load
-// would make every load wait for the one before); `inside` says which count.  There is at least one group.
+// would make every load wait for the one before, and a tile that is fetched ahead in a branch is waited for at its end: so
+// the tile behind the last is fetched too).  There is at least one group.
 template <typename T, int THREADS, int U, int NT>
 __device__ inline void load_tile(const RowSpan<T> &span, const T *row, uint32_t g, u32x4 (&q)[U]) {
 #pragma unroll
@@ -368,7 +369,7 @@ __device__ inline SoftmaxSum stream_stats(const RowSpan<T> &span, const T *row, 
       float v[U * Group<T>::W];
       u32x4 next[U];
       const bool more = span.groups - base > kTile;
-      if (more) load_tile<T, THREADS, U, NT>(span, row, base + kTile + threadIdx.x, next);
+      load_tile<T, THREADS, U, NT>(span, row, base + kTile + threadIdx.x, next);
       unpack_tile<T, U>(q, v);
       if (!more) mask_tile<T, THREADS, U>(span, base + threadIdx.x, kMinusInf, v);
       fold(st, v, sc.c);

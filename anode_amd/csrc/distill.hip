@@ -288,7 +288,7 @@ __device__ inline void stream_groups(const RowSpan<T> &span, const T *x, T *dx, 
     u32x4 old[U], next[U];
     const bool more = span.groups - base > kTile;
     if (ACC) load_tile<T, THREADS, U, 0>(span, dx, g, old);
-    if (more) load_tile<T, THREADS, U, 0>(span, x, g + kTile, next);
+    load_tile<T, THREADS, U, 0>(span, x, g + kTile, next);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float v[W], o[W];

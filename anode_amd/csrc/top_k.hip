@@ -7,14 +7,12 @@
 namespace anode {
 namespace {
 
-constexpr int kTopThreads = 512;
-constexpr int kTopWaves = kTopThreads / kWave;
-
 // A value as an unsigned number in the same order, -0 as +0; 0 for what is never taken (NaN, -inf).
+constexpr uint32_t kLowestKey = 0x00800000u;  // the lowest finite value's
 __device__ inline uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.0f);
   const uint32_t key = (b & 0x80000000u) != 0u ? ~b : b | 0x80000000u;
-  return (key <= 0x007fffffu || key > 0xff800000u) ? 0u : key;
+  return (key < kLowestKey || key > 0xff800000u) ? 0u : key;
 }
 __device__ inline float value_of(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) != 0u ? key ^ 0x80000000u : ~key);
@@ -35,160 +33,418 @@ struct KeyBits<f16_t> {
 };
 
 // An entry: key above, the class inverted below, so that the larger entry comes first in the order of the result.
+// Entries of a row are all different.
 __device__ inline uint64_t entry_of(uint32_t key, uint32_t k) { return (uint64_t(key) << 32) | uint32_t(~k); }
+__device__ inline uint32_t key_in(uint64_t entry) { return uint32_t(entry >> 32); }
 
-// Sorts the first `size` (a power of two) entries in LDS, largest first.
+// Sorts the first `size` (a power of two) entries in LDS, largest first.  Up to 128 of them one wave does it, without
+// barriers in between.
 template <int THREADS>
 __device__ inline void sort_entries(uint64_t *e, uint32_t size) {
-  for (uint32_t run = 2; run <= size; run <<= 1) {
-    for (uint32_t step = run >> 1; step > 0; step >>= 1) {
-      __syncthreads();
-      for (uint32_t i = threadIdx.x; i < size / 2; i += THREADS) {
-        const uint32_t lo = 2u * i - (i & (step - 1u)), hi = lo + step;
-        const uint64_t a = e[lo], b = e[hi];
-        if (((lo & run) == 0u) == (a < b)) {
-          e[lo] = b;
-          e[hi] = a;
+  auto exchange = [&](uint32_t i, uint32_t run, uint32_t step) {
+    const uint32_t lo = 2u * i - (i & (step - 1u)), hi = lo + step;
+    const uint64_t a = e[lo], b = e[hi];
+    if (((lo & run) == 0u) == (a < b)) {
+      e[lo] = b;
+      e[hi] = a;
+    }
+  };
+  __syncthreads();
+  if (size <= 2u * uint32_t(kWave)) {
+    if (threadIdx.x < uint32_t(kWave)) {
+      for (uint32_t run = 2; run <= size; run <<= 1) {
+        for (uint32_t step = run >> 1; step > 0; step >>= 1) {
+          if (threadIdx.x < size / 2u) exchange(threadIdx.x, run, step);
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
         }
+      }
+    }
+  } else {
+    for (uint32_t run = 2; run <= size; run <<= 1) {
+      for (uint32_t step = run >> 1; step > 0; step >>= 1) {
+        for (uint32_t i = threadIdx.x; i < size / 2u; i += THREADS) exchange(i, run, step);
+        __syncthreads();
       }
     }
   }
   __syncthreads();
 }
 
-// One workgroup a row: the k-th largest key is found digit by digit (8 bits a pass over the row, counted in LDS), then
-// the larger ones are collected, and of those that equal it the first classes in order; the k entries are sorted.
-template <typename T>
-__global__ __launch_bounds__(kTopThreads) void top_k_radix_kernel(uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc,
-                                                                  double inv_t, const T *__restrict__ x, float *__restrict__ value,
-                                                                  uint32_t *__restrict__ index, float *__restrict__ log_norm) {
+// Inclusive sum over the lanes up to this one.
+__device__ inline uint32_t wave_upto(uint32_t v) {
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const uint32_t o = __shfl_up(v, off, kWave);
+    if (int(lane) >= off) v += o;
+  }
+  return v;
+}
+
+// A key that at least j lanes reach, found bit by bit (its leading 18 bits; those below are 0): 0 where fewer lanes hold a
+// key at all.  The comparisons' results are scalar, so a step is a compare, a count and a select.
+__device__ inline uint32_t key_reached_by(uint32_t key, uint32_t j) {
+  uint32_t t = 0u;
+#pragma unroll
+  for (int bit = 31; bit >= 14; --bit) {
+    const uint32_t higher = t | (1u << bit);
+    if (uint32_t(__popcll(__ballot(key >= higher))) >= j) t = higher;
+  }
+  return t;
+}
+
+// What the exact selection of k entries needs in LDS.
+struct RadixLds {
+  uint32_t digits[256];
+  uint32_t wave_count[16];
+  uint32_t found, above, taken;
+};
+
+// The k largest entries of a row, or all of them where there are fewer, unsorted into `entries`; returns how many.  Exact
+// whatever the row holds: the k-th largest key is found digit by digit (8 bits a pass over the row, counted in LDS), the larger
+// ones are collected, and of those that equal it the first classes in order.
+template <typename T, int THREADS>
+__device__ inline uint32_t radix_select(const T *xr, uint32_t n, uint32_t from, uint32_t k, uint64_t *entries, RadixLds &l) {
   constexpr int W = Group<T>::W;
-  __shared__ uint64_t entries[kMaxSlots];
-  __shared__ uint32_t digits[256];
-  __shared__ uint32_t found, above, taken;
-  __shared__ uint32_t wave_count[kTopWaves];
-  __shared__ SoftmaxSum lds[kTopWaves];
+  constexpr int WAVES = THREADS / kWave;
   const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const RowGroups<T> rg(n, 0u);
-  for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const T *xr = x + r * stride;
-    if (log_norm != nullptr) {
-      const SoftmaxSum st = finish_stats<T, kTopThreads>(
-          stream_stats<T, kTopThreads, 4, 0>(RowSpan<T>(n, 0u), xr, sc), xr, n, sc, lds);
-      if (threadIdx.x == 0) log_norm[r] = float(double(st.m) * inv_t + log(double(st.s)));
-    }
-    uint32_t prefix = 0u, known = 0u, need = k;
-    bool all = k == 0u;  // the row holds no more than k values that may be taken (or nothing is asked for)
-    for (int shift = 24; shift >= 32 - KeyBits<T>::value && !all; shift -= 8) {
-      for (uint32_t i = threadIdx.x; i < 256u; i += kTopThreads) digits[i] = 0u;
-      __syncthreads();
-      for (uint32_t g = threadIdx.x; g < rg.groups; g += kTopThreads) {
-        float v[W];
-        load_group<T, 0>(rg, xr, g, kMinusInf, v);
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const uint32_t key = key_of(v[j]);
-          if (key != 0u && (key & known) == prefix) atomicAdd(&digits[(key >> shift) & 255u], 1u);
-        }
-      }
-      __syncthreads();
-      if (wave == 0) {  // lane l sums the digits 255 - 4 l ... 252 - 4 l, largest first
-        uint32_t d[4], own = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) own += d[i] = digits[255u - 4u * lane - uint32_t(i)];
-        uint32_t upto = own;
-#pragma unroll
-        for (int off = 1; off < kWave; off <<= 1) {
-          const uint32_t o = __shfl_up(upto, off, kWave);
-          if (int(lane) >= off) upto += o;
-        }
-        if (lane == 0) found = 256u;
-        uint32_t run = upto - own;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (run < need && run + d[i] >= need) {
-            found = 255u - 4u * lane - uint32_t(i);
-            above = run;
-          }
-          run += d[i];
-        }
-      }
-      __syncthreads();
-      if (found == 256u) {
-        all = true;  // (only the first pass can find too few)
-      } else {
-        need -= above;
-        prefix |= found << shift;
-        known |= 255u << shift;
-      }
-      __syncthreads();
-    }
-    // the k-th largest key; below the digits looked at a key repeats its sign bit, inverted
-    uint32_t kth = prefix | ((prefix & 0x80000000u) != 0u ? 0u : ~known);
-    if (all) kth = 0u;
-    if (threadIdx.x == 0) taken = 0u;
+  if (k == 0u) return 0u;
+  uint32_t prefix = 0u, known = 0u, need = k;
+  bool all = false;  // the row holds fewer than k values that may be taken
+  for (int shift = 24; shift >= 32 - KeyBits<T>::value && !all; shift -= 8) {
+    for (uint32_t i = threadIdx.x; i < 256u; i += THREADS) l.digits[i] = 0u;
     __syncthreads();
-    if (k != 0u) {
-      for (uint32_t g = threadIdx.x; g < rg.groups; g += kTopThreads) {
-        float v[W];
-        load_group<T, 0>(rg, xr, g, kMinusInf, v);
+    for (uint32_t g = threadIdx.x; g < rg.groups; g += THREADS) {
+      float v[W];
+      load_group<T, 0>(rg, xr, g, kMinusInf, v);
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-          const uint32_t key = key_of(v[j]);
-          if (key > kth) entries[atomicAdd(&taken, 1u)] = entry_of(key, rg.first(g) + uint32_t(j));
-        }
+      for (int j = 0; j < W; ++j) {
+        const uint32_t key = key_of(v[j]);
+        if (key != 0u && (key & known) == prefix) atomicAdd(&l.digits[(key >> shift) & 255u], 1u);
       }
     }
     __syncthreads();
-    uint32_t count = taken;
-    if (!all) {
-      // the first `need` classes whose key is the k-th: a workgroup's groups in turn, counted across its threads
-      uint32_t before = 0u;
-      for (uint32_t base = 0; base < rg.groups && before < need; base += kTopThreads) {
-        const uint32_t g = base + threadIdx.x;
-        uint32_t same = 0u;
-        if (g < rg.groups) {
-          float v[W];
-          load_group<T, 0>(rg, xr, g, kMinusInf, v);
+    if (wave == 0) {  // lane i sums the digits 255 - 4 i ... 252 - 4 i, largest first
+      uint32_t d[4], own = 0u;
 #pragma unroll
-          for (int j = 0; j < W; ++j) same |= uint32_t(key_of(v[j]) == kth) << j;
-        }
-        const uint32_t own = uint32_t(__popc(same));
-        uint32_t upto = own;
+      for (int i = 0; i < 4; ++i) own += d[i] = l.digits[255u - 4u * lane - uint32_t(i)];
+      uint32_t run = wave_upto(own) - own;
+      if (lane == 0) l.found = 256u;
 #pragma unroll
-        for (int off = 1; off < kWave; off <<= 1) {
-          const uint32_t o = __shfl_up(upto, off, kWave);
-          if (int(lane) >= off) upto += o;
+      for (int i = 0; i < 4; ++i) {
+        if (run < need && run + d[i] >= need) {
+          l.found = 255u - 4u * lane - uint32_t(i);
+          l.above = run;
         }
-        if (lane == kWave - 1) wave_count[wave] = upto;
-        __syncthreads();
-        uint32_t at = before + upto - own, total = 0u;
-#pragma unroll
-        for (int w = 0; w < kTopWaves; ++w) {
-          if (uint32_t(w) < wave) at += wave_count[w];
-          total += wave_count[w];
-        }
-        while (same != 0u && at < need) {
-          const uint32_t j = uint32_t(__ffs(int(same))) - 1u;
-          same &= same - 1u;
-          entries[count + at++] = entry_of(kth, rg.first(g) + j);
-        }
-        before += total;
-        __syncthreads();
+        run += d[i];
       }
-      count += need;
     }
-    uint32_t size = 2u;
-    while (size < count) size <<= 1;
-    for (uint32_t i = count + threadIdx.x; i < size; i += kTopThreads) entries[i] = 0u;
-    sort_entries<kTopThreads>(entries, size);
-    for (uint32_t i = threadIdx.x; i < k; i += kTopThreads) {
-      const bool have = i < count;
-      value[r * k + i] = have ? value_of(uint32_t(entries[i] >> 32)) : kMinusInf;
-      index[r * k + i] = have ? ~uint32_t(entries[i]) : kNoClass;
+    __syncthreads();
+    if (l.found == 256u) {
+      all = true;  // (only the first pass can find too few)
+    } else {
+      need -= l.above;
+      prefix |= l.found << shift;
+      known |= 255u << shift;
     }
     __syncthreads();
   }
+  // the k-th largest key; below the digits looked at a key repeats its sign bit, inverted
+  const uint32_t kth = all ? 0u : prefix | ((prefix & 0x80000000u) != 0u ? 0u : ~known);
+  if (threadIdx.x == 0) l.taken = 0u;
+  __syncthreads();
+  for (uint32_t g = threadIdx.x; g < rg.groups; g += THREADS) {
+    float v[W];
+    load_group<T, 0>(rg, xr, g, kMinusInf, v);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const uint32_t key = key_of(v[j]);
+      if (key > kth) entries[atomicAdd(&l.taken, 1u)] = entry_of(key, from + rg.first(g) + uint32_t(j));
+    }
+  }
+  __syncthreads();
+  const uint32_t count = l.taken;
+  if (all) return count;
+  // the first `need` classes whose key is the k-th: the workgroup's groups in turn, counted across its threads
+  uint32_t before = 0u;
+  for (uint32_t base = 0; base < rg.groups && before < need; base += THREADS) {
+    const uint32_t g = base + threadIdx.x;
+    uint32_t same = 0u;
+    if (g < rg.groups) {
+      float v[W];
+      load_group<T, 0>(rg, xr, g, kMinusInf, v);
+#pragma unroll
+      for (int j = 0; j < W; ++j) same |= uint32_t(key_of(v[j]) == kth) << j;
+    }
+    const uint32_t own = uint32_t(__popc(same));
+    const uint32_t upto = wave_upto(own);
+    if (lane == kWave - 1) l.wave_count[wave] = upto;
+    __syncthreads();
+    uint32_t at = before + upto - own, total = 0u;
+    for (int w = 0; w < WAVES; ++w) {
+      if (uint32_t(w) < wave) at += l.wave_count[w];
+      total += l.wave_count[w];
+    }
+    while (same != 0u && at < need) {
+      const uint32_t j = uint32_t(__ffs(int(same))) - 1u;
+      same &= same - 1u;
+      entries[count + at++] = entry_of(kth, from + rg.first(g) + j);
+    }
+    before += total;
+    __syncthreads();
+  }
+  return count + need;
+}
+
+// The entries in LDS that can be among the k largest, to `out` (room for `most`): those that reach a key which k of them
+// reach, and few more.  Returns their number, which may be above `most` (then `out` is incomplete).
+template <int THREADS>
+__device__ inline uint32_t drop_small(const uint64_t *entries, uint32_t count, uint32_t k, uint64_t *out, uint32_t most,
+                                      uint32_t *wave_key, uint32_t *taken) {
+  constexpr uint32_t WAVES = THREADS / kWave;
+  uint32_t top = 0u;
+  for (uint32_t i = threadIdx.x; i < count; i += THREADS) top = max(top, key_in(entries[i]));
+  const uint32_t t = key_reached_by(top, (k + WAVES - 1u) / WAVES);
+  if ((threadIdx.x & (kWave - 1)) == 0) wave_key[threadIdx.x / kWave] = t;
+  if (threadIdx.x == 0) *taken = 0u;
+  __syncthreads();
+  uint32_t least = wave_key[0];
+#pragma unroll
+  for (uint32_t w = 1; w < WAVES; ++w) least = min(least, wave_key[w]);
+  for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
+    const uint64_t e = entries[i];
+    if (key_in(e) >= least) {
+      const uint32_t at = atomicAdd(taken, 1u);
+      if (at < most) out[at] = e;
+    }
+  }
+  __syncthreads();
+  return *taken;
+}
+
+// The result of a row from its entries in LDS, at least the k largest of them: sorted, and empty slots behind.
+template <int THREADS>
+__device__ inline void write_result(uint64_t *entries, uint32_t count, size_t row, uint32_t k, float *value, uint32_t *index) {
+  uint32_t size = 2u;
+  while (size < count) size <<= 1;
+  for (uint32_t i = count + threadIdx.x; i < size; i += THREADS) entries[i] = 0u;
+  sort_entries<THREADS>(entries, size);
+  for (uint32_t i = threadIdx.x; i < k; i += THREADS) {
+    const bool have = i < count;
+    value[row * k + i] = have ? value_of(key_in(entries[i])) : kMinusInf;
+    index[row * k + i] = have ? ~uint32_t(entries[i]) : kNoClass;
+  }
+}
+
+// A part of a row: rows are cut into `parts` of `per` values where there are too few to fill the GPU.
+struct Cut {
+  uint32_t parts, per;
+};
+
+// What the parts of a row leave for the kernel that joins them.
+struct PartResults {
+  uint64_t *entries;  // [quota, parts, rows]
+  uint32_t *count;    // [parts, rows]
+  SoftmaxSum *stats;  // [parts, rows]
+  uint32_t quota;
+};
+
+// One workgroup a part of a row, which it reads once.  A threshold that k values seen so far reach -- every wave finds what its
+// share of k reaches among the largest value of each of its lanes, the least of the waves counts -- is renewed after 1, 2, 4,
+// 8 ... tiles; values that reach it are put into a list in LDS, which grows by little more than k between two renewals, whatever
+// the row's length.  What the list holds at the end is thinned the same way, sorted and written.  Rows for which the list
+// is too short (thousands of ties at the border, the largest values all in few lanes' places) are selected
+// exactly, in more passes.
+template <typename T, int THREADS, int LIST, bool NORM, int NT>
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(NORM ? 6 : 8))) void top_k_kernel(uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc,
+                                                        double inv_t, Cut cut, const T *__restrict__ x,
+                                                        float *__restrict__ value, uint32_t *__restrict__ index,
+                                                        float *__restrict__ log_norm, PartResults pr) {
+  constexpr int W = Group<T>::W;
+  constexpr int U = 16 / W;  // 16 values of a thread together
+  constexpr uint32_t WAVES = THREADS / kWave;
+  constexpr uint32_t kTile = uint32_t(THREADS) * uint32_t(U);
+  constexpr uint32_t kShort = 2u * uint32_t(THREADS);
+  __shared__ uint64_t list[LIST];
+  __shared__ uint64_t best[kShort];
+  __shared__ RadixLds radix;
+  __shared__ uint32_t wave_key[2][WAVES];
+  __shared__ uint32_t listed, taken;
+  __shared__ SoftmaxSum sums[WAVES];
+  const uint32_t wave = threadIdx.x / kWave;
+  const uint32_t share = (k + WAVES - 1u) / WAVES;
+  const uint64_t items = uint64_t(rows) * cut.parts;
+  for (uint64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const size_t r = item / cut.parts;
+    const uint32_t from = uint32_t(item % cut.parts) * cut.per;
+    const uint32_t count = min(cut.per, n - from);
+    const T *xr = x + r * stride + from;
+    const RowSpan<T> span(count, 0u);
+    if (threadIdx.x == 0) listed = 0u;
+    __syncthreads();
+    float top = kMinusInf, least = -__FLT_MAX__;
+    SoftmaxSum st = {-sc.limit, 0.0f};
+    auto put = [&](float v, uint32_t at) {
+      if (v >= least) {
+        const uint32_t place = atomicAdd(&listed, 1u);
+        if (place < uint32_t(LIST)) list[place] = entry_of(key_of(v), from + at);
+      }
+    };
+    if (span.groups != 0u) {
+      u32x4 q[U];
+      load_tile<T, THREADS, U, NT>(span, xr, threadIdx.x, q);
+      uint32_t tile = 0u, turn = 0u;
+      for (uint32_t base = 0;; base += kTile, ++tile) {
+        float v[U * W];
+        u32x4 next[U];
+        const bool more = span.groups - base > kTile;
+        load_tile<T, THREADS, U, NT>(span, xr, base + kTile + threadIdx.x, next);
+        unpack_tile<T, U>(q, v);
+        if (!more) mask_tile<T, THREADS, U>(span, base + threadIdx.x, kMinusInf, v);
+        const float tile_top = max_of(kMinusInf, v);
+        top = fmaxf(top, tile_top);
+        if ((tile & (tile - 1u)) == 0u) {
+          const uint32_t t = key_reached_by(key_of(top), share);
+          uint32_t *keys = wave_key[turn];  // (the other half may still be read)
+          turn ^= 1u;
+          if ((threadIdx.x & (kWave - 1)) == 0) keys[wave] = t;
+          __syncthreads();
+          uint32_t low = keys[0];
+#pragma unroll
+          for (uint32_t w = 1; w < WAVES; ++w) low = min(low, keys[w]);
+          least = low < kLowestKey ? -__FLT_MAX__ : value_of(low);
+        }
+        if (tile_top >= least) {  // (rare: the values are marked and fetched again, which costs no registers here)
+          uint32_t marked = 0u;
+#pragma unroll
+          for (int i = 0; i < U * W; ++i) marked |= uint32_t(v[i] >= least) << i;
+          do {
+            const uint32_t i = uint32_t(__ffs(int(marked))) - 1u;
+            marked &= marked - 1u;
+            const uint32_t at = span.first(base + threadIdx.x + i / uint32_t(W) * uint32_t(THREADS)) + i % uint32_t(W);
+            put(float(xr[at]), at);
+          } while (marked != 0u);
+        }
+        if constexpr (NORM) fold(st, v, sc.c);
+        if (!more) break;
+#pragma unroll
+        for (int u = 0; u < U; ++u) q[u] = next[u];
+      }
+    }
+    if (span.single(threadIdx.x)) {  // (at most 7: the head is empty)
+      const uint32_t at = span.single_at(threadIdx.x);
+      const float v = float(xr[at]);
+      put(v, at);
+      if constexpr (NORM) fold_one(st, v, sc.c);
+    }
+    __syncthreads();
+    uint64_t *found = best;
+    uint32_t have = listed;
+    if (have <= uint32_t(LIST)) have = drop_small<THREADS>(list, have, k, best, kShort, wave_key[0], &taken);
+    if (have > kShort || (cut.parts > 1u && have > pr.quota)) {
+      __syncthreads();
+      have = radix_select<T, THREADS>(xr, count, from, k, list, radix);
+      found = list;
+      __syncthreads();
+    }
+    if (cut.parts == 1u) {
+      write_result<THREADS>(found, have, r, k, value, index);
+      if constexpr (NORM) {
+        st = finish_stats<T, THREADS>(st, xr, n, sc, sums);
+        if (threadIdx.x == 0) log_norm[r] = float(double(st.m) * inv_t + log(double(st.s)));
+      }
+    } else {
+      for (uint32_t i = threadIdx.x; i < have; i += THREADS) pr.entries[item * pr.quota + i] = found[i];
+      if (threadIdx.x == 0) pr.count[item] = have;
+      if constexpr (NORM) {
+        st = block_merge<WAVES>(st, sc.c, sums);
+        if (threadIdx.x == 0) pr.stats[item] = st;
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// One workgroup a row: its parts' entries together, thinned, sorted and written.
+constexpr uint32_t kJoined = 4096;  // entries of a row's parts at most
+template <typename T, bool NORM>
+__global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc,
+                                                            double inv_t, uint32_t parts, const T *__restrict__ x,
+                                                            float *__restrict__ value, uint32_t *__restrict__ index,
+                                                            float *__restrict__ log_norm, PartResults pr) {
+  constexpr uint32_t kShort = 2048;
+  __shared__ uint64_t list[kJoined];
+  __shared__ uint64_t best[kShort];
+  __shared__ uint32_t wave_key[kBlock / kWave];
+  __shared__ uint32_t taken;
+  __shared__ float plain_lds[kBlock / kWave];
+  for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    uint32_t have = 0u;
+    for (uint32_t p = 0; p < parts; ++p) {
+      const size_t item = r * parts + p;
+      const uint32_t count = pr.count[item];
+      for (uint32_t i = threadIdx.x; i < count; i += kBlock) list[have + i] = pr.entries[item * pr.quota + i];
+      have += count;
+    }
+    __syncthreads();
+    const uint32_t few = drop_small<kBlock>(list, have, k, best, kShort, wave_key, &taken);
+    if (few <= kShort) {
+      write_result<kBlock>(best, few, r, k, value, index);
+    } else {
+      write_result<kBlock>(list, have, r, k, value, index);
+    }
+    if constexpr (NORM) {
+      SoftmaxSum st = {-sc.limit, 0.0f};
+      for (uint32_t i = threadIdx.x & (kWave - 1); i < parts; i += kWave) st = merge(st, pr.stats[r * parts + i], sc.c);
+      st = wave_merge(st, sc.c);
+      if (measured(st.m, sc)) {
+        st.s = true_sum(st, sc.c);
+      } else {
+        st = plain_stats<T, kBlock>(x + r * stride, n, sc.c, plain_lds);
+      }
+      if (threadIdx.x == 0) log_norm[r] = float(double(st.m) * inv_t + log(double(st.s)));
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, int THREADS, int LIST, bool NORM>
+int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, uint32_t k, float temperature, const T *x,
+                 float *value, uint32_t *index, float *log_norm, hipStream_t st) {
+  // parts of at least 4096 values, that bring the launch to eight waves a SIMD
+  const uint32_t target = uint32_t(device_cu_count()) * (2048u / uint32_t(THREADS));
+  uint64_t parts = (uint64_t(target) + rows - 1u) / rows;
+  if (parts > n / 4096u) parts = n / 4096u;
+  if (parts > 64u) parts = 64u;
+  if (k != 0u && parts > kJoined / k) parts = kJoined / k;
+  Cut cut = {1u, n};
+  if (parts > 1u) {
+    const uint64_t per = ((uint64_t(n) + parts - 1u) / parts + 1023u) / 1024u * 1024u;
+    cut = Cut{uint32_t((n + per - 1u) / per), uint32_t(per)};
+  }
+  const uint64_t items = uint64_t(rows) * cut.parts;
+  const uint32_t grid = items < (1u << 24) ? uint32_t(items) : (1u << 24);
+  const Scale sc = scale_for(temperature);
+  const double inv_t = 1.0 / double(temperature);
+  PartResults pr = {nullptr, nullptr, nullptr, kJoined / cut.parts};
+  if (cut.parts == 1u) {
+    top_k_kernel<T, THREADS, LIST, NORM, 0><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
+  } else {
+    const size_t entry_bytes = size_t(items) * pr.quota * sizeof(uint64_t), stat_bytes = size_t(items) * sizeof(SoftmaxSum);
+    ScratchLease scratch = acquire_scratch(st, entry_bytes + stat_bytes + size_t(items) * sizeof(uint32_t), symbol);
+    if (!scratch.ptr) return int(hipErrorOutOfMemory);
+    char *at = static_cast<char *>(scratch.ptr);
+    pr.entries = reinterpret_cast<uint64_t *>(at);
+    pr.stats = reinterpret_cast<SoftmaxSum *>(at + entry_bytes);
+    pr.count = reinterpret_cast<uint32_t *>(at + entry_bytes + stat_bytes);
+    top_k_kernel<T, THREADS, LIST, NORM, 0><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
+    top_k_join_kernel<T, NORM><<<rows < (1u << 24) ? rows : (1u << 24), kBlock, 0, st>>>(n, rows, stride, k, sc, inv_t, cut.parts, x,
+                                                                                       value, index, log_norm, pr);
+  }
+  note_launch(symbol);
+  return 0;
 }
 
 template <typename T>
@@ -198,11 +454,17 @@ int top_k(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, uin
   if (dim1 == 0u || (k == 0u && log_norm == nullptr)) return 0;
   if (dim0 != 0u && (x == nullptr || misaligned(x))) return refuse(symbol, "the logits are missing or not aligned to their type");
   if (k != 0u && (value == nullptr || index == nullptr)) return refuse(symbol, "an array is missing");
-  const uint32_t grid = dim1 < (1u << 24) ? dim1 : (1u << 24);
-  top_k_radix_kernel<T><<<grid, kTopThreads, 0, as_stream(stream)>>>(
-      dim0, dim1, size_t(stride != 0u ? stride : dim0), k, scale_for(temperature), 1.0 / double(temperature), x, value, index, log_norm);
-  note_launch(symbol);
-  return 0;
+  const size_t pitch = stride != 0u ? stride : dim0;
+  const hipStream_t st = as_stream(stream);
+  // (a wave's 64 lanes speak for its share of k: four waves up to 128, sixteen beyond)
+  if (k <= 128u) {
+    return log_norm != nullptr
+               ? launch_top_k<T, 256, 1536, true>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st)
+               : launch_top_k<T, 256, 1536, false>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+  }
+  return log_norm != nullptr
+             ? launch_top_k<T, 1024, 4096, true>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st)
+             : launch_top_k<T, 1024, 4096, false>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
 }
 
 }  // namespace
