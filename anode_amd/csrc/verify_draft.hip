@@ -11,8 +11,9 @@
 namespace anode {
 namespace {
 
-constexpr int kDrawThreads = 1024;
-constexpr int kDrawWaves = kDrawThreads / kWave;
+constexpr int kDrawThreads = 256;
+constexpr uint32_t kDrawWaves = kDrawThreads / kWave;
+constexpr uint32_t kBlockGroups = 512;  // 16-byte groups (2048 classes) of a row that are summed together: eight a lane
 
 struct Drafts {
   uint32_t n, drafted;       // classes; drafted tokens of a sequence at most
@@ -28,20 +29,73 @@ struct Drafts {
 struct Weights {
   const float *p, *q;
   uint32_t without;
+  __device__ static double weight(double w) { return fmax(w, 0.0); }
   __device__ double of(uint32_t j, float pj, float qj) const {
     double w = double(pj);
     if (q != nullptr) w -= double(qj);
-    return w > 0.0 && j != without ? w : 0.0;
+    return j != without ? weight(w) : 0.0;
   }
 };
 
-// The four weights of a 16-byte group of the row, in class order.
-__device__ inline void group_weights(const RowGroups<float> &rg, const Weights &ws, uint32_t g, double (&w)[4]) {
-  float p[4], q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  load_group<float, 0>(rg, ws.p, g, 0.0f, p);
-  if (ws.q != nullptr) load_group<float, 0>(rg, ws.q, g, 0.0f, q);
+// The rows that sequence b's token is drawn from once `taken` of its drafted tokens are taken.
+__device__ inline Weights weights_of(const Drafts &d, size_t b, uint32_t taken, bool refused) {
+  Weights ws;
+  ws.p = d.target + (b * (size_t(d.drafted) + 1u) + taken) * d.n;
+  ws.q = refused && d.draft != nullptr ? d.draft + (b * d.drafted + taken) * size_t(d.n) : nullptr;
+  ws.without = refused && d.draft == nullptr ? d.token[b * d.drafted + taken] : kNoClass;
+  return ws;
+}
+
+// Sums of one block of a row: what is left of the target after the draft, and the target itself, from which the token is
+// drawn where nothing is left.
+struct BlockSum {
+  double rest, whole;
+};
+
+// One block by a whole wave, groups lane, lane + 64, ... of it.
+template <bool DRAFT>
+__device__ inline BlockSum sum_block(const RowGroups<float> &rg, const Weights &ws, uint32_t lo) {
+  constexpr int U = 4;
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+  BlockSum s = {0.0, 0.0};
+  const uint32_t end = min(rg.groups - lo, kBlockGroups);            // groups of the block
+  const uint32_t whole_end = min(rg.n / 4u - lo, kBlockGroups);      // (the row's last group can be shorter)
+  if (whole_end != 0u) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w[j] = ws.of(rg.first(g) + uint32_t(j), p[j], q[j]);
+    for (uint32_t half = 0; half < kBlockGroups; half += uint32_t(U) * kWave) {
+      u32x4 p[U], q[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t at = lo + min(half + uint32_t(u) * kWave + lane, whole_end - 1u);
+        p[u] = load_stream<0>(reinterpret_cast<const u32x4 *>(ws.p + size_t(at) * 4u));
+        if (DRAFT) q[u] = load_stream<0>(reinterpret_cast<const u32x4 *>(ws.q + size_t(at) * 4u));
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const uint32_t at = half + uint32_t(u) * kWave + lane;
+        double rest[4], whole[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float pj = __uint_as_float(p[u][j]);
+          whole[j] = Weights::weight(double(pj));
+          rest[j] = DRAFT ? Weights::weight(double(pj) - double(__uint_as_float(q[u][j])))
+                          : ((lo + at) * 4u + uint32_t(j) != ws.without ? whole[j] : 0.0);
+        }
+        if (at < whole_end) {
+          s.rest += (rest[0] + rest[1]) + (rest[2] + rest[3]);
+          s.whole += (whole[0] + whole[1]) + (whole[2] + whole[3]);
+        }
+      }
+    }
+  }
+  if (whole_end < end && lane < rg.n % 4u) {
+    const uint32_t j = (lo + whole_end) * 4u + lane;
+    s.rest += ws.of(j, ws.p[j], DRAFT ? ws.q[j] : 0.0f);
+    s.whole += Weights::weight(double(ws.p[j]));
+  }
+  s.rest = wave_sum(s.rest);
+  s.whole = wave_sum(s.whole);
+  return s;
 }
 
 // Drafted tokens that sequence b takes, and how many it holds; by one whole wave.
@@ -67,128 +121,140 @@ __device__ inline uint32_t taken_tokens(const Drafts &d, size_t b, uint32_t &len
   return length;
 }
 
-// One workgroup a sequence.  Every wave sums a contiguous part of the row; the part in which the running sum passes
-// the border is summed again, every thread a contiguous piece, and the piece in which it passes is walked.
-__global__ __launch_bounds__(kDrawThreads) void verify_draft_kernel(Drafts d, uint32_t sequences, const float *__restrict__ pick,
-                                                                    uint32_t *__restrict__ out, uint32_t *__restrict__ accepted) {
-  __shared__ double part[kDrawWaves];
-  __shared__ uint32_t s_taken, s_length, s_drawn, s_first;
-  const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+// What the summing kernel leaves for the drawing kernel.
+struct Sums {
+  BlockSum *block;   // [blocks, sequences]
+  uint32_t *taken;   // [sequences]: tokens taken, and the top bit where one was refused
+};
+constexpr uint32_t kRefused = 0x80000000u;
+
+// One wave `each` blocks of a sequence's row (every wave finds out for itself which row that is).
+__global__ __launch_bounds__(kDrawThreads) void draw_sums_kernel(Drafts d, uint32_t sequences, uint32_t blocks, uint32_t each,
+                                                                 Sums out) {
   const RowGroups<float> rg(d.n, 0u);
-  for (size_t b = blockIdx.x; b < sequences; b += gridDim.x) {
-    if (wave == 0) {
-      uint32_t length;
-      const uint32_t taken = taken_tokens(d, b, length);
-      if (lane == 0) {
-        s_taken = taken;
-        s_length = length;
-        s_drawn = kNoClass;
-      }
+  const uint32_t runs = (blocks + each - 1u) / each > 0u ? (blocks + each - 1u) / each : 1u;  // waves of a sequence
+  const uint64_t items = uint64_t(sequences) * runs;
+  for (uint64_t item = uint64_t(blockIdx.x) * kDrawWaves + threadIdx.x / kWave; item < items;
+       item += uint64_t(gridDim.x) * kDrawWaves) {
+    const size_t b = item / runs;
+    const uint32_t run = uint32_t(item % runs);
+    uint32_t length;
+    const uint32_t taken = taken_tokens(d, b, length);
+    const bool refused = taken < length;
+    const bool lead = (threadIdx.x & (kWave - 1)) == 0;
+    if (run == 0u && lead) out.taken[b] = taken | (refused ? kRefused : 0u);
+    const Weights ws = weights_of(d, b, taken, refused);
+    for (uint32_t i = run * each; i < blocks && i < (run + 1u) * each; ++i) {
+      const BlockSum s = ws.q != nullptr ? sum_block<true>(rg, ws, i * kBlockGroups) : sum_block<false>(rg, ws, i * kBlockGroups);
+      if (lead) out.block[b * blocks + i] = s;
     }
-    __syncthreads();
-    const uint32_t taken = s_taken;
-    const bool refused = taken < s_length;
-    Weights ws;
-    ws.p = d.target + (b * (size_t(d.drafted) + 1u) + taken) * d.n;
-    ws.q = refused && d.draft != nullptr ? d.draft + (b * d.drafted + taken) * size_t(d.n) : nullptr;
-    ws.without = refused && d.draft == nullptr ? d.token[b * d.drafted + taken] : kNoClass;
-    const uint32_t each = (rg.groups + kDrawWaves - 1u) / kDrawWaves;  // groups of a wave
-    double total = 0.0;
-    for (int turn = 0; turn < 2; ++turn) {
-      double sum = 0.0;
-      const uint32_t end = min(rg.groups, (wave + 1u) * each);
-      for (uint32_t g = wave * each + lane; g < end; g += kWave) {
-        double w[4];
-        group_weights(rg, ws, g, w);
-        sum += (w[0] + w[1]) + (w[2] + w[3]);
-      }
-      sum = wave_sum(sum);
-      if (lane == 0) part[wave] = sum;
-      __syncthreads();
-      total = 0.0;
-      for (int w = 0; w < kDrawWaves; ++w) total += part[w];
-      if (total > 0.0 || !refused) break;
+  }
+}
+
+// Sum over the lanes up to this one, and of all of them.
+__device__ inline double lanes_upto(double v, double &total) {
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const double o = __shfl_up(v, off, kWave);
+    if (int(lane) >= off) v += o;
+  }
+  total = __shfl(v, kWave - 1, kWave);
+  return v;
+}
+// The first lane whose running sum passes the border, of those that weigh; or else (u of 1 and more, a NaN, the last
+// step's rounding) the last that weighs; -1 where none does.
+__device__ inline int lane_at(double own, double upto, double border) {
+  const uint64_t weighs = __ballot(own > 0.0);
+  const uint64_t passes = __ballot(own > 0.0 && upto > border);
+  if (passes != 0u) return __ffsll((unsigned long long)passes) - 1;
+  return weighs != 0u ? 63 - __clzll((long long)weighs) : -1;
+}
+
+// One wave a sequence: the block in which the running sum passes the border, the lane's eight groups of it in which it
+// does, and the class; nothing leaves the registers.
+__global__ __launch_bounds__(kWave) void draw_kernel(Drafts d, uint32_t sequences, uint32_t blocks, Sums in,
+                                                     const float *__restrict__ pick, uint32_t *__restrict__ out,
+                                                     uint32_t *__restrict__ accepted) {
+  constexpr int kOwn = int(kBlockGroups) / kWave;
+  const uint32_t lane = threadIdx.x;
+  const RowGroups<float> rg(d.n, 0u);
+  const uint32_t each = (blocks + kWave - 1u) / kWave;  // blocks of a lane
+  for (size_t b = blockIdx.x; b < sequences; b += gridDim.x) {
+    const uint32_t word = in.taken[b], taken = word & ~kRefused;
+    const double u = double(pick[b]);
+    const uint32_t b0 = min(blocks, lane * each), b1 = min(blocks, b0 + each);
+    double own_rest = 0.0, own_whole = 0.0;
+    for (uint32_t i = b0; i < b1; ++i) {
+      const BlockSum s = in.block[b * blocks + i];
+      own_rest += s.rest;
+      own_whole += s.whole;
+    }
+    Weights ws = weights_of(d, b, taken, (word & kRefused) != 0u);
+    double total, own = own_rest;
+    double upto = lanes_upto(own, total);
+    const bool left = total > 0.0;
+    if (!left) {
       // nothing is left of the difference (the target equals the draft there): the target's row itself
       ws.q = nullptr;
       ws.without = kNoClass;
-      __syncthreads();
+      own = own_whole;
+      upto = lanes_upto(own, total);
     }
-    const double border = double(pick[b]) * total;
-    // the part in which the running sum passes the border; where none does (u of 1 and more, a NaN) the last that weighs
-    uint32_t in = kNoClass, last = kNoClass;
-    double before = 0.0, before_last = 0.0;
-    for (uint32_t w = 0; w < uint32_t(kDrawWaves); ++w) {
-      if (!(part[w] > 0.0)) continue;
-      last = w;
-      before_last = before;
-      if (before + part[w] > border) {
-        in = w;
-        break;
-      }
-      before += part[w];
-    }
-    if (in == kNoClass) {
-      in = last;
-      before = before_last;
-    }
-    __syncthreads();
-    if (in != kNoClass) {
-      const uint32_t lo = min(rg.groups, in * each), hi = min(rg.groups, lo + each);
-      const uint32_t piece = (hi - lo + kDrawThreads - 1u) / kDrawThreads;
-      const uint32_t g0 = min(hi, lo + threadIdx.x * piece), g1 = min(hi, g0 + piece);
-      double own = 0.0;
-      for (uint32_t g = g0; g < g1; ++g) {
-        double w[4];
-        group_weights(rg, ws, g, w);
-        own += (w[0] + w[1]) + (w[2] + w[3]);
-      }
-      double upto = own;
-#pragma unroll
-      for (int off = 1; off < kWave; off <<= 1) {
-        const double o = __shfl_up(upto, off, kWave);
-        if (int(lane) >= off) upto += o;
-      }
-      if (lane == kWave - 1) part[wave] = upto;
-      if (threadIdx.x == 0) s_first = kNoClass;
-      __syncthreads();
-      for (uint32_t w = 0; w < wave; ++w) before += part[w];
-      // the first piece that passes the border, or else the last that weighs
-      const bool weighs = own > 0.0;
-      const bool passes = weighs && before + upto > border;
-      if (passes) atomicMin(&s_first, threadIdx.x);
-      __syncthreads();
-      if (s_first == kNoClass) {
-        __syncthreads();
-        if (threadIdx.x == 0) s_first = 0u;
-        __syncthreads();
-        if (weighs) atomicMax(&s_first, threadIdx.x);
-        __syncthreads();
-      }
-      if (threadIdx.x == s_first) {
-        double run = before + (upto - own);
-        uint32_t drawn = kNoClass;
-        bool done = false;
-        for (uint32_t g = g0; g < g1 && !done; ++g) {
-          double w[4];
-          group_weights(rg, ws, g, w);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (!done && w[j] > 0.0) {
-              drawn = rg.first(g) + uint32_t(j);
-              run += w[j];
-              done = run > border;
-            }
-          }
+    const double border = u * total;
+    uint32_t drawn = kNoClass;
+    const int at = lane_at(own, upto, border);
+    if (at >= 0) {
+      // among that lane's blocks in turn
+      double before = __shfl(upto - own, at, kWave);
+      const uint32_t first = uint32_t(__shfl(int(b0), at, kWave)), end = uint32_t(__shfl(int(b1), at, kWave));
+      uint32_t block = first;
+      double before_block = before;
+      for (uint32_t i = first; i < end; ++i) {
+        const BlockSum s = in.block[b * blocks + i];
+        const double w = left ? s.rest : s.whole;
+        if (w > 0.0) {
+          block = i;
+          before_block = before;
+          if (before + w > border) break;
         }
-        s_drawn = drawn;
+        before += w;
       }
-      __syncthreads();
+      // a lane's eight groups of the block, which lie side by side
+      const uint32_t g0 = block * kBlockGroups + lane * uint32_t(kOwn);
+      double w[4 * kOwn];
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const uint32_t g = g0 + uint32_t(i);
+        float p[4] = {0.0f, 0.0f, 0.0f, 0.0f}, q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (g < rg.groups) {
+          load_group<float, 0>(rg, ws.p, g, 0.0f, p);
+          if (ws.q != nullptr) load_group<float, 0>(rg, ws.q, g, 0.0f, q);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[4 * i + j] = ws.of(rg.first(g) + uint32_t(j), p[j], q[j]);
+      }
+      own = 0.0;
+#pragma unroll
+      for (int i = 0; i < 4 * kOwn; ++i) own += w[i];
+      upto = before_block + lanes_upto(own, total);
+      const int last = lane_at(own, upto, border);
+      double run = upto - own;
+      bool done = false;
+#pragma unroll
+      for (int i = 0; i < 4 * kOwn; ++i) {
+        if (!done && w[i] > 0.0) {
+          drawn = g0 * 4u + uint32_t(i);
+          run += w[i];
+          done = run > border;
+        }
+      }
+      drawn = uint32_t(__shfl(int(drawn), last, kWave));  // (a block that weighs has a lane that does)
     }
-    if (threadIdx.x == 0) accepted[b] = taken;
-    for (uint32_t i = threadIdx.x; i <= d.drafted; i += kDrawThreads) {
-      out[b * (size_t(d.drafted) + 1u) + i] = i < taken ? d.token[b * d.drafted + i] : i == taken ? s_drawn : kNoClass;
+    if (lane == 0u) accepted[b] = taken;
+    for (uint64_t i = lane; i <= d.drafted; i += kWave) {
+      out[b * (size_t(d.drafted) + 1u) + i] = i < taken ? d.token[b * d.drafted + i] : i == taken ? drawn : kNoClass;
     }
-    __syncthreads();
   }
 }
 
@@ -204,10 +270,24 @@ ANODE_EXPORT int anode_gpu_verify_draft_packed_f32(uint32_t dim0, uint32_t dim1,
   if (dim0 != 0u && target == nullptr) return refuse(__func__, "the target's probabilities are missing");
   if (dim1 != 0u && (draft_token == nullptr || accept == nullptr)) return refuse(__func__, "the drafted tokens are missing");
   if (pick == nullptr || token == nullptr || accepted == nullptr) return refuse(__func__, "an array is missing");
-  if (dim1 == 0xffffffffu) return refuse(__func__, "more drafted tokens than an index holds");
-  const uint32_t grid = dim2 < (1u << 24) ? dim2 : (1u << 24);
+  if (dim1 >= kRefused) return refuse(__func__, "more drafted tokens than 2^31 - 1");
+  const hipStream_t st = as_stream(stream);
+  const uint32_t groups = dim0 / 4u + (dim0 % 4u != 0u);
+  const uint32_t blocks = groups / kBlockGroups + (groups % kBlockGroups != 0u);
+  // blocks of a wave: so many that the launch has eight waves a SIMD
+  const uint64_t waves = uint64_t(device_cu_count()) * 32u;
+  uint64_t each = uint64_t(dim2) * blocks / waves;
+  each = each < 1u ? 1u : each > blocks ? blocks : each;
+  const uint64_t runs = blocks != 0u ? (blocks + each - 1u) / each : 1u;
+  const size_t block_bytes = size_t(dim2) * blocks * sizeof(BlockSum);
+  ScratchLease scratch = acquire_scratch(st, block_bytes + size_t(dim2) * sizeof(uint32_t), __func__);
+  if (!scratch.ptr) return int(hipErrorOutOfMemory);
+  const Sums sums = {static_cast<BlockSum *>(scratch.ptr), reinterpret_cast<uint32_t *>(static_cast<char *>(scratch.ptr) + block_bytes)};
   const Drafts d = {dim0, dim1, target, draft, draft_token, draft_length, accept};
-  verify_draft_kernel<<<grid, kDrawThreads, 0, as_stream(stream)>>>(d, dim2, pick, token, accepted);
+  const uint64_t items = (uint64_t(dim2) * runs + kDrawWaves - 1u) / kDrawWaves;
+  const uint64_t most = 1u << 24;
+  draw_sums_kernel<<<uint32_t(items < most ? items : most), kDrawThreads, 0, st>>>(d, dim2, blocks, uint32_t(each), sums);
+  draw_kernel<<<uint32_t(dim2 < most ? dim2 : most), kWave, 0, st>>>(d, dim2, blocks, sums, pick, token, accepted);
   note_launch(__func__);
   return 0;
 }
