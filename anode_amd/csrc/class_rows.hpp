@@ -42,6 +42,49 @@ static inline bool misaligned(const T *p) {
 
 constexpr float kMinusInf = -__builtin_huge_valf();
 
+// Moves between lanes without the LDS pipe (data-parallel primitives): the value of the lane 1, 2, 4 or 8 before in its
+// row of sixteen, of the last lane of the row before (rows 1 and 3), or of lane 31 (rows 2 and 3); lanes that get none keep
+// `none`.  Six such steps make lane 63 the sum of all lanes, and every lane the sum of those up to it, in about 100
+// clocks, where six exchanges through ds_bpermute take about 600 (a double is two of them).
+template <int STEP>
+__device__ inline uint32_t lane_before(uint32_t none, uint32_t v) {
+  constexpr int kControl = STEP < 4 ? 0x110 + (1 << STEP) : STEP == 4 ? 0x142 : 0x143;  // row_shr 1 2 4 8, row_bcast 15 31
+  constexpr int kRows = STEP < 4 ? 0xf : STEP == 4 ? 0xa : 0xc;
+  return uint32_t(__builtin_amdgcn_update_dpp(int(none), int(v), kControl, kRows, 0xf, false));
+}
+template <int STEP>
+__device__ inline float lane_before(float none, float v) {
+  return __uint_as_float(lane_before<STEP>(__float_as_uint(none), __float_as_uint(v)));
+}
+template <int STEP>
+__device__ inline double lane_before(double none, double v) {
+  const uint64_t n = __builtin_bit_cast(uint64_t, none), b = __builtin_bit_cast(uint64_t, v);
+  const uint64_t lo = lane_before<STEP>(uint32_t(n), uint32_t(b)), hi = lane_before<STEP>(uint32_t(n >> 32), uint32_t(b >> 32));
+  return __builtin_bit_cast(double, hi << 32 | lo);
+}
+// A lane's value in every lane (the lane is the same in all of them).
+__device__ inline uint32_t from_lane(uint32_t v, int lane) { return uint32_t(__builtin_amdgcn_readlane(int(v), lane)); }
+__device__ inline float from_lane(float v, int lane) { return __uint_as_float(from_lane(__float_as_uint(v), lane)); }
+__device__ inline double from_lane(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  return __builtin_bit_cast(double, uint64_t(from_lane(uint32_t(b >> 32), lane)) << 32 | from_lane(uint32_t(b), lane));
+}
+// Sum over the lanes up to this one.
+template <typename V>
+__device__ inline V lanes_upto(V v) {
+  v += lane_before<0>(V(0), v);
+  v += lane_before<1>(V(0), v);
+  v += lane_before<2>(V(0), v);
+  v += lane_before<3>(V(0), v);
+  v += lane_before<4>(V(0), v);
+  v += lane_before<5>(V(0), v);
+  return v;
+}
+template <typename V>
+__device__ inline V lanes_sum(V v) {
+  return from_lane(lanes_upto(v), kWave - 1);
+}
+
 // One 16-byte group of a row: W values.
 template <typename T>
 struct Group {
@@ -213,16 +256,20 @@ __device__ inline SoftmaxSum merge(SoftmaxSum a, SoftmaxSum b, float c) {
   r.s = a.s * __builtin_amdgcn_exp2f(a.m * c - shift) + b.s * __builtin_amdgcn_exp2f(b.m * c - shift);
   return r;
 }
+template <int STEP>
+__device__ inline SoftmaxSum merge_before(SoftmaxSum t, float c) {
+  return merge(t, SoftmaxSum{lane_before<STEP>(t.m, t.m), lane_before<STEP>(0.0f, t.s)}, c);
+}
 // The same in every lane of the wave, merged in a fixed order.
 __device__ inline SoftmaxSum wave_merge(SoftmaxSum t, float c) {
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) {
-    SoftmaxSum o;
-    o.m = __shfl_xor(t.m, off, kWave);
-    o.s = __shfl_xor(t.s, off, kWave);
-    t = merge(t, o, c);
-  }
-  return t;
+  t = merge_before<0>(t, c);
+  t = merge_before<1>(t, c);
+  t = merge_before<2>(t, c);
+  t = merge_before<3>(t, c);
+  t = merge_before<4>(t, c);
+  t = merge_before<5>(t, c);
+  // (an exchange, not from_lane(): results in scalar registers push the held rows of distill.hip out of the vector ones)
+  return SoftmaxSum{__shfl(t.m, kWave - 1, kWave), __shfl(t.s, kWave - 1, kWave)};
 }
 // COUNT <= 16 entries in LDS merged, the same in every lane.
 template <int COUNT>
@@ -231,14 +278,11 @@ __device__ inline SoftmaxSum lane_merge(const SoftmaxSum *lds, float c) {
   const uint32_t lane = threadIdx.x & 15u;
   SoftmaxSum t = lds[lane < uint32_t(COUNT) ? lane : 0u];
   if (lane >= uint32_t(COUNT)) t.s = 0.0f;  // (an entry again, of which nothing is added)
-#pragma unroll
-  for (int off = 8; off > 0; off >>= 1) {
-    SoftmaxSum o;
-    o.m = __shfl_xor(t.m, off, kWave);
-    o.s = __shfl_xor(t.s, off, kWave);
-    t = merge(t, o, c);
-  }
-  return t;
+  t = merge_before<0>(t, c);
+  t = merge_before<1>(t, c);
+  t = merge_before<2>(t, c);
+  t = merge_before<3>(t, c);
+  return SoftmaxSum{__shfl(t.m, 15, 16), __shfl(t.s, 15, 16)};
 }
 // The same in every thread of the workgroup; `lds` holds one entry a wave.  Ends with a barrier.
 template <int WAVES>

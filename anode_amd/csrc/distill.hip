@@ -390,8 +390,7 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32
 }
 
 // Loss and gradient, one workgroup a row: the first G groups of each streaming thread stay in registers from the statistics
-// to the gradient, so that x is read once (what lies behind them is streamed a second time).  A workgroup takes rows in
-// turn: as each register is stored it takes the next row's group, so that loads and stores overlap across rows.  The
+// to the gradient, so that x is read once (what lies behind them is streamed a second time).  The
 // slots belong to a wave of their own: their 64-bit exponentials and logarithms would spill the held registers of a
 // wave that streams, and take about as long as a small row.
 template <typename T, int S, int G, int NT>
@@ -433,20 +432,18 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
     }
     return;
   }
-  size_t r = blockIdx.x;
-  if (r >= rows) return;
   const uint32_t mine = threadIdx.x * 16u;  // (bytes) the thread's place among a step's groups
   constexpr uint32_t kStep = uint32_t(S) * 16u;
-  RowSpan<T> span(n, values_to_line(dx + r * stride));
-  u32x4 q[G];
-  {
-    const GroupBuffer xb(x + r * stride + span.head, min(span.groups, kHeld));
-#pragma unroll
-    for (int u = 0; u < G; ++u) q[u] = xb.load<0>(mine, uint32_t(u) * kStep);
-  }
-  for (;;) {
+  for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T *xr = x + r * stride;
     T *dxr = dx + r * stride;
+    const RowSpan<T> span(n, values_to_line(dxr));
+    u32x4 q[G];
+    {
+      const GroupBuffer xb(xr + span.head, min(span.groups, kHeld));
+#pragma unroll
+      for (int u = 0; u < G; ++u) q[u] = xb.load<0>(mine, uint32_t(u) * kStep);
+    }
     const float w = float(double(dy[r]) * inv_t);
     SoftmaxSum st = {-sc.limit, 0.0f};
 #pragma unroll 1
@@ -476,22 +473,17 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
 #pragma unroll
     for (int u = 0; u < G; ++u) forget(q[u]);
     const Dense d = dense_of(st, sc, w, rs.mass, rs.any != 0);
-    const size_t r2 = r + gridDim.x;
-    const bool more = r2 < rows;
-    const RowSpan<T> span2(n, values_to_line(dx + r2 * stride));
-    // (no row to come: a buffer of no groups, whose loads read nothing)
-    const GroupBuffer xb(x + r2 * stride + span2.head, more ? min(span2.groups, kHeld) : 0u);
+    single_grad<T, S, false>(span, xr, dxr, d);
     if (d.fast) {
-      const GroupBuffer db(dxr + span.head, min(span.groups, kHeld));
-      single_grad<T, S, false>(span, xr, dxr, d);
-  #pragma unroll 1
-    for (uint32_t g = kHeld + threadIdx.x; g < span.groups; g += S) {
+#pragma unroll 1
+      for (uint32_t g = kHeld + threadIdx.x; g < span.groups; g += S) {
         float v[W];
         unpack(load_stream<0, int(sizeof(T))>(reinterpret_cast<const u32x4 *>(xr + size_t(span.first(g)))), v, x);
 #pragma unroll
         for (int j = 0; j < W; ++j) v[j] = fast_term(v[j], d);
         store_group<0, int(sizeof(T))>(dxr + size_t(span.first(g)), pack(v, dx));
       }
+      const GroupBuffer db(dxr + span.head, min(span.groups, kHeld));
 #pragma unroll
       for (int u = 0; u < G; ++u) {
         float v[W];
@@ -499,10 +491,8 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
 #pragma unroll
         for (int j = 0; j < W; ++j) v[j] = fast_term(v[j], d);
         db.store<NT>(pack(v, dx), mine, uint32_t(u) * kStep);
-        q[u] = xb.load<0>(mine, uint32_t(u) * kStep);
       }
     } else {
-      single_grad<T, S, false>(span, xr, dxr, d);
 #pragma unroll 1
       for (uint32_t g = threadIdx.x; g < span.groups; g += S) {
         float v[W];
@@ -511,15 +501,10 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
         for (int j = 0; j < W; ++j) v[j] = any_term(v[j], d);
         store_group<0, int(sizeof(T))>(dxr + size_t(span.first(g)), pack(v, dx));
       }
-#pragma unroll
-      for (int u = 0; u < G; ++u) q[u] = xb.load<0>(mine, uint32_t(u) * kStep);
     }
     __syncthreads();  // 2
     if (d.any) store_slots<T, S, false>(t.k, dxr, 0u, span, kHeld, slots);
     __syncthreads();  // 3
-    if (!more) break;
-    r = r2;
-    span = span2;
   }
 }
 
@@ -675,22 +660,20 @@ template <typename T, int NT>
 void launch_fused(const Shape &s, const T *x, const Teacher &t, const float *dy, float *loss, float *row_max, float *row_sum,
                   T *dx, hipStream_t st) {
   const size_t row = size_t(s.n) * sizeof(T);
-  const uint32_t cus = uint32_t(device_cu_count());
-  auto go = [&](auto kernel, uint32_t threads, uint32_t a_cu) {
-    const uint32_t resident = cus * a_cu;
-    kernel<<<s.rows < resident ? s.rows : resident, threads, slot_bytes(t.k), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t,
-                                                                                   dy, loss, row_max, row_sum, dx);
+  auto go = [&](auto kernel, uint32_t threads) {
+    kernel<<<grid_for(s.rows), threads, slot_bytes(t.k), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, dy, loss, row_max,
+                                                              row_sum, dx);
   };
   if (row <= 4096u) {
-    go(distill_wave_kernel<T, 4, NT>, kWave, 1u << 16);
+    go(distill_wave_kernel<T, 4, NT>, kWave);
   } else if (row <= 18432u) {
-    go(distill_held_kernel<T, 192, 6, NT>, 256u, 4u);
+    go(distill_held_kernel<T, 192, 6, NT>, 256u);
   } else if (row <= 71680u) {
-    go(distill_held_kernel<T, 448, 10, NT>, 512u, 2u);
+    go(distill_held_kernel<T, 448, 10, NT>, 512u);
   } else if (row <= 136192u) {
-    go(distill_held_kernel<T, 448, 20, NT>, 512u, 2u);
+    go(distill_held_kernel<T, 448, 20, NT>, 512u);
   } else {
-    go(distill_held_kernel<T, 960, 18, NT>, 1024u, 1u);
+    go(distill_held_kernel<T, 960, 18, NT>, 1024u);
   }
 }
 

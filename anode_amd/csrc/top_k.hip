@@ -71,17 +71,6 @@ __device__ inline void sort_entries(uint64_t *e, uint32_t size) {
   __syncthreads();
 }
 
-// Inclusive sum over the lanes up to this one.
-__device__ inline uint32_t wave_upto(uint32_t v) {
-  const uint32_t lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const uint32_t o = __shfl_up(v, off, kWave);
-    if (int(lane) >= off) v += o;
-  }
-  return v;
-}
-
 // A key that at least j lanes reach, found bit by bit (its leading 18 bits; those below are 0): 0 where fewer lanes hold a
 // key at all.  The comparisons' results are scalar, so a step is a compare, a count and a select.
 __device__ inline uint32_t key_reached_by(uint32_t key, uint32_t j) {
@@ -130,7 +119,7 @@ __device__ inline uint32_t radix_select(const T *xr, uint32_t n, uint32_t from, 
       uint32_t d[4], own = 0u;
 #pragma unroll
       for (int i = 0; i < 4; ++i) own += d[i] = l.digits[255u - 4u * lane - uint32_t(i)];
-      uint32_t run = wave_upto(own) - own;
+      uint32_t run = lanes_upto(own) - own;
       if (lane == 0) l.found = 256u;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -179,7 +168,7 @@ __device__ inline uint32_t radix_select(const T *xr, uint32_t n, uint32_t from, 
       for (int j = 0; j < W; ++j) same |= uint32_t(key_of(v[j]) == kth) << j;
     }
     const uint32_t own = uint32_t(__popc(same));
-    const uint32_t upto = wave_upto(own);
+    const uint32_t upto = lanes_upto(own);
     if (lane == kWave - 1) l.wave_count[wave] = upto;
     __syncthreads();
     uint32_t at = before + upto - own, total = 0u;

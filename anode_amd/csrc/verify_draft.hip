@@ -14,6 +14,10 @@ namespace {
 constexpr int kDrawThreads = 256;
 constexpr uint32_t kDrawWaves = kDrawThreads / kWave;
 constexpr uint32_t kBlockGroups = 512;  // 16-byte groups (2048 classes) of a row that are summed together: eight a lane
+// Rows of up to 16 blocks (32768 classes) are drawn from in one launch, a workgroup a sequence; longer rows are spread over the
+// GPU first and drawn from by a second kernel.  Measured at 32768 classes 9.4 against 11.7 us for 200 sequences and
+// 8.1 against 10.0 for 16; at 131072 classes 18.5 against 10.2 us for 16 and 153 against 136 us for 1024.
+constexpr uint32_t kMostHeld = 16;
 
 struct Drafts {
   uint32_t n, drafted;       // classes; drafted tokens of a sequence at most
@@ -53,7 +57,7 @@ struct BlockSum {
 };
 
 // One block by a whole wave, groups lane, lane + 64, ... of it.
-template <bool DRAFT>
+template <bool DRAFT, int NT>
 __device__ inline BlockSum sum_block(const RowGroups<float> &rg, const Weights &ws, uint32_t lo) {
   constexpr int U = 4;
   const uint32_t lane = threadIdx.x & (kWave - 1);
@@ -67,8 +71,8 @@ __device__ inline BlockSum sum_block(const RowGroups<float> &rg, const Weights &
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const uint32_t at = lo + min(half + uint32_t(u) * kWave + lane, whole_end - 1u);
-        p[u] = load_stream<0>(reinterpret_cast<const u32x4 *>(ws.p + size_t(at) * 4u));
-        if (DRAFT) q[u] = load_stream<0>(reinterpret_cast<const u32x4 *>(ws.q + size_t(at) * 4u));
+        p[u] = load_stream<NT>(reinterpret_cast<const u32x4 *>(ws.p + size_t(at) * 4u));
+        if (DRAFT) q[u] = load_stream<NT>(reinterpret_cast<const u32x4 *>(ws.q + size_t(at) * 4u));
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -93,8 +97,8 @@ __device__ inline BlockSum sum_block(const RowGroups<float> &rg, const Weights &
     s.rest += ws.of(j, ws.p[j], DRAFT ? ws.q[j] : 0.0f);
     s.whole += Weights::weight(double(ws.p[j]));
   }
-  s.rest = wave_sum(s.rest);
-  s.whole = wave_sum(s.whole);
+  s.rest = lanes_sum(s.rest);
+  s.whole = lanes_sum(s.whole);
   return s;
 }
 
@@ -121,47 +125,6 @@ __device__ inline uint32_t taken_tokens(const Drafts &d, size_t b, uint32_t &len
   return length;
 }
 
-// What the summing kernel leaves for the drawing kernel.
-struct Sums {
-  BlockSum *block;   // [blocks, sequences]
-  uint32_t *taken;   // [sequences]: tokens taken, and the top bit where one was refused
-};
-constexpr uint32_t kRefused = 0x80000000u;
-
-// One wave `each` blocks of a sequence's row (every wave finds out for itself which row that is).
-__global__ __launch_bounds__(kDrawThreads) void draw_sums_kernel(Drafts d, uint32_t sequences, uint32_t blocks, uint32_t each,
-                                                                 Sums out) {
-  const RowGroups<float> rg(d.n, 0u);
-  const uint32_t runs = (blocks + each - 1u) / each > 0u ? (blocks + each - 1u) / each : 1u;  // waves of a sequence
-  const uint64_t items = uint64_t(sequences) * runs;
-  for (uint64_t item = uint64_t(blockIdx.x) * kDrawWaves + threadIdx.x / kWave; item < items;
-       item += uint64_t(gridDim.x) * kDrawWaves) {
-    const size_t b = item / runs;
-    const uint32_t run = uint32_t(item % runs);
-    uint32_t length;
-    const uint32_t taken = taken_tokens(d, b, length);
-    const bool refused = taken < length;
-    const bool lead = (threadIdx.x & (kWave - 1)) == 0;
-    if (run == 0u && lead) out.taken[b] = taken | (refused ? kRefused : 0u);
-    const Weights ws = weights_of(d, b, taken, refused);
-    for (uint32_t i = run * each; i < blocks && i < (run + 1u) * each; ++i) {
-      const BlockSum s = ws.q != nullptr ? sum_block<true>(rg, ws, i * kBlockGroups) : sum_block<false>(rg, ws, i * kBlockGroups);
-      if (lead) out.block[b * blocks + i] = s;
-    }
-  }
-}
-
-// Sum over the lanes up to this one, and of all of them.
-__device__ inline double lanes_upto(double v, double &total) {
-  const uint32_t lane = threadIdx.x & (kWave - 1);
-#pragma unroll
-  for (int off = 1; off < kWave; off <<= 1) {
-    const double o = __shfl_up(v, off, kWave);
-    if (int(lane) >= off) v += o;
-  }
-  total = __shfl(v, kWave - 1, kWave);
-  return v;
-}
 // The first lane whose running sum passes the border, of those that weigh; or else (u of 1 and more, a NaN, the last
 // step's rounding) the last that weighs; -1 where none does.
 __device__ inline int lane_at(double own, double upto, double border) {
@@ -171,90 +134,158 @@ __device__ inline int lane_at(double own, double upto, double border) {
   return weighs != 0u ? 63 - __clzll((long long)weighs) : -1;
 }
 
-// One wave a sequence: the block in which the running sum passes the border, the lane's eight groups of it in which it
-// does, and the class; nothing leaves the registers.
+// The drawn class, by one whole wave from the sums of the row's blocks: the block in which the running sum passes the border,
+// the lane's eight groups of it in which it does, and the class; nothing leaves the registers.
+__device__ __forceinline__ uint32_t draw_token(const RowGroups<float> &rg, Weights ws, uint32_t blocks, const BlockSum *sums, double u) {
+  constexpr int kOwn = int(kBlockGroups) / kWave;
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+  const uint32_t each = (blocks + kWave - 1u) / kWave;  // blocks of a lane
+  const uint32_t b0 = min(blocks, lane * each), b1 = min(blocks, b0 + each);
+  BlockSum mine = {0.0, 0.0};
+  for (uint32_t i = b0; i < b1; ++i) {
+    const BlockSum s = sums[i];
+    mine.rest += s.rest;
+    mine.whole += s.whole;
+  }
+  double own = mine.rest;
+  double upto = lanes_upto(own), total = from_lane(upto, kWave - 1);
+  const bool left = total > 0.0;
+  if (!left) {
+    // nothing is left of the difference (the target equals the draft there): the target's row itself
+    ws.q = nullptr;
+    ws.without = kNoClass;
+    own = mine.whole;
+    upto = lanes_upto(own);
+    total = from_lane(upto, kWave - 1);
+  }
+  const double border = u * total;
+  const int at = lane_at(own, upto, border);
+  if (at < 0) return kNoClass;
+  uint32_t block = from_lane(b0, at);
+  double before = from_lane(upto - own, at);
+  if (each > 1u) {  // among that lane's blocks in turn
+    const uint32_t end = from_lane(b1, at);
+    double run = before;
+    for (uint32_t i = block; i < end; ++i) {
+      const BlockSum s = sums[i];
+      const double w = left ? s.rest : s.whole;
+      if (w > 0.0) {
+        block = i;
+        before = run;
+        if (run + w > border) break;
+      }
+      run += w;
+    }
+  }
+  // among the lanes' eight groups of the block each, which lie side by side
+  const uint32_t g0 = block * kBlockGroups + lane * uint32_t(kOwn);
+  const uint32_t whole = rg.n / 4u;
+  const float *qs = ws.q != nullptr ? ws.q : ws.p;
+  own = 0.0;
+  if (whole != 0u) {
+#pragma unroll
+    for (int half = 0; half < kOwn; half += 4) {
+      // (a group past the row's whole ones reads the last of them again: no branch, so the loads are on their way together)
+      u32x4 p[4], q[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const size_t at = size_t(min(g0 + uint32_t(half + i), whole - 1u)) * 4u;
+        p[i] = load_stream<0>(reinterpret_cast<const u32x4 *>(ws.p + at));
+        q[i] = load_stream<0>(reinterpret_cast<const u32x4 *>(qs + at));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t g = g0 + uint32_t(half + i);
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += ws.of(g * 4u + uint32_t(j), __uint_as_float(p[i][j]), __uint_as_float(q[i][j]));
+        own += g < whole ? sum : 0.0;
+      }
+    }
+  }
+  if (whole >= g0 && whole - g0 < uint32_t(kOwn)) {  // the row's last, shorter group is this lane's
+    for (uint32_t j = whole * 4u; j < rg.n; ++j) own += ws.of(j, ws.p[j], qs[j]);
+  }
+  upto = before + lanes_upto(own);
+  const int run = lane_at(own, upto, border);
+  if (run < 0) return kNoClass;  // (not reached: the block weighs)
+  // among those 32 classes, one a lane
+  before = from_lane(upto - own, run);
+  const uint32_t first = (block * kBlockGroups + uint32_t(run) * uint32_t(kOwn)) * 4u, j = first + lane;
+  own = lane < 4u * uint32_t(kOwn) && j < rg.n ? ws.of(j, ws.p[j], qs[j]) : 0.0;
+  upto = before + lanes_upto(own);
+  const int last = lane_at(own, upto, border);
+  return last < 0 ? kNoClass : first + uint32_t(last);
+}
+
+// What a sequence gets, by one whole wave.
+__device__ inline void write_tokens(const Drafts &d, size_t b, uint32_t taken, uint32_t drawn, uint32_t *out, uint32_t *accepted) {
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+  if (lane == 0u) accepted[b] = taken;
+  for (uint64_t i = lane; i <= d.drafted; i += kWave) {
+    out[b * (size_t(d.drafted) + 1u) + i] = i < taken ? d.token[b * d.drafted + i] : i == taken ? drawn : kNoClass;
+  }
+}
+
+// One workgroup a sequence: its waves sum the row's blocks in turn, the first of them draws the token.
+template <int THREADS, int NT>
+__global__ __launch_bounds__(THREADS) void verify_kernel(Drafts d, uint32_t sequences, uint32_t blocks,
+                                                         const float *__restrict__ pick, uint32_t *__restrict__ out,
+                                                         uint32_t *__restrict__ accepted) {
+  __shared__ BlockSum sums[kMostHeld];
+  const RowGroups<float> rg(d.n, 0u);
+  for (size_t b = blockIdx.x; b < sequences; b += gridDim.x) {
+    uint32_t length;
+    const uint32_t taken = taken_tokens(d, b, length);
+    const Weights ws = weights_of(d, b, taken, taken < length);
+    for (uint32_t i = threadIdx.x / kWave; i < blocks; i += THREADS / kWave) {
+      const BlockSum s = ws.q != nullptr ? sum_block<true, NT>(rg, ws, i * kBlockGroups) : sum_block<false, NT>(rg, ws, i * kBlockGroups);
+      if ((threadIdx.x & (kWave - 1)) == 0) sums[i] = s;
+    }
+    __syncthreads();
+    if (threadIdx.x < uint32_t(kWave)) {
+      write_tokens(d, b, taken, draw_token(rg, ws, blocks, sums, double(pick[b])), out, accepted);
+    }
+    __syncthreads();
+  }
+}
+
+// What the summing kernel leaves for the drawing kernel.
+struct Sums {
+  BlockSum *block;   // [blocks, sequences]
+  uint32_t *taken;   // [sequences]: tokens taken, and the top bit where one was refused
+};
+constexpr uint32_t kRefused = 0x80000000u;
+
+// One wave a block of a sequence's row (every wave finds out for itself which row that is).
+template <int NT>
+__global__ __launch_bounds__(kDrawThreads) void draw_sums_kernel(Drafts d, uint32_t sequences, uint32_t blocks, Sums out) {
+  const RowGroups<float> rg(d.n, 0u);
+  const uint64_t items = uint64_t(sequences) * blocks;
+  for (uint64_t item = uint64_t(blockIdx.x) * kDrawWaves + threadIdx.x / kWave; item < items;
+       item += uint64_t(gridDim.x) * kDrawWaves) {
+    const size_t b = item / blocks;
+    const uint32_t i = uint32_t(item % blocks);
+    uint32_t length;
+    const uint32_t taken = taken_tokens(d, b, length);
+    const bool refused = taken < length;
+    const bool lead = (threadIdx.x & (kWave - 1)) == 0;
+    if (i == 0u && lead) out.taken[b] = taken | (refused ? kRefused : 0u);
+    const Weights ws = weights_of(d, b, taken, refused);
+    const BlockSum s = ws.q != nullptr ? sum_block<true, NT>(rg, ws, i * kBlockGroups) : sum_block<false, NT>(rg, ws, i * kBlockGroups);
+    if (lead) out.block[item] = s;
+  }
+}
+
+// One wave a sequence.
 __global__ __launch_bounds__(kWave) void draw_kernel(Drafts d, uint32_t sequences, uint32_t blocks, Sums in,
                                                      const float *__restrict__ pick, uint32_t *__restrict__ out,
                                                      uint32_t *__restrict__ accepted) {
-  constexpr int kOwn = int(kBlockGroups) / kWave;
-  const uint32_t lane = threadIdx.x;
   const RowGroups<float> rg(d.n, 0u);
-  const uint32_t each = (blocks + kWave - 1u) / kWave;  // blocks of a lane
   for (size_t b = blockIdx.x; b < sequences; b += gridDim.x) {
     const uint32_t word = in.taken[b], taken = word & ~kRefused;
-    const double u = double(pick[b]);
-    const uint32_t b0 = min(blocks, lane * each), b1 = min(blocks, b0 + each);
-    double own_rest = 0.0, own_whole = 0.0;
-    for (uint32_t i = b0; i < b1; ++i) {
-      const BlockSum s = in.block[b * blocks + i];
-      own_rest += s.rest;
-      own_whole += s.whole;
-    }
-    Weights ws = weights_of(d, b, taken, (word & kRefused) != 0u);
-    double total, own = own_rest;
-    double upto = lanes_upto(own, total);
-    const bool left = total > 0.0;
-    if (!left) {
-      // nothing is left of the difference (the target equals the draft there): the target's row itself
-      ws.q = nullptr;
-      ws.without = kNoClass;
-      own = own_whole;
-      upto = lanes_upto(own, total);
-    }
-    const double border = u * total;
-    uint32_t drawn = kNoClass;
-    const int at = lane_at(own, upto, border);
-    if (at >= 0) {
-      // among that lane's blocks in turn
-      double before = __shfl(upto - own, at, kWave);
-      const uint32_t first = uint32_t(__shfl(int(b0), at, kWave)), end = uint32_t(__shfl(int(b1), at, kWave));
-      uint32_t block = first;
-      double before_block = before;
-      for (uint32_t i = first; i < end; ++i) {
-        const BlockSum s = in.block[b * blocks + i];
-        const double w = left ? s.rest : s.whole;
-        if (w > 0.0) {
-          block = i;
-          before_block = before;
-          if (before + w > border) break;
-        }
-        before += w;
-      }
-      // a lane's eight groups of the block, which lie side by side
-      const uint32_t g0 = block * kBlockGroups + lane * uint32_t(kOwn);
-      double w[4 * kOwn];
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) {
-        const uint32_t g = g0 + uint32_t(i);
-        float p[4] = {0.0f, 0.0f, 0.0f, 0.0f}, q[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (g < rg.groups) {
-          load_group<float, 0>(rg, ws.p, g, 0.0f, p);
-          if (ws.q != nullptr) load_group<float, 0>(rg, ws.q, g, 0.0f, q);
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[4 * i + j] = ws.of(rg.first(g) + uint32_t(j), p[j], q[j]);
-      }
-      own = 0.0;
-#pragma unroll
-      for (int i = 0; i < 4 * kOwn; ++i) own += w[i];
-      upto = before_block + lanes_upto(own, total);
-      const int last = lane_at(own, upto, border);
-      double run = upto - own;
-      bool done = false;
-#pragma unroll
-      for (int i = 0; i < 4 * kOwn; ++i) {
-        if (!done && w[i] > 0.0) {
-          drawn = g0 * 4u + uint32_t(i);
-          run += w[i];
-          done = run > border;
-        }
-      }
-      drawn = uint32_t(__shfl(int(drawn), last, kWave));  // (a block that weighs has a lane that does)
-    }
-    if (lane == 0u) accepted[b] = taken;
-    for (uint64_t i = lane; i <= d.drafted; i += kWave) {
-      out[b * (size_t(d.drafted) + 1u) + i] = i < taken ? d.token[b * d.drafted + i] : i == taken ? drawn : kNoClass;
-    }
+    const Weights ws = weights_of(d, b, taken, (word & kRefused) != 0u);
+    write_tokens(d, b, taken, draw_token(rg, ws, blocks, in.block + b * blocks, double(pick[b])), out, accepted);
   }
 }
 
@@ -273,21 +304,33 @@ ANODE_EXPORT int anode_gpu_verify_draft_packed_f32(uint32_t dim0, uint32_t dim1,
   if (dim1 >= kRefused) return refuse(__func__, "more drafted tokens than 2^31 - 1");
   const hipStream_t st = as_stream(stream);
   const uint32_t groups = dim0 / 4u + (dim0 % 4u != 0u);
-  const uint32_t blocks = groups / kBlockGroups + (groups % kBlockGroups != 0u);
-  // blocks of a wave: so many that the launch has eight waves a SIMD
-  const uint64_t waves = uint64_t(device_cu_count()) * 32u;
-  uint64_t each = uint64_t(dim2) * blocks / waves;
-  each = each < 1u ? 1u : each > blocks ? blocks : each;
-  const uint64_t runs = blocks != 0u ? (blocks + each - 1u) / each : 1u;
-  const size_t block_bytes = size_t(dim2) * blocks * sizeof(BlockSum);
-  ScratchLease scratch = acquire_scratch(st, block_bytes + size_t(dim2) * sizeof(uint32_t), __func__);
-  if (!scratch.ptr) return int(hipErrorOutOfMemory);
-  const Sums sums = {static_cast<BlockSum *>(scratch.ptr), reinterpret_cast<uint32_t *>(static_cast<char *>(scratch.ptr) + block_bytes)};
+  const uint32_t blocks = groups == 0u ? 1u : groups / kBlockGroups + (groups % kBlockGroups != 0u);
   const Drafts d = {dim0, dim1, target, draft, draft_token, draft_length, accept};
-  const uint64_t items = (uint64_t(dim2) * runs + kDrawWaves - 1u) / kDrawWaves;
   const uint64_t most = 1u << 24;
-  draw_sums_kernel<<<uint32_t(items < most ? items : most), kDrawThreads, 0, st>>>(d, dim2, blocks, uint32_t(each), sums);
-  draw_kernel<<<uint32_t(dim2 < most ? dim2 : most), kWave, 0, st>>>(d, dim2, blocks, sums, pick, token, accepted);
+  const uint32_t grid = dim2 < most ? dim2 : uint32_t(most);
+  // a token's rows are read once, past the caches where they are large (the model's other rows are not read at all)
+  const bool nt = (stream_policy(size_t(dim2) * dim0 * 2u * sizeof(float), tuning().reduce_nontemporal) & kNtLoad) != 0;
+  const uint32_t cus = uint32_t(device_cu_count());
+  if (blocks <= kMostHeld) {
+    // one launch, a workgroup a sequence, as wide as lets all of them run at once
+    auto go = [&](auto kernel, uint32_t threads) { kernel<<<grid, threads, 0, st>>>(d, dim2, blocks, pick, token, accepted); };
+    if (blocks <= 4u || dim2 > 2u * cus) {
+      nt ? go(verify_kernel<256, kNtLoad>, 256u) : go(verify_kernel<256, 0>, 256u);
+    } else if (dim2 > cus) {
+      nt ? go(verify_kernel<512, kNtLoad>, 512u) : go(verify_kernel<512, 0>, 512u);
+    } else {
+      nt ? go(verify_kernel<1024, kNtLoad>, 1024u) : go(verify_kernel<1024, 0>, 1024u);
+    }
+  } else {
+    const size_t block_bytes = size_t(dim2) * blocks * sizeof(BlockSum);
+    ScratchLease scratch = acquire_scratch(st, block_bytes + size_t(dim2) * sizeof(uint32_t), __func__);
+    if (!scratch.ptr) return int(hipErrorOutOfMemory);
+    const Sums sums = {static_cast<BlockSum *>(scratch.ptr), reinterpret_cast<uint32_t *>(static_cast<char *>(scratch.ptr) + block_bytes)};
+    const uint64_t items = (uint64_t(dim2) * blocks + kDrawWaves - 1u) / kDrawWaves;
+    auto go = [&](auto kernel) { kernel<<<uint32_t(items < most ? items : most), kDrawThreads, 0, st>>>(d, dim2, blocks, sums); };
+    nt ? go(draw_sums_kernel<kNtLoad>) : go(draw_sums_kernel<0>);
+    draw_kernel<<<grid, kWave, 0, st>>>(d, dim2, blocks, sums, pick, token, accepted);
+  }
   note_launch(__func__);
   return 0;
 }
