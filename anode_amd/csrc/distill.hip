@@ -29,33 +29,35 @@ struct Teacher {
 // value * inv_t - shift + log_scale.
 struct TeacherRow {
   double shift, log_scale, mass;
-  bool any;       // a slot counts
-  bool repeated;  // a class is named twice
+  bool any;  // a slot counts
 };
 
-// The slots of a row in LDS.
+// The slots of a row in LDS.  A streaming thread finds those that lie in its groups by a list of its own, and the turns of its
+// that have one by a bit mask, so that it takes their part off the values while it still has them in registers.
 struct Slots {
-  float *p;         // [k]: the probability; 0 for a slot that does not count
-  uint32_t *index;  // [k]: its class; kNoClass for a slot that does not count
-  float *x;         // [k]: the student's logit, read before dx (which may be x) is written; then the gradient there
-  float *old;       // [k]: what dx held (accumulating)
+  float *p;         // [k]: the probability
+  float *x;         // [k]: the student's logit
+  float *off;       // [k]: what is taken off the gradient of its class
+  uint32_t *index;  // [k]: the class; kNoClass for a slot that does not count
+  uint32_t *next;   // [k]: the next slot of the same thread, or kNoClass
+  uint32_t *head;   // [threads]: a thread's first slot, or kNoClass
+  uint32_t *turns;  // [threads]: bit i for a slot in the thread's groups of turn i, i + 32, ...
   uint32_t *seen;   // [kSeen], for k > 64: the classes met so far
 };
 constexpr uint32_t kSeen = 2u * kMaxSlots;
-__device__ inline Slots slots_in(uint32_t *lds, uint32_t k) {
+__device__ inline Slots slots_in(uint32_t *lds, uint32_t k, uint32_t threads) {
   float *f = reinterpret_cast<float *>(lds);
-  return Slots{f, lds + k, f + 2u * k, f + 3u * k, lds + 4u * k};
+  uint32_t *t = lds + 5u * k;
+  return Slots{f, f + k, f + 2u * k, lds + 3u * k, lds + 4u * k, t, t + threads, t + 2u * threads};
 }
-uint32_t slot_bytes(uint32_t k) { return 16u * k + (k > uint32_t(kWave) ? 4u * kSeen : 0u); }
+uint32_t slot_bytes(uint32_t k, uint32_t threads) { return 20u * k + 8u * threads + (k > uint32_t(kWave) ? 4u * kSeen : 0u); }
 
-// Reads the slots of a row, by one whole wave: x and dx are the row's; only classes in [from, from + count) are kept (the
-// mass is the whole row's).
-template <typename T, bool ACC>
-__device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x, const T *dx, uint32_t n, uint32_t from,
-                                        uint32_t count, double inv_t, const Slots &s) {
+// Reads the slots of a row, by one whole wave: x is the row, n its length.
+template <typename T>
+__device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x, uint32_t n, double inv_t, const Slots &s) {
   const uint32_t lane = threadIdx.x & (kWave - 1);
   const size_t first = row * t.k;
-  TeacherRow r = {0.0, 0.0, 0.0, false, false};
+  TeacherRow r = {0.0, 0.0, 0.0, false};
   float top = kMinusInf;
   for (uint32_t j = lane; j < t.k; j += kWave) {
     const uint32_t at = t.index[first + j];
@@ -64,7 +66,6 @@ __device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x
     s.index[j] = counts ? at : kNoClass;
     s.p[j] = v;
     s.x[j] = counts ? float(x[at]) : 0.0f;
-    if (ACC) s.old[j] = counts ? float(dx[at]) : 0.0f;
     if (counts) top = fmaxf(top, v);
   }
   top = wave_max(top);
@@ -77,7 +78,7 @@ __device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x
     s.p[j] = float(e);
     sum += e;
   }
-  sum = wave_sum(sum);
+  sum = lanes_sum(sum);
   r.mass = sum;
   if (t.log_norm == nullptr) {
     const float scale = float(1.0 / sum);
@@ -85,40 +86,81 @@ __device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x
     r.mass = 1.0;
     r.log_scale = -log(sum);
   }
-  // whether a class is named twice: among 64 slots by comparing, beyond in a table
-  if (t.k <= uint32_t(kWave)) {
-    const uint32_t mine = lane < t.k ? s.index[lane] : kNoClass;
-    bool twice = false;
-    for (uint32_t i = 0; i < t.k; ++i) {
-      const uint32_t other = uint32_t(__builtin_amdgcn_readlane(int(mine), int(i)));
-      twice |= other == mine && i != lane;
+  return r;
+}
+
+// Whether a class is named twice, by the wave that read the slots: among 64 slots by comparing, beyond in a table.
+__device__ inline bool repeated_slots(uint32_t k, const Slots &s) {
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+  bool twice = false;
+  if (k <= uint32_t(kWave)) {
+    const uint32_t mine = lane < k ? s.index[lane] : kNoClass;
+    for (uint32_t i = 0; i < k; ++i) twice |= from_lane(mine, int(i)) == mine && i != lane;
+    return __any(twice && mine != kNoClass);
+  }
+  for (uint32_t i = lane; i < kSeen; i += kWave) s.seen[i] = kNoClass;
+  for (uint32_t j = lane; j < k; j += kWave) {
+    const uint32_t mine = s.index[j];
+    if (mine == kNoClass) continue;
+    uint32_t at = (mine * 2654435761u) >> 21;  // (kSeen = 2^11 places, at most half of them taken)
+    for (;;) {
+      const uint32_t held = atomicCAS(&s.seen[at], kNoClass, mine);
+      if (held == kNoClass) break;
+      if (held == mine) {
+        twice = true;
+        break;
+      }
+      at = (at + 1u) & (kSeen - 1u);
     }
-    r.repeated = __any(twice && mine != kNoClass);
-  } else {
-    for (uint32_t i = lane; i < kSeen; i += kWave) s.seen[i] = kNoClass;
-    bool twice = false;
-    for (uint32_t j = lane; j < t.k; j += kWave) {
-      const uint32_t mine = s.index[j];
-      if (mine == kNoClass) continue;
-      uint32_t at = (mine * 2654435761u) >> 21;  // (kSeen = 2^11 places, at most half of them taken)
-      for (;;) {
-        const uint32_t held = atomicCAS(&s.seen[at], kNoClass, mine);
-        if (held == kNoClass) break;
-        if (held == mine) {
-          twice = true;
-          break;
-        }
-        at = (at + 1u) & (kSeen - 1u);
+  }
+  return __any(twice);
+}
+
+// Deals the slots that lie in [from, from + n of the span) of the row to the streaming threads, w times their
+// probability each; by the wave that read them.  A class that is named more than once gets all of its mass from the first
+// slot that names it, added in slot order.
+template <typename T, int THREADS>
+__device__ inline void deal_slots(uint32_t k, bool any, const RowSpan<T> &span, uint32_t from, double w, const Slots &s) {
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+  const uint32_t end = span.head + span.groups * uint32_t(RowSpan<T>::W);
+  for (uint32_t i = lane; i < uint32_t(THREADS); i += kWave) {
+    s.head[i] = kNoClass;
+    s.turns[i] = 0u;
+  }
+  if (!any) return;
+  const bool repeated = repeated_slots(k, s);
+  for (uint32_t j = lane; j < k; j += kWave) {
+    const uint32_t at = s.index[j] - from;
+    s.next[j] = kNoClass;
+    double p = double(s.p[j]);
+    bool mine = s.index[j] != kNoClass && at < end + span.tail;  // (a class below `from` wraps)
+    if (repeated && mine) {
+      p = 0.0;
+      for (uint32_t i = 0; i < k; ++i) {
+        if (s.index[i] != s.index[j]) continue;
+        if (i < j) mine = false;
+        p += double(s.p[i]);
       }
     }
-    r.repeated = __any(twice);
+    s.off[j] = float(w * p);
+    if (!mine) continue;
+    const bool single = at < span.head || at >= end;
+    const uint32_t place = single ? (at < span.head ? at : at - end + span.head) : (at - span.head) / uint32_t(RowSpan<T>::W);
+    const uint32_t thread = place % uint32_t(THREADS);
+    s.next[j] = atomicExch(&s.head[thread], j);
+    if (!single) atomicOr(&s.turns[thread], 1u << (place / uint32_t(THREADS) & 31u));
   }
-  if (from != 0u || count != n) {
-    for (uint32_t j = lane; j < t.k; j += kWave) {
-      if (s.index[j] - from >= count) s.index[j] = kNoClass;  // (below `from` the difference wraps)
-    }
+}
+
+// Takes the slots of the thread's list that lie in the W classes from `first` on off their values.
+template <int W>
+__device__ inline void take_slots(const Slots &s, uint32_t first, float (&v)[W]) {
+  for (uint32_t j = s.head[threadIdx.x]; j != kNoClass; j = s.next[j]) {
+    const uint32_t at = s.index[j] - first;
+    const float off = s.off[j];
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] -= at == uint32_t(i) ? off : 0.0f;
   }
-  return r;
 }
 
 // The row's loss from its slots in LDS, by the wave that read them.
@@ -132,17 +174,34 @@ __device__ inline float slots_loss(const Teacher &t, size_t row, SoftmaxSum st, 
     const double lp = double(t.value[row * t.k + j]) * inv_t - tr.shift + tr.log_scale;
     loss += double(p) * (lp - ((double(s.x[j]) - double(st.m)) * inv_t - log_s));
   }
-  return float(wave_sum(loss));
+  return float(lanes_sum(loss));
 }
 
-// The row's loss straight from memory, by one whole wave.
+// A lane's slot of a row: the first 64 slots are asked for before the row is streamed, so that their chain of loads (class,
+// logit) is over when the statistics are there.
+struct LaneSlot {
+  float value, x;
+  bool counts;
+};
 template <typename T>
-__device__ inline float row_loss(const Teacher &t, size_t row, const T *x, uint32_t n, SoftmaxSum st, double inv_t) {
+__device__ inline LaneSlot lane_slot(const Teacher &t, size_t row, const T *x, uint32_t n, uint32_t j) {
+  LaneSlot s = {kMinusInf, 0.0f, false};
+  if (j < t.k) {
+    const uint32_t at = t.index[row * t.k + j];
+    s.value = t.value[row * t.k + j];
+    s.counts = at < n && s.value > kMinusInf;
+    if (s.counts) s.x = float(x[at]);
+  }
+  return s;
+}
+
+// The row's loss straight from memory, by one whole wave; `mine` is its lanes' first slots.
+template <typename T>
+__device__ inline float row_loss(const Teacher &t, size_t row, const T *x, uint32_t n, SoftmaxSum st, double inv_t, LaneSlot mine) {
   const uint32_t lane = threadIdx.x & (kWave - 1);
-  const size_t first = row * t.k;
-  float top = kMinusInf;
-  for (uint32_t j = lane; j < t.k; j += kWave) {
-    if (t.counts(first + j, n)) top = fmaxf(top, t.value[first + j]);
+  float top = mine.counts ? mine.value : kMinusInf;
+  for (uint32_t j = lane + kWave; j < t.k; j += kWave) {
+    if (t.counts(row * t.k + j, n)) top = fmaxf(top, t.value[row * t.k + j]);
   }
   top = wave_max(top);
   if (!(top > kMinusInf)) return 0.0f;
@@ -151,15 +210,16 @@ __device__ inline float row_loss(const Teacher &t, size_t row, const T *x, uint3
   const double log_s = log(double(st.s));
   double mass = 0.0, loss = 0.0;
   for (uint32_t j = lane; j < t.k; j += kWave) {
-    if (!t.counts(first + j, n)) continue;
-    const double a = double(t.value[first + j]) * inv_t - shift, e = exp(a);
-    const double lq = (double(float(x[t.index[first + j]])) - double(st.m)) * inv_t - log_s;
+    const LaneSlot s = j == lane ? mine : lane_slot(t, row, x, n, j);
+    if (!s.counts) continue;
+    const double a = double(s.value) * inv_t - shift, e = exp(a);
+    const double lq = (double(s.x) - double(st.m)) * inv_t - log_s;
     if (e != 0.0) loss += e * (a - lq);  // (a slot without mass adds nothing, whatever the student says)
     mass += e;
   }
-  loss = wave_sum(loss);
+  loss = lanes_sum(loss);
   if (t.log_norm == nullptr) {
-    mass = wave_sum(mass);
+    mass = lanes_sum(mass);
     loss = loss / mass - log(mass);
   }
   return float(loss);
@@ -183,10 +243,12 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(uint32_t n, uint32_t r
   __shared__ SoftmaxSum lds[THREADS / kWave];
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T *xr = x + r * stride;
+    LaneSlot slot = {};
+    if (threadIdx.x < uint32_t(kWave)) slot = lane_slot(t, r, xr, n, threadIdx.x);
     const SoftmaxSum st =
         finish_stats<T, THREADS>(stream_stats<T, THREADS, kUnroll, NT>(RowSpan<T>(n, 0u), xr, sc), xr, n, sc, lds);
     if (threadIdx.x < uint32_t(kWave)) {
-      const float l = row_loss(t, r, xr, n, st, inv_t);
+      const float l = row_loss(t, r, xr, n, st, inv_t, slot);
       if (threadIdx.x == 0) {
         loss[r] = l;
         row_max[r] = st.m;
@@ -229,8 +291,9 @@ __global__ __launch_bounds__(kWave) void distill_join_kernel(uint32_t n, uint32_
                                                              float *__restrict__ row_max, float *__restrict__ row_sum) {
   __shared__ float lds[1];
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const LaneSlot slot = lane_slot(t, r, x + r * stride, n, threadIdx.x);
     const SoftmaxSum st = join_parts<T, kWave>(partial + r * parts, parts, x + r * stride, n, sc, lds);
-    const float l = row_loss(t, r, x + r * stride, n, st, inv_t);
+    const float l = row_loss(t, r, x + r * stride, n, st, inv_t, slot);
     if (threadIdx.x == 0) {
       loss[r] = l;
       row_max[r] = st.m;
@@ -262,27 +325,29 @@ __device__ inline float any_term(float x, const Dense &d) {
   return d.any ? __builtin_amdgcn_exp2f((x - d.m) * d.c) * d.scale : 0.0f;
 }
 
-// The single values of a span.
+// The single values of a span; `at` of the slots' classes counts from the row's start, the span starts at `from`.
 template <typename T, int THREADS, bool ACC>
-__device__ inline void single_grad(const RowSpan<T> &span, const T *x, T *dx, const Dense &d) {
+__device__ inline void single_grad(const RowSpan<T> &span, const T *x, T *dx, uint32_t from, const Dense &d, const Slots &slots) {
 #pragma unroll 1
   for (uint32_t i = threadIdx.x; span.single(i); i += THREADS) {
     const uint32_t at = span.single_at(i);
-    float v = any_term(float(x[at]), d);
-    if (ACC) v += float(dx[at]);
-    dx[at] = T(v);
+    float v[1] = {any_term(float(x[at]), d)};
+    if (ACC) v[0] += float(dx[at]);
+    take_slots(slots, from + at, v);
+    dx[at] = T(v[0]);
   }
 }
 
-// The dense part of dx over a span, streamed.  Every thread reads and writes its own groups only, in turn, so dx
-// may be x.
+// The groups of a span, streamed; q holds the thread's first tile already.  Every thread reads and writes its own groups only,
+// in turn, so dx may be x.
 template <typename T, int THREADS, int U, bool ACC, int NT, bool FAST>
-__device__ inline void stream_groups(const RowSpan<T> &span, const T *x, T *dx, const Dense &d) {
+__device__ inline void stream_groups(const RowSpan<T> &span, const T *x, T *dx, uint32_t from, const Dense &d, const Slots &slots,
+                                     u32x4 (&q)[U]) {
   constexpr int W = Group<T>::W;
   constexpr uint32_t kTile = uint32_t(THREADS) * uint32_t(U);
   if (span.groups == 0u) return;
-  u32x4 q[U];
-  load_tile<T, THREADS, U, 0>(span, x, threadIdx.x, q);
+  const uint32_t turns = slots.turns[threadIdx.x];
+  uint32_t turn = 0u;
   for (uint32_t base = 0;; base += kTile) {
     const uint32_t g = base + threadIdx.x;
     u32x4 old[U], next[U];
@@ -290,64 +355,22 @@ __device__ inline void stream_groups(const RowSpan<T> &span, const T *x, T *dx, 
     if (ACC) load_tile<T, THREADS, U, 0>(span, dx, g, old);
     load_tile<T, THREADS, U, 0>(span, x, g + kTile, next);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < U; ++u, ++turn) {
       float v[W], o[W];
       unpack(q[u], v, x);
       if (ACC) unpack(old[u], o, x);
+      const uint32_t at = g + uint32_t(u) * uint32_t(THREADS);
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         v[j] = FAST ? fast_term(v[j], d) : any_term(v[j], d);
         if (ACC) v[j] += o[j];
       }
-      const uint32_t at = g + uint32_t(u) * uint32_t(THREADS);
+      if ((turns >> (turn & 31u) & 1u) != 0u) take_slots(slots, from + span.first(at), v);
       if (at < span.groups) store_group<NT, int(sizeof(T))>(dx + size_t(span.first(at)), pack(v, dx));
     }
     if (!more) break;
 #pragma unroll
     for (int u = 0; u < U; ++u) q[u] = next[u];
-  }
-}
-template <typename T, int THREADS, bool ACC, int NT>
-__device__ inline void stream_grad(const RowSpan<T> &span, const T *x, T *dx, const Dense &d) {
-  single_grad<T, THREADS, ACC>(span, x, dx, d);
-  if (d.fast) {
-    stream_groups<T, THREADS, kUnroll, ACC, NT, true>(span, x, dx, d);
-  } else {
-    stream_groups<T, THREADS, kUnroll, ACC, 0, false>(span, x, dx, d);
-  }
-}
-
-// The gradient at the classes that slots name, into slots.x, by the wave that read the slots.
-__device__ inline void slot_grads(uint32_t k, SoftmaxSum st, double inv_t, double w, const TeacherRow &tr, const Slots &s) {
-  if (!tr.any) return;
-  for (uint32_t j = threadIdx.x & (kWave - 1); j < k; j += kWave) {
-    if (s.index[j] == kNoClass) continue;
-    const double q = exp((double(s.x[j]) - double(st.m)) * inv_t) / double(st.s);
-    double p = double(s.p[j]);
-    if (tr.repeated) {  // all of the class's mass, added in slot order whichever of its slots does it
-      p = 0.0;
-      for (uint32_t i = 0; i < k; ++i) p += s.index[i] == s.index[j] ? double(s.p[i]) : 0.0;
-    }
-    s.x[j] = float(w * (tr.mass * q - p));
-  }
-}
-// ... and from there to dx.  A class is stored by the wave that stored the 16-byte group it lies in (threads take groups in
-// turn, `held` groups first where a kernel keeps that many in registers), so that a wave's own order of stores decides.
-// Slots that name one class write the same value.
-template <typename T, int THREADS, bool ACC>
-__device__ inline void store_slots(uint32_t k, T *dx, uint32_t from, const RowSpan<T> &span, uint32_t held, const Slots &s) {
-#pragma unroll 1
-  for (uint32_t j = threadIdx.x & (kWave - 1); j < k; j += kWave) {
-    if (s.index[j] == kNoClass) continue;
-    const uint32_t at = s.index[j] - from, end = span.head + span.groups * uint32_t(RowSpan<T>::W);
-    uint32_t turn;
-    if (at < span.head || at >= end) {
-      turn = at < span.head ? at : at - end + span.head;
-    } else {
-      turn = (at - span.head) / uint32_t(RowSpan<T>::W);
-      if (turn >= held) turn -= held;
-    }
-    if (turn % uint32_t(THREADS) / kWave == threadIdx.x / kWave) dx[from + at] = T(ACC ? s.old[j] + s.x[j] : s.x[j]);
   }
 }
 
@@ -357,15 +380,22 @@ struct RowShared {
   int any;
 };
 
-// One workgroup a part of a row.
-template <typename T, int THREADS, bool ACC, int NT>
+// What a pass over the parts of rows left (part_stats_kernel), and where the rows' results go.
+struct Joined {
+  const SoftmaxSum *partial;  // null: row_max and row_sum are inputs
+  float *loss, *row_max, *row_sum;
+};
+
+// One workgroup a part of a row.  JOIN: the row's statistics are put together from its parts by every workgroup for itself, and
+// the first part's writes them and the loss.
+template <typename T, int THREADS, bool ACC, bool JOIN, int NT>
 __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32_t rows, size_t stride, Scale sc, double inv_t,
                                                               Parts ps, const float *__restrict__ dy, const T *x, Teacher t,
-                                                              const float *__restrict__ row_max,
-                                                              const float *__restrict__ row_sum, T *dx) {
+                                                              Joined jn, T *dx) {
   extern __shared__ uint32_t slot_lds[];
   __shared__ RowShared rs;
-  const Slots slots = slots_in(slot_lds, t.k);
+  __shared__ float plain_lds[THREADS / kWave];
+  const Slots slots = slots_in(slot_lds, t.k, THREADS);
   const uint64_t items = uint64_t(rows) * ps.parts;
   for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
     const size_t r = i / ps.parts;
@@ -373,26 +403,47 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32
     const uint32_t from = ps.first(part), count = ps.count(part, n);
     const T *xr = x + r * stride;
     T *dxr = dx + r * stride;
-    const SoftmaxSum st = {row_max[r], row_sum[r]};
+    const RowSpan<T> span(count, values_to_line(dxr + from));
+    u32x4 q[kUnroll];
+    if (span.groups != 0u) load_tile<T, THREADS, kUnroll, 0>(span, xr + from, threadIdx.x, q);
+    SoftmaxSum st;
+    if (JOIN) {
+      st = join_parts<T, THREADS>(jn.partial + r * ps.parts, ps.parts, xr, n, sc, plain_lds);
+    } else {
+      st = SoftmaxSum{jn.row_max[r], jn.row_sum[r]};
+    }
     const double w = double(dy[r]) * inv_t;
     if (threadIdx.x < uint32_t(kWave)) {
-      const TeacherRow tr = read_slots<T, ACC>(t, r, xr, dxr, n, from, count, inv_t, slots);
+      const TeacherRow tr = read_slots(t, r, xr, n, inv_t, slots);
       if (threadIdx.x == 0) rs = RowShared{float(tr.mass), tr.any};
-      slot_grads(t.k, st, inv_t, w, tr, slots);
+      deal_slots<T, THREADS>(t.k, tr.any, span, from, w, slots);
+      if (JOIN && part == 0u) {
+        const float l = slots_loss(t, r, st, inv_t, tr, slots);
+        if (threadIdx.x == 0) {
+          jn.loss[r] = l;
+          jn.row_max[r] = st.m;
+          jn.row_sum[r] = st.s;
+        }
+      }
     }
     __syncthreads();
     const Dense d = dense_of(st, sc, float(w), rs.mass, rs.any != 0);
-    const RowSpan<T> span(count, values_to_line(dxr + from));
-    if (!ACC || d.any) stream_grad<T, THREADS, ACC, NT>(span, xr + from, dxr + from, d);
-    if (d.any) store_slots<T, THREADS, ACC>(t.k, dxr, from, span, 0xffffffffu, slots);
+    if (!ACC || d.any) {
+      single_grad<T, THREADS, ACC>(span, xr + from, dxr + from, from, d, slots);
+      if (d.fast) {
+        stream_groups<T, THREADS, kUnroll, ACC, NT, true>(span, xr + from, dxr + from, from, d, slots, q);
+      } else {
+        stream_groups<T, THREADS, kUnroll, ACC, 0, false>(span, xr + from, dxr + from, from, d, slots, q);
+      }
+    }
     __syncthreads();
   }
 }
 
 // Loss and gradient, one workgroup a row: the first G groups of each streaming thread stay in registers from the statistics
-// to the gradient, so that x is read once (what lies behind them is streamed a second time).  The
-// slots belong to a wave of their own: their 64-bit exponentials and logarithms would spill the held registers of a
-// wave that streams, and take about as long as a small row.
+// to the gradient, so that x is read once (what lies behind them is streamed a second time).  The slots belong to a wave of
+// their own: their 64-bit exponentials and logarithms would spill the held registers of a wave that streams, and take
+// about as long as a small row.
 template <typename T, int S, int G, int NT>
 __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) void distill_held_kernel(
     uint32_t n, uint32_t rows, size_t stride, Scale sc, double inv_t, const T *x, Teacher t, const float *__restrict__ dy,
@@ -401,11 +452,12 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
   constexpr int THREADS = S + kWave;
   constexpr int WAVES = S / kWave;
   constexpr uint32_t kHeld = uint32_t(S) * uint32_t(G);
+  static_assert(G % 2 == 0 && G <= 32, "two groups are folded together; a bit of Slots::turns for each");
   extern __shared__ uint32_t slot_lds[];
   __shared__ SoftmaxSum parts[WAVES];
   __shared__ float plain_lds[WAVES + 1];
   __shared__ RowShared rs;
-  const Slots slots = slots_in(slot_lds, t.k);
+  const Slots slots = slots_in(slot_lds, t.k, S);
   // the row's statistics, by every wave alike
   auto joined = [&](const T *xr) {
     const SoftmaxSum st = lane_merge<WAVES>(parts, sc.c);
@@ -415,10 +467,10 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
   if (threadIdx.x >= uint32_t(S)) {
     for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
       const T *xr = x + r * stride;
-      const TeacherRow tr = read_slots<T, false>(t, r, xr, dx + r * stride, n, 0u, n, inv_t, slots);
+      const TeacherRow tr = read_slots(t, r, xr, n, inv_t, slots);
       if (threadIdx.x == uint32_t(S)) rs = RowShared{float(tr.mass), tr.any};
-      const double w = double(dy[r]) * inv_t;
-      __syncthreads();  // 1: the parts and the mass are there
+      deal_slots<T, S>(t.k, tr.any, RowSpan<T>(n, values_to_line(dx + r * stride)), 0u, double(dy[r]) * inv_t, slots);
+      __syncthreads();  // 1: the parts, the mass and the lists are there
       const SoftmaxSum st = joined(xr);
       const float l = slots_loss(t, r, st, inv_t, tr, slots);
       if (threadIdx.x == uint32_t(S)) {
@@ -426,9 +478,7 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
         row_max[r] = st.m;
         row_sum[r] = st.s;
       }
-      slot_grads(t.k, st, inv_t, w, tr, slots);
-      __syncthreads();  // 2: the slots' gradients are there
-      __syncthreads();  // 3: and stored
+      __syncthreads();  // 2: all of it is done with
     }
     return;
   }
@@ -473,16 +523,20 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
 #pragma unroll
     for (int u = 0; u < G; ++u) forget(q[u]);
     const Dense d = dense_of(st, sc, w, rs.mass, rs.any != 0);
-    single_grad<T, S, false>(span, xr, dxr, d);
-    if (d.fast) {
+    const uint32_t turns = slots.turns[threadIdx.x];
+    single_grad<T, S, false>(span, xr, dxr, 0u, d, slots);
+    // the groups behind the held ones, or, of a row that the fast form does not measure, all of them
+    uint32_t turn = d.fast ? uint32_t(G) : 0u;
 #pragma unroll 1
-      for (uint32_t g = kHeld + threadIdx.x; g < span.groups; g += S) {
-        float v[W];
-        unpack(load_stream<0, int(sizeof(T))>(reinterpret_cast<const u32x4 *>(xr + size_t(span.first(g)))), v, x);
+    for (uint32_t g = turn * uint32_t(S) + threadIdx.x; g < span.groups; g += S, ++turn) {
+      float v[W];
+      unpack(load_stream<0, int(sizeof(T))>(reinterpret_cast<const u32x4 *>(xr + size_t(span.first(g)))), v, x);
 #pragma unroll
-        for (int j = 0; j < W; ++j) v[j] = fast_term(v[j], d);
-        store_group<0, int(sizeof(T))>(dxr + size_t(span.first(g)), pack(v, dx));
-      }
+      for (int j = 0; j < W; ++j) v[j] = any_term(v[j], d);
+      if ((turns >> (turn & 31u) & 1u) != 0u) take_slots(slots, span.first(g), v);
+      store_group<0, int(sizeof(T))>(dxr + size_t(span.first(g)), pack(v, dx));
+    }
+    if (d.fast) {
       const GroupBuffer db(dxr + span.head, min(span.groups, kHeld));
 #pragma unroll
       for (int u = 0; u < G; ++u) {
@@ -490,21 +544,11 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
         unpack(q[u], v, x);
 #pragma unroll
         for (int j = 0; j < W; ++j) v[j] = fast_term(v[j], d);
+        if ((turns >> u & 1u) != 0u) take_slots(slots, span.first(uint32_t(u) * uint32_t(S) + threadIdx.x), v);
         db.store<NT>(pack(v, dx), mine, uint32_t(u) * kStep);
-      }
-    } else {
-#pragma unroll 1
-      for (uint32_t g = threadIdx.x; g < span.groups; g += S) {
-        float v[W];
-        unpack(load_stream<0, int(sizeof(T))>(reinterpret_cast<const u32x4 *>(xr + size_t(span.first(g)))), v, x);
-#pragma unroll
-        for (int j = 0; j < W; ++j) v[j] = any_term(v[j], d);
-        store_group<0, int(sizeof(T))>(dxr + size_t(span.first(g)), pack(v, dx));
       }
     }
     __syncthreads();  // 2
-    if (d.any) store_slots<T, S, false>(t.k, dxr, 0u, span, kHeld, slots);
-    __syncthreads();  // 3
   }
 }
 
@@ -516,15 +560,16 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(4))) void
   constexpr int W = Group<T>::W;
   extern __shared__ uint32_t slot_lds[];
   __shared__ SoftmaxSum lds[1];
-  const Slots slots = slots_in(slot_lds, t.k);
+  const Slots slots = slots_in(slot_lds, t.k, kWave);
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T *xr = x + r * stride;
     T *dxr = dx + r * stride;
     const RowSpan<T> span(n, values_to_line(dxr));
     u32x4 q[G];
     if (span.groups != 0u) load_tile<T, kWave, G, 0>(span, xr, threadIdx.x, q);
-    const TeacherRow tr = read_slots<T, false>(t, r, xr, dxr, n, 0u, n, inv_t, slots);
     const double w = double(dy[r]) * inv_t;
+    const TeacherRow tr = read_slots(t, r, xr, n, inv_t, slots);
+    deal_slots<T, kWave>(t.k, tr.any, span, 0u, w, slots);
     SoftmaxSum st = {-sc.limit, 0.0f};
     for (uint32_t i = threadIdx.x; span.single(i); i += kWave) fold_one(st, float(xr[span.single_at(i)]), sc.c);
     if (span.groups != 0u) {
@@ -540,9 +585,10 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(4))) void
       row_max[r] = st.m;
       row_sum[r] = st.s;
     }
-    slot_grads(t.k, st, inv_t, w, tr, slots);
+    __syncthreads();
     const Dense d = dense_of(st, sc, float(w), float(tr.mass), tr.any);
-    single_grad<T, kWave, false>(span, xr, dxr, d);
+    const uint32_t turns = slots.turns[threadIdx.x];
+    single_grad<T, kWave, false>(span, xr, dxr, 0u, d, slots);
 #pragma unroll
     for (int u = 0; u < G; ++u) {
       const uint32_t at = uint32_t(u) * kWave + threadIdx.x;
@@ -550,9 +596,9 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(4))) void
       unpack(q[u], v, x);
 #pragma unroll
       for (int j = 0; j < W; ++j) v[j] = any_term(v[j], d);
+      if ((turns >> u & 1u) != 0u) take_slots(slots, span.first(at), v);
       if (at < span.groups) store_group<NT, int(sizeof(T))>(dxr + size_t(span.first(at)), pack(v, dx));
     }
-    if (d.any) store_slots<T, kWave, false>(t.k, dxr, 0u, span, 0xffffffffu, slots);
     __syncthreads();
   }
 }
@@ -583,14 +629,20 @@ int check_arrays(const char *symbol, const Shape &s, const T *x, const Teacher &
   return 0;
 }
 
+// Few long rows go in parts, each read a second time for the gradient: 14.8 against 18.7 us for 24 rows of 131072 bf16 logits.
+// At 64 rows the two are even, and shorter rows are quicker on one CU each (16 rows of 32768: 13.7 against 11.2 us).
+constexpr uint32_t kFewRows = 32;
+constexpr size_t kLongRow = 136192;  // bytes
+
 uint32_t grid_for(uint64_t items) { return items < (1u << 24) ? uint32_t(items) : (1u << 24); }
 
-// Parts of at least one tile of a workgroup (kBlock * kUnroll groups), no more than bring the launch to `target`
-// workgroups.
+// Parts of at least one tile of a workgroup (kBlock * kUnroll groups), no more than bring the launch to kWanted workgroups:
+// four a CU (1001 rows of 50257 halves: loss and gradient 58.6 us whole, 66.3 us in two and three parts).
+constexpr uint32_t kWanted = 1024;
 template <typename T>
-Parts cut_rows(const Shape &s, uint32_t target) {
+Parts cut_rows(const Shape &s) {
   const uint32_t tile = uint32_t(kBlock * kUnroll * Group<T>::W);
-  uint64_t parts = (uint64_t(target) + s.rows - 1u) / s.rows;
+  uint64_t parts = kWanted / s.rows;
   if (parts > s.n / tile) parts = s.n / tile;
   if (parts <= 1u) return Parts{1u, s.n};
   const uint64_t unit = 1024;  // parts start whole 128-byte lines into a row
@@ -606,7 +658,7 @@ int distill(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, f
   if (dim1 == 0u) return 0;
   if (const int e = check_arrays(symbol, s, x, t, {loss, row_max, row_sum})) return e;
   const hipStream_t st = as_stream(stream);
-  const Parts ps = cut_rows<T>(s, 1024u);
+  const Parts ps = cut_rows<T>(s);
   if (ps.parts > 1u) {
     ScratchLease scratch = acquire_scratch(st, size_t(s.rows) * ps.parts * sizeof(SoftmaxSum), symbol);
     if (!scratch.ptr) return int(hipErrorOutOfMemory);
@@ -628,14 +680,15 @@ int distill(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, f
 template <typename T, bool ACC, int NT>
 void launch_bwd(const Shape &s, const float *dy, const T *x, const Teacher &t, const float *row_max, const float *row_sum, T *dx,
                 hipStream_t st) {
-  const Parts ps = cut_rows<T>(s, 2048u);
+  const Parts ps = cut_rows<T>(s);
   const uint32_t grid = grid_for(uint64_t(s.rows) * ps.parts);
+  const Joined jn = {nullptr, nullptr, const_cast<float *>(row_max), const_cast<float *>(row_sum)};  // (read only)
   if (size_t(s.n) * sizeof(T) <= 16384u) {
-    distill_bwd_kernel<T, kWave, ACC, NT><<<grid, kWave, slot_bytes(t.k), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, ps, dy, x, t,
-                                                                               row_max, row_sum, dx);
+    distill_bwd_kernel<T, kWave, ACC, false, NT><<<grid, kWave, slot_bytes(t.k, kWave), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t,
+                                                                                             ps, dy, x, t, jn, dx);
   } else {
-    distill_bwd_kernel<T, kBlock, ACC, NT><<<grid, kBlock, slot_bytes(t.k), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, ps, dy, x,
-                                                                                 t, row_max, row_sum, dx);
+    distill_bwd_kernel<T, kBlock, ACC, false, NT><<<grid, kBlock, slot_bytes(t.k, kBlock), st>>>(s.n, s.rows, s.stride, s.sc,
+                                                                                                s.inv_t, ps, dy, x, t, jn, dx);
   }
 }
 
@@ -661,7 +714,8 @@ void launch_fused(const Shape &s, const T *x, const Teacher &t, const float *dy,
                   T *dx, hipStream_t st) {
   const size_t row = size_t(s.n) * sizeof(T);
   auto go = [&](auto kernel, uint32_t threads) {
-    kernel<<<grid_for(s.rows), threads, slot_bytes(t.k), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, dy, loss, row_max,
+    const uint32_t streaming = threads > uint32_t(kWave) ? threads - uint32_t(kWave) : threads;
+    kernel<<<grid_for(s.rows), threads, slot_bytes(t.k, streaming), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, dy, loss, row_max,
                                                               row_sum, dx);
   };
   if (row <= 4096u) {
@@ -670,7 +724,7 @@ void launch_fused(const Shape &s, const T *x, const Teacher &t, const float *dy,
     go(distill_held_kernel<T, 192, 6, NT>, 256u);
   } else if (row <= 71680u) {
     go(distill_held_kernel<T, 448, 10, NT>, 512u);
-  } else if (row <= 136192u) {
+  } else if (row <= kLongRow) {
     go(distill_held_kernel<T, 448, 20, NT>, 512u);
   } else {
     go(distill_held_kernel<T, 960, 18, NT>, 1024u);
@@ -689,6 +743,19 @@ int distill_fused(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t str
     // 16-bit arrays that lie an odd number of elements apart: buffer accesses ask for 4-byte alignment of both
     const int e = distill<T>(symbol, dim0, dim1, stride, temperature, x, t, loss, row_max, row_sum, stream);
     return e != 0 ? e : distill_bwd<T, false>(symbol, dim0, dim1, stride, temperature, dy, x, t, row_max, row_sum, dx, stream);
+  }
+  const Parts ps = cut_rows<T>(s);
+  if (s.rows <= kFewRows && size_t(s.n) * sizeof(T) > kLongRow && ps.parts > 1u) {
+    const hipStream_t st = as_stream(stream);
+    ScratchLease scratch = acquire_scratch(st, size_t(s.rows) * ps.parts * sizeof(SoftmaxSum), symbol);
+    if (!scratch.ptr) return int(hipErrorOutOfMemory);
+    SoftmaxSum *partial = static_cast<SoftmaxSum *>(scratch.ptr);
+    const uint32_t grid = grid_for(uint64_t(s.rows) * ps.parts);
+    part_stats_kernel<T><<<grid, kBlock, 0, st>>>(s.n, s.rows, s.stride, s.sc, ps, x, partial);
+    distill_bwd_kernel<T, kBlock, false, true, 0><<<grid, kBlock, slot_bytes(t.k, kBlock), st>>>(
+        s.n, s.rows, s.stride, s.sc, s.inv_t, ps, dy, x, t, Joined{partial, loss, row_max, row_sum}, dx);
+    note_launch(symbol);
+    return 0;
   }
   if (stream_policy(s.bytes(sizeof(T)), tuning().nontemporal) & kNtStore) {
     launch_fused<T, kNtStore>(s, x, t, dy, loss, row_max, row_sum, dx, as_stream(stream));
