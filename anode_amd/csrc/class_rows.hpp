@@ -233,17 +233,20 @@ __device__ inline float max_of(float m, const float (&v)[COUNT]) {
 
 // The fast form.
 template <int COUNT>
-__device__ inline void fold(SoftmaxSum &t, const float (&v)[COUNT], float c) {
-  const float m = max_of(t.m, v);
+__device__ inline void fold_below(SoftmaxSum &t, float m, const float (&v)[COUNT], float c) {  // m: the new reference, >= t.m and all values
   const float shift = m * c;
   if (m > t.m) {
     t.s *= __builtin_amdgcn_exp2f(t.m * c - shift);
     t.m = m;
   }
-  float s[2] = {0.0f, 0.0f};
+  float s[2] = {__builtin_amdgcn_exp2f(fmaf(v[0], c, -shift)), __builtin_amdgcn_exp2f(fmaf(v[1], c, -shift))};
 #pragma unroll
-  for (int j = 0; j < COUNT; ++j) s[j & 1] += __builtin_amdgcn_exp2f(fmaf(v[j], c, -shift));
+  for (int j = 2; j < COUNT; ++j) s[j & 1] += __builtin_amdgcn_exp2f(fmaf(v[j], c, -shift));
   t.s += s[0] + s[1];
+}
+template <int COUNT>
+__device__ inline void fold(SoftmaxSum &t, const float (&v)[COUNT], float c) {
+  fold_below(t, max_of(t.m, v), v, c);
 }
 __device__ inline void fold_one(SoftmaxSum &t, float x, float c) {
   const float v[2] = {x, kMinusInf};

@@ -37,34 +37,19 @@ struct KeyBits<f16_t> {
 __device__ inline uint64_t entry_of(uint32_t key, uint32_t k) { return (uint64_t(key) << 32) | uint32_t(~k); }
 __device__ inline uint32_t key_in(uint64_t entry) { return uint32_t(entry >> 32); }
 
-// Sorts the first `size` (a power of two) entries in LDS, largest first.  Up to 128 of them one wave does it, without
-// barriers in between.
+// Sorts the first `size` (a power of two) entries in LDS, largest first.
 template <int THREADS>
 __device__ inline void sort_entries(uint64_t *e, uint32_t size) {
-  auto exchange = [&](uint32_t i, uint32_t run, uint32_t step) {
-    const uint32_t lo = 2u * i - (i & (step - 1u)), hi = lo + step;
-    const uint64_t a = e[lo], b = e[hi];
-    if (((lo & run) == 0u) == (a < b)) {
-      e[lo] = b;
-      e[hi] = a;
-    }
-  };
-  __syncthreads();
-  if (size <= 2u * uint32_t(kWave)) {
-    if (threadIdx.x < uint32_t(kWave)) {
-      for (uint32_t run = 2; run <= size; run <<= 1) {
-        for (uint32_t step = run >> 1; step > 0; step >>= 1) {
-          if (threadIdx.x < size / 2u) exchange(threadIdx.x, run, step);
-          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          __builtin_amdgcn_wave_barrier();
+  for (uint32_t run = 2; run <= size; run <<= 1) {
+    for (uint32_t step = run >> 1; step > 0; step >>= 1) {
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < size / 2u; i += THREADS) {
+        const uint32_t lo = 2u * i - (i & (step - 1u)), hi = lo + step;
+        const uint64_t a = e[lo], b = e[hi];
+        if (((lo & run) == 0u) == (a < b)) {
+          e[lo] = b;
+          e[hi] = a;
         }
-      }
-    }
-  } else {
-    for (uint32_t run = 2; run <= size; run <<= 1) {
-      for (uint32_t step = run >> 1; step > 0; step >>= 1) {
-        for (uint32_t i = threadIdx.x; i < size / 2u; i += THREADS) exchange(i, run, step);
-        __syncthreads();
       }
     }
   }
@@ -213,17 +198,39 @@ __device__ inline uint32_t drop_small(const uint64_t *entries, uint32_t count, u
   return *taken;
 }
 
-// The result of a row from its entries in LDS, at least the k largest of them: sorted, and empty slots behind.
+// The result of a row from its entries in LDS, at least the k largest of them, and empty slots behind.  Up to 256 entries are
+// counted against each other (a thread an entry, the others read two at a time by all lanes alike); more are sorted.
 template <int THREADS>
 __device__ inline void write_result(uint64_t *entries, uint32_t count, size_t row, uint32_t k, float *value, uint32_t *index) {
-  uint32_t size = 2u;
-  while (size < count) size <<= 1;
-  for (uint32_t i = count + threadIdx.x; i < size; i += THREADS) entries[i] = 0u;
-  sort_entries<THREADS>(entries, size);
-  for (uint32_t i = threadIdx.x; i < k; i += THREADS) {
-    const bool have = i < count;
-    value[row * k + i] = have ? value_of(key_in(entries[i])) : kMinusInf;
-    index[row * k + i] = have ? ~uint32_t(entries[i]) : kNoClass;
+  if (count <= 256u) {
+    if (threadIdx.x == 0u) entries[count] = 0u;  // (the second of the last pair; the array has room)
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
+      const uint64_t own = entries[i];
+      uint32_t rank = 0u;
+      for (uint32_t j = 0; j < count; j += 2) {
+        typedef uint64_t pair __attribute__((ext_vector_type(2)));
+        const pair e = *reinterpret_cast<const pair *>(&entries[j]);
+        rank += (e.x > own ? 1u : 0u) + (e.y > own ? 1u : 0u);
+      }
+      if (rank < k) {
+        value[row * k + rank] = value_of(key_in(own));
+        index[row * k + rank] = ~uint32_t(own);
+      }
+    }
+  } else {
+    uint32_t size = 2u;
+    while (size < count) size <<= 1;
+    for (uint32_t i = count + threadIdx.x; i < size; i += THREADS) entries[i] = 0u;
+    sort_entries<THREADS>(entries, size);
+    for (uint32_t i = threadIdx.x; i < k && i < count; i += THREADS) {
+      value[row * k + i] = value_of(key_in(entries[i]));
+      index[row * k + i] = ~uint32_t(entries[i]);
+    }
+  }
+  for (uint32_t i = count + threadIdx.x; i < k; i += THREADS) {
+    value[row * k + i] = kMinusInf;
+    index[row * k + i] = kNoClass;
   }
 }
 
@@ -246,18 +253,18 @@ struct PartResults {
 // the row's length.  What the list holds at the end is thinned the same way, sorted and written.  Rows for which the list
 // is too short (thousands of ties at the border, the largest values all in few lanes' places) are selected
 // exactly, in more passes.
-template <typename T, int THREADS, int LIST, bool NORM, int NT>
-__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(NORM ? 6 : 8))) void top_k_kernel(uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc,
+template <typename T, int THREADS, int LIST, bool NORM>
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS > 512 ? 8 : THREADS > 256 ? 6 : 5))) void top_k_kernel(uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc,
                                                         double inv_t, Cut cut, const T *__restrict__ x,
                                                         float *__restrict__ value, uint32_t *__restrict__ index,
                                                         float *__restrict__ log_norm, PartResults pr) {
   constexpr int W = Group<T>::W;
-  constexpr int U = 16 / W;  // 16 values of a thread together
+  constexpr int U = THREADS > 256 ? 16 / W : 4;  // groups of a thread together
   constexpr uint32_t WAVES = THREADS / kWave;
   constexpr uint32_t kTile = uint32_t(THREADS) * uint32_t(U);
-  constexpr uint32_t kShort = 2u * uint32_t(THREADS);
-  __shared__ uint64_t list[LIST];
-  __shared__ uint64_t best[kShort];
+  constexpr uint32_t kShort = THREADS > 256 ? 2u * uint32_t(THREADS) : 512u;
+  __shared__ __align__(16) uint64_t list[LIST];
+  __shared__ __align__(16) uint64_t best[kShort];
   __shared__ RadixLds radix;
   __shared__ uint32_t wave_key[2][WAVES];
   __shared__ uint32_t listed, taken;
@@ -283,13 +290,13 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(NORM ? 
     };
     if (span.groups != 0u) {
       u32x4 q[U];
-      load_tile<T, THREADS, U, NT>(span, xr, threadIdx.x, q);
+      load_tile<T, THREADS, U, 0>(span, xr, threadIdx.x, q);
       uint32_t tile = 0u, turn = 0u;
       for (uint32_t base = 0;; base += kTile, ++tile) {
         float v[U * W];
         u32x4 next[U];
         const bool more = span.groups - base > kTile;
-        load_tile<T, THREADS, U, NT>(span, xr, base + kTile + threadIdx.x, next);
+        load_tile<T, THREADS, U, 0>(span, xr, base + kTile + threadIdx.x, next);
         unpack_tile<T, U>(q, v);
         if (!more) mask_tile<T, THREADS, U>(span, base + threadIdx.x, kMinusInf, v);
         const float tile_top = max_of(kMinusInf, v);
@@ -305,7 +312,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(NORM ? 
           for (uint32_t w = 1; w < WAVES; ++w) low = min(low, keys[w]);
           least = low < kLowestKey ? -__FLT_MAX__ : value_of(low);
         }
-        if (tile_top >= least) {  // (rare: the values are marked and fetched again, which costs no registers here)
+        if (tile_top >= least) {  // (rare: the values are marked and fetched again; an indexed register is dearer)
           uint32_t marked = 0u;
 #pragma unroll
           for (int i = 0; i < U * W; ++i) marked |= uint32_t(v[i] >= least) << i;
@@ -316,7 +323,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(NORM ? 
             put(float(xr[at]), at);
           } while (marked != 0u);
         }
-        if constexpr (NORM) fold(st, v, sc.c);
+        if constexpr (NORM) fold_below(st, fmaxf(top, -sc.limit), v, sc.c);
         if (!more) break;
 #pragma unroll
         for (int u = 0; u < U; ++u) q[u] = next[u];
@@ -332,7 +339,13 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(NORM ? 
     uint64_t *found = best;
     uint32_t have = listed;
     if (have <= uint32_t(LIST)) have = drop_small<THREADS>(list, have, k, best, kShort, wave_key[0], &taken);
-    if (have > kShort || (cut.parts > 1u && have > pr.quota)) {
+    if (have <= kShort && cut.parts > 1u && have > pr.quota) {  // more than the part has room for: the k largest of them
+      uint32_t size = 2u;
+      while (size < have) size <<= 1;
+      for (uint32_t i = have + threadIdx.x; i < size; i += THREADS) best[i] = 0u;
+      sort_entries<THREADS>(best, size);
+      have = k;
+    } else if (have > kShort) {
       __syncthreads();
       have = radix_select<T, THREADS>(xr, count, from, k, list, radix);
       found = list;
@@ -364,18 +377,31 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
                                                             float *__restrict__ value, uint32_t *__restrict__ index,
                                                             float *__restrict__ log_norm, PartResults pr) {
   constexpr uint32_t kShort = 2048;
-  __shared__ uint64_t list[kJoined];
-  __shared__ uint64_t best[kShort];
+  __shared__ __align__(16) uint64_t list[kJoined];
+  __shared__ __align__(16) uint64_t best[kShort];
+  __shared__ uint32_t first[65];
   __shared__ uint32_t wave_key[kBlock / kWave];
   __shared__ uint32_t taken;
   __shared__ float plain_lds[kBlock / kWave];
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    uint32_t have = 0u;
-    for (uint32_t p = 0; p < parts; ++p) {
-      const size_t item = r * parts + p;
-      const uint32_t count = pr.count[item];
-      for (uint32_t i = threadIdx.x; i < count; i += kBlock) list[have + i] = pr.entries[item * pr.quota + i];
-      have += count;
+    SoftmaxSum st = {-sc.limit, 0.0f};
+    if constexpr (NORM) {
+      const uint32_t lane = threadIdx.x & (kWave - 1);
+      if (lane < parts) st = pr.stats[r * parts + lane];
+    }
+    // (at most 64 parts: a lane finds where its part's entries begin, a thread which part its entry is of)
+    if (threadIdx.x < uint32_t(kWave)) {
+      const uint32_t count = threadIdx.x < parts ? pr.count[r * parts + threadIdx.x] : 0u;
+      first[threadIdx.x + 1u] = lanes_upto(count);
+      if (threadIdx.x == 0u) first[0] = 0u;
+    }
+    __syncthreads();
+    const uint32_t have = first[kWave];
+    for (uint32_t i = threadIdx.x; i < have; i += kBlock) {
+      uint32_t part = 0u;
+#pragma unroll
+      for (uint32_t step = 32u; step > 0u; step >>= 1) part += first[part + step] <= i ? step : 0u;
+      list[i] = pr.entries[(r * parts + part) * pr.quota + (i - first[part])];
     }
     __syncthreads();
     const uint32_t few = drop_small<kBlock>(list, have, k, best, kShort, wave_key, &taken);
@@ -385,8 +411,6 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
       write_result<kBlock>(list, have, r, k, value, index);
     }
     if constexpr (NORM) {
-      SoftmaxSum st = {-sc.limit, 0.0f};
-      for (uint32_t i = threadIdx.x & (kWave - 1); i < parts; i += kWave) st = merge(st, pr.stats[r * parts + i], sc.c);
       st = wave_merge(st, sc.c);
       if (measured(st.m, sc)) {
         st.s = true_sum(st, sc.c);
@@ -402,12 +426,12 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
 template <typename T, int THREADS, int LIST, bool NORM>
 int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, uint32_t k, float temperature, const T *x,
                  float *value, uint32_t *index, float *log_norm, hipStream_t st) {
-  // parts of at least 4096 values, that bring the launch to eight waves a SIMD
-  const uint32_t target = uint32_t(device_cu_count()) * (2048u / uint32_t(THREADS));
-  uint64_t parts = (uint64_t(target) + rows - 1u) / rows;
+  // parts of at least 4096 values, no more than bring the launch to eight waves a CU, and with room for three times k
+  // entries each among those that are joined (a part leaves little more than k)
+  uint64_t parts = uint64_t(device_cu_count()) * (512u / uint32_t(THREADS)) / rows;
   if (parts > n / 4096u) parts = n / 4096u;
   if (parts > 64u) parts = 64u;
-  if (k != 0u && parts > kJoined / k) parts = kJoined / k;
+  if (k != 0u && parts > kJoined / (3u * k)) parts = kJoined / (3u * k);
   Cut cut = {1u, n};
   if (parts > 1u) {
     const uint64_t per = ((uint64_t(n) + parts - 1u) / parts + 1023u) / 1024u * 1024u;
@@ -419,7 +443,7 @@ int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, u
   const double inv_t = 1.0 / double(temperature);
   PartResults pr = {nullptr, nullptr, nullptr, kJoined / cut.parts};
   if (cut.parts == 1u) {
-    top_k_kernel<T, THREADS, LIST, NORM, 0><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
+    top_k_kernel<T, THREADS, LIST, NORM><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
   } else {
     const size_t entry_bytes = size_t(items) * pr.quota * sizeof(uint64_t), stat_bytes = size_t(items) * sizeof(SoftmaxSum);
     ScratchLease scratch = acquire_scratch(st, entry_bytes + stat_bytes + size_t(items) * sizeof(uint32_t), symbol);
@@ -428,7 +452,7 @@ int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, u
     pr.entries = reinterpret_cast<uint64_t *>(at);
     pr.stats = reinterpret_cast<SoftmaxSum *>(at + entry_bytes);
     pr.count = reinterpret_cast<uint32_t *>(at + entry_bytes + stat_bytes);
-    top_k_kernel<T, THREADS, LIST, NORM, 0><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
+    top_k_kernel<T, THREADS, LIST, NORM><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
     top_k_join_kernel<T, NORM><<<rows < (1u << 24) ? rows : (1u << 24), kBlock, 0, st>>>(n, rows, stride, k, sc, inv_t, cut.parts, x,
                                                                                        value, index, log_norm, pr);
   }
@@ -445,15 +469,18 @@ int top_k(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, uin
   if (k != 0u && (value == nullptr || index == nullptr)) return refuse(symbol, "an array is missing");
   const size_t pitch = stride != 0u ? stride : dim0;
   const hipStream_t st = as_stream(stream);
-  // (a wave's 64 lanes speak for its share of k: four waves up to 128, sixteen beyond)
-  if (k <= 128u) {
-    return log_norm != nullptr
-               ? launch_top_k<T, 256, 1536, true>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st)
-               : launch_top_k<T, 256, 1536, false>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
-  }
-  return log_norm != nullptr
-             ? launch_top_k<T, 1024, 4096, true>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st)
-             : launch_top_k<T, 1024, 4096, false>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+  auto go = [&](auto norm) {
+    constexpr bool NORM = decltype(norm)::value;
+    // a wave's 64 lanes speak for its share of k: two or four waves up to 128, eight up to 256, sixteen beyond.  Two for short rows: 65536 rows of
+    // 1000 floats 100 against 200 us, 8192 of 16000 bf16 62 against 74; 1024 of 32768 35 against 28.
+    if (k > 256u) {
+      return launch_top_k<T, 1024, 4096, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+    }
+    if (k > 128u) return launch_top_k<T, 512, 3072, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+    return dim0 <= 16384u ? launch_top_k<T, 128, 1024, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st)
+                          : launch_top_k<T, 256, 1536, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+  };
+  return log_norm != nullptr ? go(std::true_type{}) : go(std::false_type{});
 }
 
 }  // namespace
