@@ -22,6 +22,31 @@ static inline int refuse(const char *symbol, const char *what) {
   return int(hipErrorInvalidValue);
 }
 
+// The code of the error recorded last (runtime.hip).
+int recorded_error();
+
+// The stream's scratch (runtime.hip) for these entry points, which return an error code and let no exception out: ptr is
+// null when it cannot be had, and `error` then what the entry point returns.
+struct RowsScratch {
+  ScratchLease lease;
+  int error;
+};
+static inline RowsScratch rows_scratch(hipStream_t stream, size_t bytes, const char *symbol) {
+  RowsScratch s = {ScratchLease{}, 0};
+  try {
+    s.lease = acquire_scratch(stream, bytes, symbol);
+    if (s.lease.ptr == nullptr) s.error = recorded_error();
+  } catch (...) {
+    note_error(symbol, hipErrorOutOfMemory, "cannot keep account of the scratch");
+  }
+  if (s.lease.ptr == nullptr && s.error == 0) s.error = int(hipErrorOutOfMemory);
+  return s;
+}
+// The scratch that each of them needs for [classes, rows] (distill.hip, top_k.hip, verify_draft.hip).
+size_t distill_scratch(uint32_t classes, uint32_t rows);
+size_t top_k_scratch(uint32_t classes, uint32_t rows, uint32_t k);
+size_t verify_scratch(uint32_t classes, uint32_t sequences);
+
 // What the row entry points ask of their scalars; 0 when they are fine.  The checks come before any device call.
 static inline int check_rows(const char *symbol, uint32_t classes, uint32_t stride, uint32_t k, float temperature) {
   if (stride != 0u && stride < classes) return refuse(symbol, "the stride is shorter than a row (0 = rows without padding)");

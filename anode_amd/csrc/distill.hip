@@ -639,16 +639,20 @@ uint32_t grid_for(uint64_t items) { return items < (1u << 24) ? uint32_t(items) 
 // Parts of at least one tile of a workgroup (kBlock * kUnroll groups), no more than bring the launch to kWanted workgroups:
 // four a CU (1001 rows of 50257 halves: loss and gradient 58.6 us whole, 66.3 us in two and three parts).
 constexpr uint32_t kWanted = 1024;
+Parts cut_rows(uint32_t n, uint32_t rows, uint32_t width) {
+  const uint32_t tile = uint32_t(kBlock * kUnroll) * width;
+  uint64_t parts = kWanted / rows;
+  if (parts > n / tile) parts = n / tile;
+  if (parts <= 1u) return Parts{1u, n};
+  const uint64_t unit = 1024;  // parts start whole 128-byte lines into a row
+  const uint64_t per = ((uint64_t(n) + parts - 1u) / parts + unit - 1u) / unit * unit;
+  return Parts{uint32_t((n + per - 1u) / per), uint32_t(per < n ? per : n)};
+}
 template <typename T>
 Parts cut_rows(const Shape &s) {
-  const uint32_t tile = uint32_t(kBlock * kUnroll * Group<T>::W);
-  uint64_t parts = kWanted / s.rows;
-  if (parts > s.n / tile) parts = s.n / tile;
-  if (parts <= 1u) return Parts{1u, s.n};
-  const uint64_t unit = 1024;  // parts start whole 128-byte lines into a row
-  const uint64_t per = ((uint64_t(s.n) + parts - 1u) / parts + unit - 1u) / unit * unit;
-  return Parts{uint32_t((s.n + per - 1u) / per), uint32_t(per < s.n ? per : s.n)};
+  return cut_rows(s.n, s.rows, uint32_t(Group<T>::W));
 }
+size_t partial_bytes(uint32_t rows, const Parts &ps) { return size_t(rows) * ps.parts * sizeof(SoftmaxSum); }
 
 template <typename T>
 int distill(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, float temperature, const T *x, const Teacher &t,
@@ -660,9 +664,9 @@ int distill(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, f
   const hipStream_t st = as_stream(stream);
   const Parts ps = cut_rows<T>(s);
   if (ps.parts > 1u) {
-    ScratchLease scratch = acquire_scratch(st, size_t(s.rows) * ps.parts * sizeof(SoftmaxSum), symbol);
-    if (!scratch.ptr) return int(hipErrorOutOfMemory);
-    SoftmaxSum *partial = static_cast<SoftmaxSum *>(scratch.ptr);
+    const RowsScratch scratch = rows_scratch(st, partial_bytes(s.rows, ps), symbol);
+    if (scratch.error != 0) return scratch.error;
+    SoftmaxSum *partial = static_cast<SoftmaxSum *>(scratch.lease.ptr);
     part_stats_kernel<T><<<grid_for(uint64_t(s.rows) * ps.parts), kBlock, 0, st>>>(s.n, s.rows, s.stride, s.sc, ps, x, partial);
     distill_join_kernel<T><<<grid_for(s.rows), kWave, 0, st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, ps.parts, x, t, partial, loss,
                                                              row_max, row_sum);
@@ -709,6 +713,12 @@ int distill_bwd(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t strid
   return 0;
 }
 
+template <typename T>
+bool overlap(const T *x, const T *dx, const Shape &s) {
+  const size_t len = (s.rows - 1u) * s.stride + s.n;
+  return x < dx + len && dx < x + len;
+}
+
 template <typename T, int NT>
 void launch_fused(const Shape &s, const T *x, const Teacher &t, const float *dy, float *loss, float *row_max, float *row_sum,
                   T *dx, hipStream_t st) {
@@ -745,11 +755,12 @@ int distill_fused(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t str
     return e != 0 ? e : distill_bwd<T, false>(symbol, dim0, dim1, stride, temperature, dy, x, t, row_max, row_sum, dx, stream);
   }
   const Parts ps = cut_rows<T>(s);
-  if (s.rows <= kFewRows && size_t(s.n) * sizeof(T) > kLongRow && ps.parts > 1u) {
+  // (not where dx is x: a part would overwrite logits that the other parts' workgroups still gather)
+  if (s.rows <= kFewRows && size_t(s.n) * sizeof(T) > kLongRow && ps.parts > 1u && !overlap(x, dx, s)) {
     const hipStream_t st = as_stream(stream);
-    ScratchLease scratch = acquire_scratch(st, size_t(s.rows) * ps.parts * sizeof(SoftmaxSum), symbol);
-    if (!scratch.ptr) return int(hipErrorOutOfMemory);
-    SoftmaxSum *partial = static_cast<SoftmaxSum *>(scratch.ptr);
+    const RowsScratch scratch = rows_scratch(st, partial_bytes(s.rows, ps), symbol);
+    if (scratch.error != 0) return scratch.error;
+    SoftmaxSum *partial = static_cast<SoftmaxSum *>(scratch.lease.ptr);
     const uint32_t grid = grid_for(uint64_t(s.rows) * ps.parts);
     part_stats_kernel<T><<<grid, kBlock, 0, st>>>(s.n, s.rows, s.stride, s.sc, ps, x, partial);
     distill_bwd_kernel<T, kBlock, false, true, 0><<<grid, kBlock, slot_bytes(t.k, kBlock), st>>>(
@@ -767,6 +778,16 @@ int distill_fused(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t str
 }
 
 }  // namespace
+
+size_t distill_scratch(uint32_t classes, uint32_t rows) {
+  if (classes == 0u || rows == 0u) return 0u;
+  size_t most = 0u;
+  for (uint32_t width : {4u, 8u}) {
+    const Parts ps = cut_rows(classes, rows, width);
+    if (ps.parts > 1u && partial_bytes(rows, ps) > most) most = partial_bytes(rows, ps);
+  }
+  return most;
+}
 }  // namespace anode
 
 // One set of entry points for each element type: SUFFIX of the names, ABI type, device type.

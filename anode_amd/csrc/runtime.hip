@@ -125,6 +125,8 @@ void note_launch(const char *symbol) {
   pending = e;
 }
 
+int recorded_error() { return g_last_error.load(std::memory_order_relaxed); }
+
 void note_error(const char *symbol, hipError_t e, const char *what) {
   g_last_error.store(int(e), std::memory_order_relaxed);
   std::fprintf(stderr, "%s: %s: %s; nothing was enqueued\n", symbol, what, hipGetErrorString(e));

@@ -423,38 +423,52 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
   }
 }
 
-template <typename T, int THREADS, int LIST, bool NORM>
-int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, uint32_t k, float temperature, const T *x,
-                 float *value, uint32_t *index, float *log_norm, hipStream_t st) {
-  // parts of at least 4096 values, no more than bring the launch to eight waves a CU, and with room for three times k
-  // entries each among those that are joined (a part leaves little more than k)
-  uint64_t parts = uint64_t(device_cu_count()) * (512u / uint32_t(THREADS)) / rows;
+// Threads of a workgroup: a wave's 64 lanes speak for its share of k, so two or four waves take up to 128, eight up to 256, sixteen
+// more.  Two for short rows: 65536 rows of 1000 floats 100 against 200 us, 8192 of 16000 bf16 62 against 74; 1024 of 32768
+// 35 against 28.  Eight for k = 200: 156 against 203 us with sixteen.
+uint32_t threads_for(uint32_t n, uint32_t k) { return k > 256u ? 1024u : k > 128u ? 512u : n <= 16384u ? 128u : 256u; }
+
+// Parts of at least 4096 values, no more than bring the launch to eight waves a CU, and with room for three times k entries
+// each among those that are joined (a part leaves little more than k).
+Cut cut_row(uint32_t n, uint32_t rows, uint32_t k, uint32_t threads) {
+  uint64_t parts = uint64_t(device_cu_count()) * (512u / threads) / rows;
   if (parts > n / 4096u) parts = n / 4096u;
   if (parts > 64u) parts = 64u;
   if (k != 0u && parts > kJoined / (3u * k)) parts = kJoined / (3u * k);
-  Cut cut = {1u, n};
-  if (parts > 1u) {
-    const uint64_t per = ((uint64_t(n) + parts - 1u) / parts + 1023u) / 1024u * 1024u;
-    cut = Cut{uint32_t((n + per - 1u) / per), uint32_t(per)};
-  }
+  if (parts <= 1u) return Cut{1u, n};
+  const uint64_t per = ((uint64_t(n) + parts - 1u) / parts + 1023u) / 1024u * 1024u;
+  return Cut{uint32_t((n + per - 1u) / per), uint32_t(per)};
+}
+struct PartBytes {
+  size_t entries, stats, counts;
+};
+PartBytes part_bytes(uint32_t rows, const Cut &cut) {
+  const size_t items = size_t(rows) * cut.parts;
+  return PartBytes{items * (kJoined / cut.parts) * sizeof(uint64_t), items * sizeof(SoftmaxSum), items * sizeof(uint32_t)};
+}
+
+template <typename T, int THREADS, int LIST, bool NORM>
+int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, uint32_t k, float temperature, const T *x,
+                 float *value, uint32_t *index, float *log_norm, hipStream_t st) {
+  const Cut cut = cut_row(n, rows, k, THREADS);
   const uint64_t items = uint64_t(rows) * cut.parts;
-  const uint32_t grid = items < (1u << 24) ? uint32_t(items) : (1u << 24);
+  const uint32_t most = 1u << 24, grid = items < most ? uint32_t(items) : most;
   const Scale sc = scale_for(temperature);
   const double inv_t = 1.0 / double(temperature);
   PartResults pr = {nullptr, nullptr, nullptr, kJoined / cut.parts};
   if (cut.parts == 1u) {
     top_k_kernel<T, THREADS, LIST, NORM><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
   } else {
-    const size_t entry_bytes = size_t(items) * pr.quota * sizeof(uint64_t), stat_bytes = size_t(items) * sizeof(SoftmaxSum);
-    ScratchLease scratch = acquire_scratch(st, entry_bytes + stat_bytes + size_t(items) * sizeof(uint32_t), symbol);
-    if (!scratch.ptr) return int(hipErrorOutOfMemory);
-    char *at = static_cast<char *>(scratch.ptr);
+    const PartBytes bytes = part_bytes(rows, cut);
+    const RowsScratch scratch = rows_scratch(st, bytes.entries + bytes.stats + bytes.counts, symbol);
+    if (scratch.error != 0) return scratch.error;
+    char *at = static_cast<char *>(scratch.lease.ptr);
     pr.entries = reinterpret_cast<uint64_t *>(at);
-    pr.stats = reinterpret_cast<SoftmaxSum *>(at + entry_bytes);
-    pr.count = reinterpret_cast<uint32_t *>(at + entry_bytes + stat_bytes);
+    pr.stats = reinterpret_cast<SoftmaxSum *>(at + bytes.entries);
+    pr.count = reinterpret_cast<uint32_t *>(at + bytes.entries + bytes.stats);
     top_k_kernel<T, THREADS, LIST, NORM><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
-    top_k_join_kernel<T, NORM><<<rows < (1u << 24) ? rows : (1u << 24), kBlock, 0, st>>>(n, rows, stride, k, sc, inv_t, cut.parts, x,
-                                                                                       value, index, log_norm, pr);
+    top_k_join_kernel<T, NORM><<<rows < most ? rows : most, kBlock, 0, st>>>(n, rows, stride, k, sc, inv_t, cut.parts, x, value,
+                                                                           index, log_norm, pr);
   }
   note_launch(symbol);
   return 0;
@@ -471,19 +485,25 @@ int top_k(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, uin
   const hipStream_t st = as_stream(stream);
   auto go = [&](auto norm) {
     constexpr bool NORM = decltype(norm)::value;
-    // a wave's 64 lanes speak for its share of k: two or four waves up to 128, eight up to 256, sixteen beyond.  Two for short rows: 65536 rows of
-    // 1000 floats 100 against 200 us, 8192 of 16000 bf16 62 against 74; 1024 of 32768 35 against 28.
-    if (k > 256u) {
-      return launch_top_k<T, 1024, 4096, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+    switch (threads_for(dim0, k)) {
+      case 128u: return launch_top_k<T, 128, 1024, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+      case 256u: return launch_top_k<T, 256, 1536, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+      case 512u: return launch_top_k<T, 512, 3072, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+      default: return launch_top_k<T, 1024, 4096, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
     }
-    if (k > 128u) return launch_top_k<T, 512, 3072, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
-    return dim0 <= 16384u ? launch_top_k<T, 128, 1024, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st)
-                          : launch_top_k<T, 256, 1536, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
   };
   return log_norm != nullptr ? go(std::true_type{}) : go(std::false_type{});
 }
 
 }  // namespace
+
+size_t top_k_scratch(uint32_t classes, uint32_t rows, uint32_t k) {
+  if (rows == 0u || k > kMaxSlots) return 0u;
+  const Cut cut = cut_row(classes, rows, k, threads_for(classes, k));
+  if (cut.parts == 1u) return 0u;
+  const PartBytes b = part_bytes(rows, cut);
+  return b.entries + b.stats + b.counts;
+}
 }  // namespace anode
 
 ANODE_EXPORT int anode_gpu_top_k_rows_f32(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature,

@@ -289,8 +289,27 @@ __global__ __launch_bounds__(kWave) void draw_kernel(Drafts d, uint32_t sequence
   }
 }
 
+// Blocks of a row, one at least.
+uint32_t blocks_of(uint32_t n) {
+  const uint32_t groups = n / 4u + (n % 4u != 0u);
+  return groups == 0u ? 1u : groups / kBlockGroups + (groups % kBlockGroups != 0u);
+}
+
 }  // namespace
+
+size_t verify_scratch(uint32_t classes, uint32_t sequences) {
+  const uint32_t blocks = blocks_of(classes);
+  return blocks <= kMostHeld ? 0u : size_t(sequences) * (blocks * sizeof(BlockSum) + sizeof(uint32_t));
+}
 }  // namespace anode
+
+// The most that any of the entry points over rows of classes asks of the stream's scratch.
+ANODE_EXPORT size_t anode_gpu_class_rows_scratch_bytes(uint32_t dim0, uint32_t dim1, uint32_t k) {
+  size_t most = anode::distill_scratch(dim0, dim1);
+  const size_t top = anode::top_k_scratch(dim0, dim1, k), verify = anode::verify_scratch(dim0, dim1);
+  if (top > most) most = top;
+  return verify > most ? verify : most;
+}
 
 ANODE_EXPORT int anode_gpu_verify_draft_packed_f32(uint32_t dim0, uint32_t dim1, uint32_t dim2, const float *target,
                                                    const float *draft, const uint32_t *draft_token, const uint32_t *draft_length,
@@ -303,8 +322,7 @@ ANODE_EXPORT int anode_gpu_verify_draft_packed_f32(uint32_t dim0, uint32_t dim1,
   if (pick == nullptr || token == nullptr || accepted == nullptr) return refuse(__func__, "an array is missing");
   if (dim1 >= kRefused) return refuse(__func__, "more drafted tokens than 2^31 - 1");
   const hipStream_t st = as_stream(stream);
-  const uint32_t groups = dim0 / 4u + (dim0 % 4u != 0u);
-  const uint32_t blocks = groups == 0u ? 1u : groups / kBlockGroups + (groups % kBlockGroups != 0u);
+  const uint32_t blocks = blocks_of(dim0);
   const Drafts d = {dim0, dim1, target, draft, draft_token, draft_length, accept};
   const uint64_t most = 1u << 24;
   const uint32_t grid = dim2 < most ? dim2 : uint32_t(most);
@@ -322,10 +340,10 @@ ANODE_EXPORT int anode_gpu_verify_draft_packed_f32(uint32_t dim0, uint32_t dim1,
       nt ? go(verify_kernel<1024, kNtLoad>, 1024u) : go(verify_kernel<1024, 0>, 1024u);
     }
   } else {
-    const size_t block_bytes = size_t(dim2) * blocks * sizeof(BlockSum);
-    ScratchLease scratch = acquire_scratch(st, block_bytes + size_t(dim2) * sizeof(uint32_t), __func__);
-    if (!scratch.ptr) return int(hipErrorOutOfMemory);
-    const Sums sums = {static_cast<BlockSum *>(scratch.ptr), reinterpret_cast<uint32_t *>(static_cast<char *>(scratch.ptr) + block_bytes)};
+    const RowsScratch scratch = rows_scratch(st, verify_scratch(dim0, dim2), __func__);
+    if (scratch.error != 0) return scratch.error;
+    char *at = static_cast<char *>(scratch.lease.ptr);
+    const Sums sums = {reinterpret_cast<BlockSum *>(at), reinterpret_cast<uint32_t *>(at + size_t(dim2) * blocks * sizeof(BlockSum))};
     const uint64_t items = (uint64_t(dim2) * blocks + kDrawWaves - 1u) / kDrawWaves;
     auto go = [&](auto kernel) { kernel<<<uint32_t(items < most ? items : most), kDrawThreads, 0, st>>>(d, dim2, blocks, sums); };
     nt ? go(draw_sums_kernel<kNtLoad>) : go(draw_sums_kernel<0>);

@@ -19,10 +19,12 @@ from ._lib import KernelConfig, load
 DEFAULT_CONFIG = KernelConfig(1024, 1024)
 
 
-def _as_arg(a):
+def _as_arg(a, device):
     if isinstance(a, torch.Tensor):
-        if not a.is_cuda:
-            raise ValueError("the ABI takes device pointers: tensor is not on the GPU")
+        if a.get_device() != device:
+            if not a.is_cuda:
+                raise ValueError("the ABI takes device pointers: tensor is not on the GPU")
+            raise ValueError(f"the ABI works on the current device ({device}): tensor is on device {a.get_device()}")
         if not a.is_contiguous():
             raise ValueError("the ABI takes packed arrays: tensor is not contiguous")
         return a.data_ptr()
@@ -45,10 +47,10 @@ def _entry(name: str):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _current_stream() -> int:
-    if _raw_stream is None or not torch.cuda.is_initialized():
-        return torch.cuda.current_stream().cuda_stream
-    return _raw_stream(torch.cuda.current_device())
+def _current_stream(device: int) -> int:
+    if _raw_stream is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device)
 
 
 def call(name: str, *args, cfg: Optional[KernelConfig] = None, stream: Optional[int] = None):
@@ -57,9 +59,10 @@ def call(name: str, *args, cfg: Optional[KernelConfig] = None, stream: Optional[
     fn, count = _entries.get(name) or _entry(name)
     if len(args) != count:
         raise TypeError(f"{name} takes {count} arguments before (cfg, stream): {load().prototypes[name][2][:-2]}")
+    device = torch.cuda.current_device()
     if stream is None:
-        stream = _current_stream()
-    return fn(*[_as_arg(a) for a in args], _DEFAULT_CONFIG_REF if cfg is None else ctypes.byref(cfg), stream)
+        stream = _current_stream(device)
+    return fn(*[_as_arg(a, device) for a in args], _DEFAULT_CONFIG_REF if cfg is None else ctypes.byref(cfg), stream)
 
 
 def take_last_error() -> int:

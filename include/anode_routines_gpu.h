@@ -286,10 +286,12 @@ void anode_gpu_softmax_nd_cat_nll_bwd_ignore_packed_accumulate_f32(uint32_t pref
  * uint32_t.  Row r of a [dim0 classes, dim1 rows] array of logits starts r * stride elements into it (a padded
  * vocabulary; what lies between dim0 and stride is neither read nor written); stride = 0 means rows without padding.
  * dim0 * dim1 may pass 2^32 here.  Per-row arrays of k slots are packed, slots first.  0xffffffff stands for "no class".
- * These entry points check their arguments before they touch the device: they return 0, or hipErrorInvalidValue
- * (1), also recorded for anode_gpu_take_last_error(), with the reason on stderr and nothing enqueued.  Refused are
- * stride < dim0 (unless 0), k > 1024, a temperature that is not positive and finite (or so small that its
- * reciprocal is not), missing arrays and 16-bit or float arrays that are not aligned to their type. ---- */
+ * These entry points check their arguments before they touch the device: they return 0, or an error code that is also
+ * recorded for anode_gpu_take_last_error(), with the reason on stderr and nothing enqueued: hipErrorInvalidValue (1)
+ * for stride < dim0 (unless 0), k > 1024, a temperature that is not positive and finite (or so small that its
+ * reciprocal is not), missing arrays and logits that are not aligned to their type.  Few long rows are cut into parts,
+ * whose results meet in the stream's scratch (below): a stream that is captured needs
+ * anode_gpu_class_rows_scratch_bytes() of it reserved first, or the call returns hipErrorStreamCaptureUnsupported (900). ---- */
 
 /* The k largest values of every row, largest first, and their classes: [k, dim1] each.  Of equal values (-0 equals +0)
  * the lower class comes first; NaN and -inf are never taken, as in anode_gpu_arg_max_packed_u32, and slots left over
@@ -400,6 +402,9 @@ size_t anode_host_arg_max_f32(const float *xs, size_t len);
  * tiling is fixed for a build and only moves through the library's undeclared measurement hook, after which the
  * query must be repeated. */
 size_t anode_gpu_reduce_scratch_bytes(uint32_t dim0, uint32_t dim1, uint32_t dim2);
+/* The same for the entry points over rows of classes: the most that any of them needs for dim0 classes, dim1 rows (or
+ * sequences) and k slots; 0 for shapes that need none. */
+size_t anode_gpu_class_rows_scratch_bytes(uint32_t dim0, uint32_t dim1, uint32_t k);
 /* Makes `stream` (current device) hold at least `bytes` of scratch, so that later calls allocate nothing (call it
  * before capturing the stream).  Returns 0 or the hipError_t of the failed allocation. */
 int anode_gpu_reserve_scratch(struct CUstream_st *stream, size_t bytes);

@@ -119,3 +119,34 @@ print("refused")
     env = dict(os.environ, HIP_VISIBLE_DEVICES="", ROCR_VISIBLE_DEVICES="")
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, env=env)
     assert r.returncode == 0 and "refused" in r.stdout, r.stderr
+
+
+def test_scratch_query():
+    q = _lib.load().symbol("anode_gpu_class_rows_scratch_bytes")
+    assert q(0, 0, 0) == 0 and q(131072, 0, 64) == 0 and q(0, 100, 5) == 0
+    assert q(1000, 256, 10) == 0                      # short rows: one workgroup each
+    assert q(131072, 4096, 64) >= 4096 * 64 * 16      # the sums of a sequence's 64 blocks
+    few = q(131072, 1, 64)
+    assert 0 < few <= q(131072, 8, 64) < 1 << 26
+    for k in (0, 1, 64, 1024, 5000):
+        assert q(0xFFFFFFFF, 1, k) < 1 << 27
+
+
+def test_scratch_that_cannot_be_had_is_an_error_code():
+    # no device: nothing can be allocated.  Shapes that need scratch return the code that was recorded, and enqueue nothing.
+    code = r"""
+import sys
+sys.path.insert(0, %r); sys.path.insert(0, %r)
+import test_class_rows_refusals as t
+for name, names, change in (("anode_gpu_top_k_rows_f32", t.CALLS["top_k_rows"][1], {"dim0": 131072, "dim1": 2}),
+                            ("anode_gpu_softmax_distill_rows_bf16", t.CALLS["softmax_distill_rows"][1], {"dim0": 131072, "dim1": 2}),
+                            ("anode_gpu_softmax_distill_fused_fwd_bwd_rows_f32", t.CALLS["softmax_distill_fused_fwd_bwd_rows"][1],
+                             {"dim0": 131072, "dim1": 2, "dx": t.P + (1 << 30)}),
+                            ("anode_gpu_verify_draft_packed_f32", t.VERIFY[1], {"dim0": 131072})):
+    rc, err = t._call(name, names, **change)
+    assert rc != 0 and rc == err, (name, rc, err)
+print("reported")
+""" % (_lib.REPO_ROOT, os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, HIP_VISIBLE_DEVICES="", ROCR_VISIBLE_DEVICES="")
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, env=env)
+    assert r.returncode == 0 and "reported" in r.stdout, r.stderr
