@@ -52,8 +52,9 @@ __device__ inline Slots slots_in(uint32_t *lds, uint32_t k, uint32_t threads) {
 }
 uint32_t slot_bytes(uint32_t k, uint32_t threads) { return 20u * k + 8u * threads + (k > uint32_t(kWave) ? 4u * kSeen : 0u); }
 
-// Reads the slots of a row, by one whole wave: x is the row, n its length.
-template <typename T>
+// Reads the slots of a row, by one whole wave: x is the row, n its length.  LOSS: the student's logits too, which the loss asks for
+// and the gradient does not.
+template <bool LOSS, typename T>
 __device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x, uint32_t n, double inv_t, const Slots &s) {
   const uint32_t lane = threadIdx.x & (kWave - 1);
   const size_t first = row * t.k;
@@ -65,7 +66,7 @@ __device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x
     const bool counts = at < n && v > kMinusInf;
     s.index[j] = counts ? at : kNoClass;
     s.p[j] = v;
-    s.x[j] = counts ? float(x[at]) : 0.0f;
+    if (LOSS) s.x[j] = counts ? float(x[at]) : 0.0f;
     if (counts) top = fmaxf(top, v);
   }
   top = wave_max(top);
@@ -414,7 +415,7 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32
     }
     const double w = double(dy[r]) * inv_t;
     if (threadIdx.x < uint32_t(kWave)) {
-      const TeacherRow tr = read_slots(t, r, xr, n, inv_t, slots);
+      const TeacherRow tr = read_slots<JOIN>(t, r, xr, n, inv_t, slots);
       if (threadIdx.x == 0) rs = RowShared{float(tr.mass), tr.any};
       deal_slots<T, THREADS>(t.k, tr.any, span, from, w, slots);
       if (JOIN && part == 0u) {
@@ -467,7 +468,7 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
   if (threadIdx.x >= uint32_t(S)) {
     for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
       const T *xr = x + r * stride;
-      const TeacherRow tr = read_slots(t, r, xr, n, inv_t, slots);
+      const TeacherRow tr = read_slots<true>(t, r, xr, n, inv_t, slots);
       if (threadIdx.x == uint32_t(S)) rs = RowShared{float(tr.mass), tr.any};
       deal_slots<T, S>(t.k, tr.any, RowSpan<T>(n, values_to_line(dx + r * stride)), 0u, double(dy[r]) * inv_t, slots);
       __syncthreads();  // 1: the parts, the mass and the lists are there
@@ -568,7 +569,7 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(4))) void
     u32x4 q[G];
     if (span.groups != 0u) load_tile<T, kWave, G, 0>(span, xr, threadIdx.x, q);
     const double w = double(dy[r]) * inv_t;
-    const TeacherRow tr = read_slots(t, r, xr, n, inv_t, slots);
+    const TeacherRow tr = read_slots<true>(t, r, xr, n, inv_t, slots);
     deal_slots<T, kWave>(t.k, tr.any, span, 0u, w, slots);
     SoftmaxSum st = {-sc.limit, 0.0f};
     for (uint32_t i = threadIdx.x; span.single(i); i += kWave) fold_one(st, float(xr[span.single_at(i)]), sc.c);
