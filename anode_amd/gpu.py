@@ -19,19 +19,14 @@ from ._lib import KernelConfig, load
 DEFAULT_CONFIG = KernelConfig(1024, 1024)
 
 
-def _as_arg(a, device):
-    if isinstance(a, torch.Tensor):
-        if a.get_device() != device:
-            if not a.is_cuda:
-                raise ValueError("the ABI takes device pointers: tensor is not on the GPU")
-            raise ValueError(f"the ABI works on the current device ({device}): tensor is on device {a.get_device()}")
-        if not a.is_contiguous():
-            raise ValueError("the ABI takes packed arrays: tensor is not contiguous")
-        return a.data_ptr()
-    return a
+def _refuse(a: torch.Tensor, device: int):
+    if not a.is_cuda:
+        raise ValueError("the ABI takes device pointers: tensor is not on the GPU")
+    if a.get_device() != device:
+        raise ValueError(f"the ABI works on the current device ({device}): tensor is on device {a.get_device()}")
+    raise ValueError("the ABI takes packed arrays: tensor is not contiguous")
 
 
-_DEFAULT_CONFIG_REF = ctypes.byref(DEFAULT_CONFIG)
 _entries = {}  # name -> (function, number of arguments before (cfg, stream))
 
 
@@ -47,12 +42,6 @@ def _entry(name: str):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _current_stream(device: int) -> int:
-    if _raw_stream is None:
-        return torch.cuda.current_stream(device).cuda_stream
-    return _raw_stream(device)
-
-
 def call(name: str, *args, cfg: Optional[KernelConfig] = None, stream: Optional[int] = None):
     """Invoke entry point `name`; `args` are everything before (cfg, stream).  Returns what the entry point returns:
     None, or for those that can refuse their arguments 0 or an error code (nothing is enqueued then)."""
@@ -60,9 +49,16 @@ def call(name: str, *args, cfg: Optional[KernelConfig] = None, stream: Optional[
     if len(args) != count:
         raise TypeError(f"{name} takes {count} arguments before (cfg, stream): {load().prototypes[name][2][:-2]}")
     device = torch.cuda.current_device()
+    values = []
+    for a in args:
+        if isinstance(a, torch.Tensor):
+            if a.get_device() != device or not a.is_contiguous():
+                _refuse(a, device)
+            a = a.data_ptr()
+        values.append(a)
     if stream is None:
-        stream = _current_stream(device)
-    return fn(*[_as_arg(a, device) for a in args], _DEFAULT_CONFIG_REF if cfg is None else ctypes.byref(cfg), stream)
+        stream = torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device)
+    return fn(*values, ctypes.byref(DEFAULT_CONFIG if cfg is None else cfg), stream)
 
 
 def take_last_error() -> int:

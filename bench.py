@@ -597,6 +597,29 @@ def all_symbols(torch, gpu):
     add("anode_gpu_smooth_negative_f1_loss_3d1_packed_f32", ss, (P, Cc, Nn, 1e-3, x, t01, E(Cc * Nn)), 8 * ns)
     add("anode_gpu_smooth_negative_f1_loss_3d1_bwd_packed_f32", ss, (P, Cc, Nn, 1e-3, Rn(Cc * Nn), x, t01, y), 12 * ns)
 
+    # rows of many classes: top-k, distillation from 64 slots a row, verification of three drafted tokens a sequence
+    K, R, k = 131072, 512, 64
+    value, index = E(R * k), E(R * k, torch.int32)
+    norm, loss, top, total, w = E(R), E(R), E(R), E(R), Rn(R)
+    for suffix, dt in (("f32", torch.float32), ("bf16", torch.bfloat16), ("f16", torch.float16)):
+        z, dz = Rn(K * R).to(dt), E(K * R, dt).zero_()
+        rs, nb, head = f"[{R},{K}] {suffix}", z.element_size() * K * R, (K, R, 0, k, 2.0)
+        add(f"anode_gpu_top_k_rows_{suffix}", rs, (K, R, 0, k, 2.0, z, value, index, norm), nb)
+        add(f"anode_gpu_softmax_distill_rows_{suffix}", rs, (*head, z, value, index, norm, loss, top, total), nb)
+        for acc in ("", "_accumulate"):
+            add(f"anode_gpu_softmax_distill_bwd_rows{acc}_{suffix}", rs, (*head, w, z, value, index, norm, top, total, dz),
+                (3 if acc else 2) * nb)
+        add(f"anode_gpu_softmax_distill_fused_fwd_bwd_rows_{suffix}", rs,
+            (*head, z, value, index, norm, w, loss, top, total, dz), 2 * nb)
+    B, G = 256, 3
+    target = torch.softmax(Rn(B * (G + 1) * K).view(-1, K), 1)
+    draft = torch.softmax(Rn(B * G * K).view(-1, K), 1)
+    token = torch.randint(0, K, (B * G,), device="cuda", dtype=torch.int32, generator=g)
+    # (independent rows: about half of the drafted tokens are taken; counted are the two rows that a refusal reads)
+    add("anode_gpu_verify_draft_packed_f32", f"[{B},{G},{K}]",
+        (K, G, B, target.view(-1), draft.view(-1), token, None, torch.rand(B * G, device="cuda", generator=g),
+         torch.rand(B, device="cuda", generator=g), E(B * (G + 1), torch.int32), E(B, torch.int32)), 8 * K * B)
+
     for sym, _, args, _ in L:
         gpu.call(sym, *args)
     torch.cuda.synchronize()
