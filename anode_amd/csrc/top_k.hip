@@ -56,15 +56,19 @@ __device__ inline void sort_entries(uint64_t *e, uint32_t size) {
   __syncthreads();
 }
 
-// A key that at least j lanes reach, found bit by bit (its leading 18 bits; those below are 0): 0 where fewer lanes hold a
-// key at all.  The comparisons' results are scalar, so a step is a compare, a count and a select.
+// A key that at least j lanes reach, found bit by bit: its leading 18 bits for floats (those below are 0), exactly for the
+// 16-bit types, whose keys have no more; 0 where fewer lanes hold a key at all.  The comparisons' results are scalar, so a
+// step is a compare, a count and a select.
+template <typename T>
 __device__ inline uint32_t key_reached_by(uint32_t key, uint32_t j) {
+  constexpr int kLow = sizeof(T) == 4 ? 14 : KeyBits<T>::value == 16 ? 16 : 13;
   uint32_t t = 0u;
 #pragma unroll
-  for (int bit = 31; bit >= 14; --bit) {
+  for (int bit = 31; bit >= kLow; --bit) {
     const uint32_t higher = t | (1u << bit);
     if (uint32_t(__popcll(__ballot(key >= higher))) >= j) t = higher;
   }
+  if (sizeof(T) == 2 && t != 0u && (t & 0x80000000u) == 0u) t |= (1u << kLow) - 1u;  // (below its bits a key repeats its sign, inverted)
   return t;
 }
 
@@ -75,16 +79,75 @@ struct RadixLds {
   uint32_t found, above, taken;
 };
 
-// The k largest entries of a row, or all of them where there are fewer, unsorted into `entries`; returns how many.  Exact
-// whatever the row holds: the k-th largest key is found digit by digit (8 bits a pass over the row, counted in LDS), the larger
-// ones are collected, and of those that equal it the first classes in order.
+// The entries of a row whose key is above `border`, unsorted into `entries` (room for `most`, k at least): all of them where they
+// are k or more, else with the first classes in order of those that equal the border, k together (fewer where the row
+// has fewer).  Returns their number, kNoClass where there is no room.
 template <typename T, int THREADS>
-__device__ inline uint32_t radix_select(const T *xr, uint32_t n, uint32_t from, uint32_t k, uint64_t *entries, RadixLds &l) {
+__device__ inline uint32_t collect(const T *xr, uint32_t n, uint32_t from, uint32_t border, uint32_t k, uint64_t *entries,
+                                   uint32_t most, RadixLds &l) {
   constexpr int W = Group<T>::W;
   constexpr int WAVES = THREADS / kWave;
   const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const RowGroups<T> rg(n, 0u);
-  if (k == 0u) return 0u;
+  __syncthreads();
+  if (threadIdx.x == 0) l.taken = 0u;
+  __syncthreads();
+  for (uint32_t g = threadIdx.x; g < rg.groups; g += THREADS) {
+    float v[W];
+    load_group<T, 0>(rg, xr, g, kMinusInf, v);
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+      const uint32_t key = key_of(v[j]);
+      if (key > border) {
+        const uint32_t at = atomicAdd(&l.taken, 1u);
+        if (at < most) entries[at] = entry_of(key, from + rg.first(g) + uint32_t(j));
+      }
+    }
+  }
+  __syncthreads();
+  const uint32_t count = l.taken;
+  if (count > most) return kNoClass;
+  if (count >= k || border == 0u) return count;
+  // the workgroup's groups in turn, counted across its threads
+  const uint32_t need = k - count;
+  uint32_t before = 0u;
+  for (uint32_t base = 0; base < rg.groups && before < need; base += THREADS) {
+    const uint32_t g = base + threadIdx.x;
+    uint32_t same = 0u;
+    if (g < rg.groups) {
+      float v[W];
+      load_group<T, 0>(rg, xr, g, kMinusInf, v);
+#pragma unroll
+      for (int j = 0; j < W; ++j) same |= uint32_t(key_of(v[j]) == border) << j;
+    }
+    const uint32_t own = uint32_t(__popc(same));
+    const uint32_t upto = lanes_upto(own);
+    if (lane == kWave - 1) l.wave_count[wave] = upto;
+    __syncthreads();
+    uint32_t at = before + upto - own, total = 0u;
+    for (int w = 0; w < WAVES; ++w) {
+      if (uint32_t(w) < wave) at += l.wave_count[w];
+      total += l.wave_count[w];
+    }
+    while (same != 0u && at < need) {
+      const uint32_t j = uint32_t(__ffs(int(same))) - 1u;
+      same &= same - 1u;
+      entries[count + at++] = entry_of(border, from + rg.first(g) + j);
+    }
+    before += total;
+    __syncthreads();
+  }
+  return count + min(need, before);
+}
+
+// The k largest entries of a row, or all of them where there are fewer, unsorted into `entries`; returns how many.  Exact
+// whatever the row holds: the k-th largest key is found digit by digit (8 bits a pass over the row, counted in LDS; a wave whose
+// digits are all alike, as in a row of ties, counts them with one addition), then collect().
+template <typename T, int THREADS>
+__device__ inline uint32_t radix_select(const T *xr, uint32_t n, uint32_t from, uint32_t k, uint64_t *entries, RadixLds &l) {
+  constexpr int W = Group<T>::W;
+  const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const RowGroups<T> rg(n, 0u);
   uint32_t prefix = 0u, known = 0u, need = k;
   bool all = false;  // the row holds fewer than k values that may be taken
   for (int shift = 24; shift >= 32 - KeyBits<T>::value && !all; shift -= 8) {
@@ -95,8 +158,15 @@ __device__ inline uint32_t radix_select(const T *xr, uint32_t n, uint32_t from, 
       load_group<T, 0>(rg, xr, g, kMinusInf, v);
 #pragma unroll
       for (int j = 0; j < W; ++j) {
-        const uint32_t key = key_of(v[j]);
-        if (key != 0u && (key & known) == prefix) atomicAdd(&l.digits[(key >> shift) & 255u], 1u);
+        const uint32_t key = key_of(v[j]), digit = (key >> shift) & 255u;
+        if (key != 0u && (key & known) == prefix) {
+          const uint64_t here = __ballot(true);
+          if (__all(digit == uint32_t(__builtin_amdgcn_readfirstlane(int(digit))))) {
+            if (lane == uint32_t(__ffsll((unsigned long long)here)) - 1u) atomicAdd(&l.digits[digit], uint32_t(__popcll(here)));
+          } else {
+            atomicAdd(&l.digits[digit], 1u);
+          }
+        }
       }
     }
     __syncthreads();
@@ -127,60 +197,18 @@ __device__ inline uint32_t radix_select(const T *xr, uint32_t n, uint32_t from, 
   }
   // the k-th largest key; below the digits looked at a key repeats its sign bit, inverted
   const uint32_t kth = all ? 0u : prefix | ((prefix & 0x80000000u) != 0u ? 0u : ~known);
-  if (threadIdx.x == 0) l.taken = 0u;
-  __syncthreads();
-  for (uint32_t g = threadIdx.x; g < rg.groups; g += THREADS) {
-    float v[W];
-    load_group<T, 0>(rg, xr, g, kMinusInf, v);
-#pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const uint32_t key = key_of(v[j]);
-      if (key > kth) entries[atomicAdd(&l.taken, 1u)] = entry_of(key, from + rg.first(g) + uint32_t(j));
-    }
-  }
-  __syncthreads();
-  const uint32_t count = l.taken;
-  if (all) return count;
-  // the first `need` classes whose key is the k-th: the workgroup's groups in turn, counted across its threads
-  uint32_t before = 0u;
-  for (uint32_t base = 0; base < rg.groups && before < need; base += THREADS) {
-    const uint32_t g = base + threadIdx.x;
-    uint32_t same = 0u;
-    if (g < rg.groups) {
-      float v[W];
-      load_group<T, 0>(rg, xr, g, kMinusInf, v);
-#pragma unroll
-      for (int j = 0; j < W; ++j) same |= uint32_t(key_of(v[j]) == kth) << j;
-    }
-    const uint32_t own = uint32_t(__popc(same));
-    const uint32_t upto = lanes_upto(own);
-    if (lane == kWave - 1) l.wave_count[wave] = upto;
-    __syncthreads();
-    uint32_t at = before + upto - own, total = 0u;
-    for (int w = 0; w < WAVES; ++w) {
-      if (uint32_t(w) < wave) at += l.wave_count[w];
-      total += l.wave_count[w];
-    }
-    while (same != 0u && at < need) {
-      const uint32_t j = uint32_t(__ffs(int(same))) - 1u;
-      same &= same - 1u;
-      entries[count + at++] = entry_of(kth, from + rg.first(g) + j);
-    }
-    before += total;
-    __syncthreads();
-  }
-  return count + need;
+  return collect<T, THREADS>(xr, n, from, kth, k, entries, k, l);
 }
 
 // The entries in LDS that can be among the k largest, to `out` (room for `most`): those that reach a key which k of them
 // reach, and few more.  Returns their number, which may be above `most` (then `out` is incomplete).
-template <int THREADS>
+template <typename T, int THREADS>
 __device__ inline uint32_t drop_small(const uint64_t *entries, uint32_t count, uint32_t k, uint64_t *out, uint32_t most,
                                       uint32_t *wave_key, uint32_t *taken) {
   constexpr uint32_t WAVES = THREADS / kWave;
   uint32_t top = 0u;
   for (uint32_t i = threadIdx.x; i < count; i += THREADS) top = max(top, key_in(entries[i]));
-  const uint32_t t = key_reached_by(top, (k + WAVES - 1u) / WAVES);
+  const uint32_t t = key_reached_by<T>(top, (k + WAVES - 1u) / WAVES);
   if ((threadIdx.x & (kWave - 1)) == 0) wave_key[threadIdx.x / kWave] = t;
   if (threadIdx.x == 0) *taken = 0u;
   __syncthreads();
@@ -196,6 +224,32 @@ __device__ inline uint32_t drop_small(const uint64_t *entries, uint32_t count, u
   }
   __syncthreads();
   return *taken;
+}
+
+// The selection where the list was too short, out of line: inlined it costs the streaming loop registers (119 against 114 us).  With
+// the threshold that the whole row gives -- `top` is the thread's largest value -- it reads the row once more; that settles
+// rising rows, and ties at the threshold itself (zeros, a mask's lowest value), of which the first in order are
+// wanted.  Else the exact k-th key is found.  The result is in `best`.
+template <typename T, int THREADS>
+__device__ __attribute__((noinline)) uint32_t select_again(const T *xr, uint32_t n, uint32_t from, float top, uint32_t k, uint64_t *list,
+                                                           uint32_t room, uint64_t *best, uint32_t most, RadixLds *l) {
+  constexpr uint32_t WAVES = THREADS / kWave;
+  const uint32_t t = key_reached_by<T>(key_of(top), (k + WAVES - 1u) / WAVES);
+  __syncthreads();
+  if ((threadIdx.x & (kWave - 1)) == 0) l->wave_count[threadIdx.x / kWave] = t;
+  __syncthreads();
+  uint32_t border = l->wave_count[0];
+  for (uint32_t w = 1; w < WAVES; ++w) border = min(border, l->wave_count[w]);
+  uint32_t have = collect<T, THREADS>(xr, n, from, border, k, list, room, *l);
+  __syncthreads();
+  if (have != kNoClass) {
+    have = drop_small<T, THREADS>(list, have, k, best, most, l->wave_count, &l->taken);
+    if (have <= most) return have;
+  }
+  __syncthreads();
+  have = radix_select<T, THREADS>(xr, n, from, k, best, *l);
+  __syncthreads();
+  return have;
 }
 
 // The result of a row from its entries in LDS, at least the k largest of them, and empty slots behind.  Up to 256 entries are
@@ -251,8 +305,7 @@ struct PartResults {
 // share of k reaches among the largest value of each of its lanes, the least of the waves counts -- is renewed after 1, 2, 4,
 // 8 ... tiles; values that reach it are put into a list in LDS, which grows by little more than k between two renewals, whatever
 // the row's length.  What the list holds at the end is thinned the same way, sorted and written.  Rows for which the list
-// is too short (thousands of ties at the border, the largest values all in few lanes' places) are selected
-// exactly, in more passes.
+// is too short (thousands of ties at the threshold, the largest values all in few lanes' places, rising rows) are read again.
 template <typename T, int THREADS, int LIST, bool NORM>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS > 512 ? 8 : THREADS > 256 ? 6 : 5))) void top_k_kernel(uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc,
                                                         double inv_t, Cut cut, const T *__restrict__ x,
@@ -282,10 +335,15 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
     __syncthreads();
     float top = kMinusInf, least = -__FLT_MAX__;
     SoftmaxSum st = {-sc.limit, 0.0f};
+    bool full = false;  // this thread has seen the list overflow
     auto put = [&](float v, uint32_t at) {
       if (v >= least) {
         const uint32_t place = atomicAdd(&listed, 1u);
-        if (place < uint32_t(LIST)) list[place] = entry_of(key_of(v), from + at);
+        if (place < uint32_t(LIST)) {
+          list[place] = entry_of(key_of(v), from + at);
+        } else {
+          full = true;
+        }
       }
     };
     if (span.groups != 0u) {
@@ -302,7 +360,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
         const float tile_top = max_of(kMinusInf, v);
         top = fmaxf(top, tile_top);
         if ((tile & (tile - 1u)) == 0u) {
-          const uint32_t t = key_reached_by(key_of(top), share);
+          const uint32_t t = key_reached_by<T>(key_of(top), share);
           uint32_t *keys = wave_key[turn];  // (the other half may still be read)
           turn ^= 1u;
           if ((threadIdx.x & (kWave - 1)) == 0) keys[wave] = t;
@@ -312,7 +370,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
           for (uint32_t w = 1; w < WAVES; ++w) low = min(low, keys[w]);
           least = low < kLowestKey ? -__FLT_MAX__ : value_of(low);
         }
-        if (tile_top >= least) {  // (rare: the values are marked and fetched again; an indexed register is dearer)
+        if (tile_top >= least && !full) {  // (rare: the values are marked and fetched again; an indexed register is dearer)
           uint32_t marked = 0u;
 #pragma unroll
           for (int i = 0; i < U * W; ++i) marked |= uint32_t(v[i] >= least) << i;
@@ -336,29 +394,24 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
       if constexpr (NORM) fold_one(st, v, sc.c);
     }
     __syncthreads();
-    uint64_t *found = best;
     uint32_t have = listed;
-    if (have <= uint32_t(LIST)) have = drop_small<THREADS>(list, have, k, best, kShort, wave_key[0], &taken);
-    if (have <= kShort && cut.parts > 1u && have > pr.quota) {  // more than the part has room for: the k largest of them
+    if (have <= uint32_t(LIST)) have = drop_small<T, THREADS>(list, have, k, best, kShort, wave_key[0], &taken);
+    if (have > kShort) have = select_again<T, THREADS>(xr, count, from, top, k, list, uint32_t(LIST), best, kShort, &radix);
+    if (cut.parts > 1u && have > pr.quota) {  // more than the part has room for: the k largest of them
       uint32_t size = 2u;
       while (size < have) size <<= 1;
       for (uint32_t i = have + threadIdx.x; i < size; i += THREADS) best[i] = 0u;
       sort_entries<THREADS>(best, size);
       have = k;
-    } else if (have > kShort) {
-      __syncthreads();
-      have = radix_select<T, THREADS>(xr, count, from, k, list, radix);
-      found = list;
-      __syncthreads();
     }
     if (cut.parts == 1u) {
-      write_result<THREADS>(found, have, r, k, value, index);
+      write_result<THREADS>(best, have, r, k, value, index);
       if constexpr (NORM) {
         st = finish_stats<T, THREADS>(st, xr, n, sc, sums);
         if (threadIdx.x == 0) log_norm[r] = float(double(st.m) * inv_t + log(double(st.s)));
       }
     } else {
-      for (uint32_t i = threadIdx.x; i < have; i += THREADS) pr.entries[item * pr.quota + i] = found[i];
+      for (uint32_t i = threadIdx.x; i < have; i += THREADS) pr.entries[item * pr.quota + i] = best[i];
       if (threadIdx.x == 0) pr.count[item] = have;
       if constexpr (NORM) {
         st = block_merge<WAVES>(st, sc.c, sums);
@@ -404,7 +457,7 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
       list[i] = pr.entries[(r * parts + part) * pr.quota + (i - first[part])];
     }
     __syncthreads();
-    const uint32_t few = drop_small<kBlock>(list, have, k, best, kShort, wave_key, &taken);
+    const uint32_t few = drop_small<T, kBlock>(list, have, k, best, kShort, wave_key, &taken);
     if (few <= kShort) {
       write_result<kBlock>(best, few, r, k, value, index);
     } else {
@@ -488,7 +541,7 @@ int top_k(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, uin
     switch (threads_for(dim0, k)) {
       case 128u: return launch_top_k<T, 128, 1024, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
       case 256u: return launch_top_k<T, 256, 1536, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
-      case 512u: return launch_top_k<T, 512, 3072, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+      case 512u: return launch_top_k<T, 512, 2560, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
       default: return launch_top_k<T, 1024, 4096, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
     }
   };
