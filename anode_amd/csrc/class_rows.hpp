@@ -151,41 +151,27 @@ __device__ inline u32x4 pack(const float (&v)[8], const T *) {
   return q;
 }
 
-// A row's values in 16-byte groups: group g holds the values g * W - shift ... g * W - shift + W - 1 of the row's
-// `n`, those of them that exist.  Rows may start at any element: with shift = 0 the groups start where the row does
-// (a 16-byte load needs no alignment beyond the element's); a kernel that stores chooses the shift so that its
-// groups start on 16-byte boundaries of the output.
+// A row's values in 16-byte groups from its start: group g holds the values g * W ... g * W + W - 1 of the row's `n`, those of
+// them that exist.  (A 16-byte load needs no alignment beyond the element's.)
 template <typename T>
 struct RowGroups {
   static constexpr int W = Group<T>::W;
-  uint32_t n, shift, groups;
-  __device__ RowGroups(uint32_t n_, uint32_t shift_)
-      : n(n_), shift(shift_), groups(uint32_t((uint64_t(n_) + shift_ + uint32_t(W) - 1u) / uint32_t(W))) {
-    if (n_ == 0u) groups = 0u;
-  }
-  // index of the group's first value; wrapped below zero for the first group of a shifted row
-  __device__ uint32_t first(uint32_t g) const { return g * uint32_t(W) - shift; }
-  __device__ bool whole(uint32_t g) const {
-    const uint64_t at = uint64_t(g) * uint32_t(W);
-    return at >= shift && at + uint32_t(W) <= uint64_t(n) + shift;
-  }
-  __device__ bool has(uint32_t g, int j) const {
-    const uint64_t at = uint64_t(g) * uint32_t(W) + uint32_t(j);
-    return at >= shift && at < uint64_t(n) + shift;
-  }
+  uint32_t n, groups;
+  __device__ explicit RowGroups(uint32_t n_) : n(n_), groups(n_ / uint32_t(W) + (n_ % uint32_t(W) != 0u)) {}
+  __device__ uint32_t first(uint32_t g) const { return g * uint32_t(W); }
+  __device__ bool whole(uint32_t g) const { return g < n / uint32_t(W); }
 };
 
 // 16-byte groups through a buffer descriptor: one offset register serves every group of a thread (the rest of the address
 // is scalar), a group past the end loads zeros and stores nothing.  The memory has to be 4-byte aligned and shorter than
-// 4 GiB.  NT: kNtStore as in store_stream(), kNtLoad as in load_stream().
+// 4 GiB.  NT: kNtStore as in store_stream().
 struct GroupBuffer {
   __amdgpu_buffer_rsrc_t rsrc;
   template <typename T>
   __device__ GroupBuffer(const T *p, uint32_t groups)
       : rsrc(__builtin_amdgcn_make_buffer_rsrc(const_cast<T *>(p), 0, int(groups * 16u), 0x00027000)) {}
-  template <int NT>
   __device__ u32x4 load(uint32_t thread_bytes, uint32_t bytes) const {
-    return __builtin_amdgcn_raw_buffer_load_b128(rsrc, int(thread_bytes), int(bytes), (NT & kNtLoad) != 0 ? 2 : 0);
+    return __builtin_amdgcn_raw_buffer_load_b128(rsrc, int(thread_bytes), int(bytes), 0);
   }
   template <int NT>
   __device__ void store(u32x4 v, uint32_t thread_bytes, uint32_t bytes) const {
@@ -197,14 +183,14 @@ struct GroupBuffer {
 };
 
 // The values of group g; those that are not the row's are `fill` and are not read.
-template <typename T, int NT>
+template <typename T>
 __device__ inline void load_group(const RowGroups<T> &rg, const T *row, uint32_t g, float fill, float (&v)[Group<T>::W]) {
   constexpr int W = Group<T>::W;
   if (rg.whole(g)) {
-    unpack(load_stream<NT, int(sizeof(T))>(reinterpret_cast<const u32x4 *>(row + rg.first(g))), v, row);
+    unpack(load_stream<0, int(sizeof(T))>(reinterpret_cast<const u32x4 *>(row + rg.first(g))), v, row);
   } else {
 #pragma unroll
-    for (int j = 0; j < W; ++j) v[j] = rg.has(g, j) ? float(row[size_t(rg.first(g) + uint32_t(j))]) : fill;
+    for (int j = 0; j < W; ++j) v[j] = rg.first(g) + uint32_t(j) < rg.n ? float(row[rg.first(g) + uint32_t(j)]) : fill;
   }
 }
 
@@ -222,7 +208,7 @@ __device__ inline void store_group(void *p, V v) {
 // ---- statistics of a row: its maximum m and S = sum of exp((x - m) / T) = sum of exp2((x - m) * c) ----
 //
 // The fast form spends one fused multiply-add on a value's exponent: exp2(x * c - R) with R = fl(b * c) for a running
-// reference b >= the values seen.  R's rounding is a factor common to all terms, which row_stats() takes out again at the
+// reference b >= the values seen.  R's rounding is a factor common to all terms, which true_sum() takes out again at the
 // end.  b starts at -limit, limit = 65536 / c: while it stays inside (-limit, limit) R is off by less than 2^-8 and
 // nothing overflows, whatever single values hold (-inf and the lowest value of a type add 0, a NaN shows in S).  A
 // row whose maximum lies outside -- nothing but -inf or a mask's lowest values, +inf, or values without measure --
@@ -396,12 +382,12 @@ __device__ inline void forget(u32x4 &q) { asm volatile("" : "+v"(q)); }
 // U groups of a thread: g, g + THREADS, ...  A group past the end reads the last one again (a branch round each load
 // would make every load wait for the one before, and a tile that is fetched ahead in a branch is waited for at its end: so
 // the tile behind the last is fetched too).  There is at least one group.
-template <typename T, int THREADS, int U, int NT>
+template <typename T, int THREADS, int U>
 __device__ inline void load_tile(const RowSpan<T> &span, const T *row, uint32_t g, u32x4 (&q)[U]) {
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t at = min(g + uint32_t(u) * uint32_t(THREADS), span.groups - 1u);
-    q[u] = load_stream<NT, int(sizeof(T))>(reinterpret_cast<const u32x4 *>(row + size_t(span.first(at))));
+    q[u] = load_stream<0, int(sizeof(T))>(reinterpret_cast<const u32x4 *>(row + size_t(span.first(at))));
   }
 }
 template <typename T, int U>
@@ -428,7 +414,7 @@ __device__ inline void mask_tile(const RowSpan<T> &span, uint32_t g, float fill,
 
 // A thread's running reference and sum over its part of a row (merge them with block_merge): tiles of U groups a thread,
 // the next tile on its way while one is folded.
-template <typename T, int THREADS, int U, int NT>
+template <typename T, int THREADS, int U>
 __device__ inline SoftmaxSum stream_stats(const RowSpan<T> &span, const T *row, Scale sc) {
   constexpr uint32_t kTile = uint32_t(THREADS) * uint32_t(U);
   SoftmaxSum st = {-sc.limit, 0.0f};
@@ -436,12 +422,12 @@ __device__ inline SoftmaxSum stream_stats(const RowSpan<T> &span, const T *row, 
   for (uint32_t i = threadIdx.x; span.single(i); i += THREADS) fold_one(st, float(row[span.single_at(i)]), sc.c);
   if (span.groups != 0u) {
     u32x4 q[U];
-    load_tile<T, THREADS, U, NT>(span, row, threadIdx.x, q);
+    load_tile<T, THREADS, U>(span, row, threadIdx.x, q);
     for (uint32_t base = 0;; base += kTile) {
       float v[U * Group<T>::W];
       u32x4 next[U];
       const bool more = span.groups - base > kTile;
-      load_tile<T, THREADS, U, NT>(span, row, base + kTile + threadIdx.x, next);
+      load_tile<T, THREADS, U>(span, row, base + kTile + threadIdx.x, next);
       unpack_tile<T, U>(q, v);
       if (!more) mask_tile<T, THREADS, U>(span, base + threadIdx.x, kMinusInf, v);
       fold(st, v, sc.c);

@@ -12,8 +12,6 @@
 // close, and they are few.
 #include "class_rows.hpp"
 
-#include <cmath>
-
 namespace anode {
 namespace {
 
@@ -237,7 +235,7 @@ struct Parts {
 };
 
 // One workgroup a row: statistics and loss.
-template <typename T, int THREADS, int NT>
+template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void distill_kernel(uint32_t n, uint32_t rows, size_t stride, Scale sc, double inv_t,
                                                           const T *__restrict__ x, Teacher t, float *__restrict__ loss,
                                                           float *__restrict__ row_max, float *__restrict__ row_sum) {
@@ -247,7 +245,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(uint32_t n, uint32_t r
     LaneSlot slot = {};
     if (threadIdx.x < uint32_t(kWave)) slot = lane_slot(t, r, xr, n, threadIdx.x);
     const SoftmaxSum st =
-        finish_stats<T, THREADS>(stream_stats<T, THREADS, kUnroll, NT>(RowSpan<T>(n, 0u), xr, sc), xr, n, sc, lds);
+        finish_stats<T, THREADS>(stream_stats<T, THREADS, kUnroll>(RowSpan<T>(n, 0u), xr, sc), xr, n, sc, lds);
     if (threadIdx.x < uint32_t(kWave)) {
       const float l = row_loss(t, r, xr, n, st, inv_t, slot);
       if (threadIdx.x == 0) {
@@ -269,7 +267,7 @@ __global__ __launch_bounds__(kBlock) void part_stats_kernel(uint32_t n, uint32_t
     const uint32_t r = uint32_t(i / ps.parts), part = uint32_t(i % ps.parts);
     const RowSpan<T> span(ps.count(part, n), 0u);
     const SoftmaxSum st = block_merge<kBlock / kWave>(
-        stream_stats<T, kBlock, kUnroll, 0>(span, x + size_t(r) * stride + ps.first(part), sc), sc.c, lds);
+        stream_stats<T, kBlock, kUnroll>(span, x + size_t(r) * stride + ps.first(part), sc), sc.c, lds);
     if (threadIdx.x == 0) partial[i] = st;
   }
 }
@@ -353,8 +351,8 @@ __device__ inline void stream_groups(const RowSpan<T> &span, const T *x, T *dx, 
     const uint32_t g = base + threadIdx.x;
     u32x4 old[U], next[U];
     const bool more = span.groups - base > kTile;
-    if (ACC) load_tile<T, THREADS, U, 0>(span, dx, g, old);
-    load_tile<T, THREADS, U, 0>(span, x, g + kTile, next);
+    if (ACC) load_tile<T, THREADS, U>(span, dx, g, old);
+    load_tile<T, THREADS, U>(span, x, g + kTile, next);
 #pragma unroll
     for (int u = 0; u < U; ++u, ++turn) {
       float v[W], o[W];
@@ -406,7 +404,7 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32
     T *dxr = dx + r * stride;
     const RowSpan<T> span(count, values_to_line(dxr + from));
     u32x4 q[kUnroll];
-    if (span.groups != 0u) load_tile<T, THREADS, kUnroll, 0>(span, xr + from, threadIdx.x, q);
+    if (span.groups != 0u) load_tile<T, THREADS, kUnroll>(span, xr + from, threadIdx.x, q);
     SoftmaxSum st;
     if (JOIN) {
       st = join_parts<T, THREADS>(jn.partial + r * ps.parts, ps.parts, xr, n, sc, plain_lds);
@@ -493,7 +491,7 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
     {
       const GroupBuffer xb(xr + span.head, min(span.groups, kHeld));
 #pragma unroll
-      for (int u = 0; u < G; ++u) q[u] = xb.load<0>(mine, uint32_t(u) * kStep);
+      for (int u = 0; u < G; ++u) q[u] = xb.load(mine, uint32_t(u) * kStep);
     }
     const float w = float(double(dy[r]) * inv_t);
     SoftmaxSum st = {-sc.limit, 0.0f};
@@ -567,7 +565,7 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(4))) void
     T *dxr = dx + r * stride;
     const RowSpan<T> span(n, values_to_line(dxr));
     u32x4 q[G];
-    if (span.groups != 0u) load_tile<T, kWave, G, 0>(span, xr, threadIdx.x, q);
+    if (span.groups != 0u) load_tile<T, kWave, G>(span, xr, threadIdx.x, q);
     const double w = double(dy[r]) * inv_t;
     const TeacherRow tr = read_slots<true>(t, r, xr, n, inv_t, slots);
     deal_slots<T, kWave>(t.k, tr.any, span, 0u, w, slots);
@@ -620,6 +618,17 @@ int prepare(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, u
   return 0;
 }
 
+// Whether the rows of two arrays lie in each other without being the same ones.  (Rows of one padded array may lie between the
+// rows of another.)
+template <typename T>
+bool tangled(const T *x, const T *dx, const Shape &s) {
+  if (x == dx || s.n == 0u) return false;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(dx);
+  const size_t apart = a < b ? b - a : a - b, row = size_t(s.n) * sizeof(T), step = s.stride * sizeof(T);
+  const size_t rows = apart / step, into = apart % step;
+  return (rows < s.rows && into < row) || (rows + 1u < s.rows && step - into < row);
+}
+
 template <typename T>
 int check_arrays(const char *symbol, const Shape &s, const T *x, const Teacher &t, std::initializer_list<const void *> needed) {
   if (s.n != 0u && (x == nullptr || misaligned(x))) return refuse(symbol, "the logits are missing or not aligned to their type");
@@ -630,10 +639,22 @@ int check_arrays(const char *symbol, const Shape &s, const T *x, const Teacher &
   return 0;
 }
 
-// Few long rows go in parts, each read a second time for the gradient: 14.8 against 18.7 us for 24 rows of 131072 bf16 logits.
-// At 64 rows the two are even, and shorter rows are quicker on one CU each (16 rows of 32768: 13.7 against 11.2 us).
+// Bytes of a row up to which one wave streams it alone: 8192 rows of 16 KB 30.7 us for the loss and 82 with the gradient, with four
+// waves 40 and 101; of 4096 rows of 32 KB the loss takes 29.7 and 30.1 us, with the gradient 84 and 77.  Where the rows
+// do not fill the GPU the gradient takes four waves from 4 KB on: 1024 rows of 16 KB 15.6 against 22 us, 2048 rows
+// 27.5 against 25.8.
+constexpr size_t kWaveRow = 16384;
+
+// Bytes of a row that the workgroups of the fused call hold in registers: those of a wave, and of the three smaller of
+// distill_held_kernel.  At each border the smaller one is the quicker: 94.8 against 182 us (32768 rows of 4 KB), 66.5
+// against 143 (8192 of 18 KB), 62 against 66 (2048 of 70 KB), 58.6 against 67.9 (1024 of 140 KB).
+constexpr size_t kHeldByWave = size_t(kWave) * 4u * 16u;
+constexpr size_t kHeldBySmall = 192u * 6u * 16u, kHeldByMiddle = 448u * 10u * 16u, kHeldByLarge = 448u * 20u * 16u;
+
+// Few rows that only the widest workgroup would hold go in parts, each read a second time for the gradient: 14.8 against 18.7
+// us for 24 rows of 131072 bf16 logits.  At 64 rows the two are even, and shorter rows are quicker on one CU each (16
+// rows of 32768: 13.7 against 11.2 us).
 constexpr uint32_t kFewRows = 32;
-constexpr size_t kLongRow = 136192;  // bytes
 
 uint32_t grid_for(uint64_t items) { return items < (1u << 24) ? uint32_t(items) : (1u << 24); }
 
@@ -671,12 +692,10 @@ int distill(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, f
     part_stats_kernel<T><<<grid_for(uint64_t(s.rows) * ps.parts), kBlock, 0, st>>>(s.n, s.rows, s.stride, s.sc, ps, x, partial);
     distill_join_kernel<T><<<grid_for(s.rows), kWave, 0, st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, ps.parts, x, t, partial, loss,
                                                              row_max, row_sum);
-  } else if (size_t(s.n) * sizeof(T) <= 16384u) {
-    distill_kernel<T, kWave, 0><<<grid_for(s.rows), kWave, 0, st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, loss, row_max,
-                                                                  row_sum);
+  } else if (size_t(s.n) * sizeof(T) <= kWaveRow) {
+    distill_kernel<T, kWave><<<grid_for(s.rows), kWave, 0, st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, loss, row_max, row_sum);
   } else {
-    distill_kernel<T, kBlock, 0><<<grid_for(s.rows), kBlock, 0, st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, loss, row_max,
-                                                                    row_sum);
+    distill_kernel<T, kBlock><<<grid_for(s.rows), kBlock, 0, st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, loss, row_max, row_sum);
   }
   note_launch(symbol);
   return 0;
@@ -688,7 +707,8 @@ void launch_bwd(const Shape &s, const float *dy, const T *x, const Teacher &t, c
   const Parts ps = cut_rows<T>(s);
   const uint32_t grid = grid_for(uint64_t(s.rows) * ps.parts);
   const Joined jn = {nullptr, nullptr, const_cast<float *>(row_max), const_cast<float *>(row_sum)};  // (read only)
-  if (size_t(s.n) * sizeof(T) <= 16384u) {
+  const size_t row = size_t(s.n) * sizeof(T);
+  if (row <= kHeldByWave || (row <= kWaveRow && s.rows > kWanted)) {
     distill_bwd_kernel<T, kWave, ACC, false, NT><<<grid, kWave, slot_bytes(t.k, kWave), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t,
                                                                                              ps, dy, x, t, jn, dx);
   } else {
@@ -705,6 +725,7 @@ int distill_bwd(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t strid
   if (dim1 == 0u || dim0 == 0u) return 0;
   if (const int e = check_arrays(symbol, s, x, t, {dy, row_max, row_sum, dx})) return e;
   if (misaligned(dx)) return refuse(symbol, "the gradient is not aligned to its type");
+  if (tangled<T>(x, dx, s)) return refuse(symbol, "the gradient's rows lie across the logits'");
   if (stream_policy(s.bytes(sizeof(T)), tuning().nontemporal) & kNtStore) {
     launch_bwd<T, ACC, kNtStore>(s, dy, x, t, row_max, row_sum, dx, as_stream(stream));
   } else {
@@ -712,12 +733,6 @@ int distill_bwd(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t strid
   }
   note_launch(symbol);
   return 0;
-}
-
-template <typename T>
-bool overlap(const T *x, const T *dx, const Shape &s) {
-  const size_t len = (s.rows - 1u) * s.stride + s.n;
-  return x < dx + len && dx < x + len;
 }
 
 template <typename T, int NT>
@@ -729,13 +744,13 @@ void launch_fused(const Shape &s, const T *x, const Teacher &t, const float *dy,
     kernel<<<grid_for(s.rows), threads, slot_bytes(t.k, streaming), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, dy, loss, row_max,
                                                               row_sum, dx);
   };
-  if (row <= 4096u) {
+  if (row <= kHeldByWave) {
     go(distill_wave_kernel<T, 4, NT>, kWave);
-  } else if (row <= 18432u) {
+  } else if (row <= kHeldBySmall) {
     go(distill_held_kernel<T, 192, 6, NT>, 256u);
-  } else if (row <= 71680u) {
+  } else if (row <= kHeldByMiddle) {
     go(distill_held_kernel<T, 448, 10, NT>, 512u);
-  } else if (row <= kLongRow) {
+  } else if (row <= kHeldByLarge) {
     go(distill_held_kernel<T, 448, 20, NT>, 512u);
   } else {
     go(distill_held_kernel<T, 960, 18, NT>, 1024u);
@@ -750,6 +765,7 @@ int distill_fused(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t str
   if (dim1 == 0u) return 0;
   if (const int e = check_arrays(symbol, s, x, t, {dy, loss, row_max, row_sum})) return e;
   if (dim0 != 0u && (dx == nullptr || misaligned(dx))) return refuse(symbol, "the gradient is missing or not aligned to its type");
+  if (tangled<T>(x, dx, s)) return refuse(symbol, "the gradient's rows lie across the logits'");
   if (((reinterpret_cast<uintptr_t>(x) - reinterpret_cast<uintptr_t>(dx)) & 3u) != 0u) {
     // 16-bit arrays that lie an odd number of elements apart: buffer accesses ask for 4-byte alignment of both
     const int e = distill<T>(symbol, dim0, dim1, stride, temperature, x, t, loss, row_max, row_sum, stream);
@@ -757,7 +773,7 @@ int distill_fused(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t str
   }
   const Parts ps = cut_rows<T>(s);
   // (not where dx is x: a part would overwrite logits that the other parts' workgroups still gather)
-  if (s.rows <= kFewRows && size_t(s.n) * sizeof(T) > kLongRow && ps.parts > 1u && !overlap(x, dx, s)) {
+  if (s.rows <= kFewRows && size_t(s.n) * sizeof(T) > kHeldByLarge && ps.parts > 1u && x != dx) {
     const hipStream_t st = as_stream(stream);
     const RowsScratch scratch = rows_scratch(st, partial_bytes(s.rows, ps), symbol);
     if (scratch.error != 0) return scratch.error;

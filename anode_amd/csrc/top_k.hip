@@ -88,13 +88,13 @@ __device__ inline uint32_t collect(const T *xr, uint32_t n, uint32_t from, uint3
   constexpr int W = Group<T>::W;
   constexpr int WAVES = THREADS / kWave;
   const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const RowGroups<T> rg(n, 0u);
+  const RowGroups<T> rg(n);
   __syncthreads();
   if (threadIdx.x == 0) l.taken = 0u;
   __syncthreads();
   for (uint32_t g = threadIdx.x; g < rg.groups; g += THREADS) {
     float v[W];
-    load_group<T, 0>(rg, xr, g, kMinusInf, v);
+    load_group<T>(rg, xr, g, kMinusInf, v);
 #pragma unroll
     for (int j = 0; j < W; ++j) {
       const uint32_t key = key_of(v[j]);
@@ -116,7 +116,7 @@ __device__ inline uint32_t collect(const T *xr, uint32_t n, uint32_t from, uint3
     uint32_t same = 0u;
     if (g < rg.groups) {
       float v[W];
-      load_group<T, 0>(rg, xr, g, kMinusInf, v);
+      load_group<T>(rg, xr, g, kMinusInf, v);
 #pragma unroll
       for (int j = 0; j < W; ++j) same |= uint32_t(key_of(v[j]) == border) << j;
     }
@@ -147,7 +147,7 @@ template <typename T, int THREADS>
 __device__ inline uint32_t radix_select(const T *xr, uint32_t n, uint32_t from, uint32_t k, uint64_t *entries, RadixLds &l) {
   constexpr int W = Group<T>::W;
   const uint32_t lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const RowGroups<T> rg(n, 0u);
+  const RowGroups<T> rg(n);
   uint32_t prefix = 0u, known = 0u, need = k;
   bool all = false;  // the row holds fewer than k values that may be taken
   for (int shift = 24; shift >= 32 - KeyBits<T>::value && !all; shift -= 8) {
@@ -155,7 +155,7 @@ __device__ inline uint32_t radix_select(const T *xr, uint32_t n, uint32_t from, 
     __syncthreads();
     for (uint32_t g = threadIdx.x; g < rg.groups; g += THREADS) {
       float v[W];
-      load_group<T, 0>(rg, xr, g, kMinusInf, v);
+      load_group<T>(rg, xr, g, kMinusInf, v);
 #pragma unroll
       for (int j = 0; j < W; ++j) {
         const uint32_t key = key_of(v[j]), digit = (key >> shift) & 255u;
@@ -307,10 +307,9 @@ struct PartResults {
 // the row's length.  What the list holds at the end is thinned the same way, sorted and written.  Rows for which the list
 // is too short (thousands of ties at the threshold, the largest values all in few lanes' places, rising rows) are read again.
 template <typename T, int THREADS, int LIST, bool NORM>
-__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS > 512 ? 8 : THREADS > 256 ? 6 : 5))) void top_k_kernel(uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc,
-                                                        double inv_t, Cut cut, const T *__restrict__ x,
-                                                        float *__restrict__ value, uint32_t *__restrict__ index,
-                                                        float *__restrict__ log_norm, PartResults pr) {
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS > 512 ? 8 : THREADS > 256 ? 6 : 5))) void top_k_kernel(
+    uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc, double inv_t, Cut cut, const T *__restrict__ x,
+    float *__restrict__ value, uint32_t *__restrict__ index, float *__restrict__ log_norm, PartResults pr) {
   constexpr int W = Group<T>::W;
   constexpr int U = THREADS > 256 ? 16 / W : 4;  // groups of a thread together
   constexpr uint32_t WAVES = THREADS / kWave;
@@ -348,13 +347,13 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
     };
     if (span.groups != 0u) {
       u32x4 q[U];
-      load_tile<T, THREADS, U, 0>(span, xr, threadIdx.x, q);
+      load_tile<T, THREADS, U>(span, xr, threadIdx.x, q);
       uint32_t tile = 0u, turn = 0u;
       for (uint32_t base = 0;; base += kTile, ++tile) {
         float v[U * W];
         u32x4 next[U];
         const bool more = span.groups - base > kTile;
-        load_tile<T, THREADS, U, 0>(span, xr, base + kTile + threadIdx.x, next);
+        load_tile<T, THREADS, U>(span, xr, base + kTile + threadIdx.x, next);
         unpack_tile<T, U>(q, v);
         if (!more) mask_tile<T, THREADS, U>(span, base + threadIdx.x, kMinusInf, v);
         const float tile_top = max_of(kMinusInf, v);

@@ -233,7 +233,7 @@ __global__ __launch_bounds__(THREADS) void verify_kernel(Drafts d, uint32_t sequ
                                                          const float *__restrict__ pick, uint32_t *__restrict__ out,
                                                          uint32_t *__restrict__ accepted) {
   __shared__ BlockSum sums[kMostHeld];
-  const RowGroups<float> rg(d.n, 0u);
+  const RowGroups<float> rg(d.n);
   for (size_t b = blockIdx.x; b < sequences; b += gridDim.x) {
     uint32_t length;
     const uint32_t taken = taken_tokens(d, b, length);
@@ -260,7 +260,7 @@ constexpr uint32_t kRefused = 0x80000000u;
 // One wave a block of a sequence's row (every wave finds out for itself which row that is).
 template <int NT>
 __global__ __launch_bounds__(kDrawThreads) void draw_sums_kernel(Drafts d, uint32_t sequences, uint32_t blocks, Sums out) {
-  const RowGroups<float> rg(d.n, 0u);
+  const RowGroups<float> rg(d.n);
   const uint64_t items = uint64_t(sequences) * blocks;
   for (uint64_t item = uint64_t(blockIdx.x) * kDrawWaves + threadIdx.x / kWave; item < items;
        item += uint64_t(gridDim.x) * kDrawWaves) {
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(kDrawThreads) void draw_sums_kernel(Drafts d, uint3
 __global__ __launch_bounds__(kWave) void draw_kernel(Drafts d, uint32_t sequences, uint32_t blocks, Sums in,
                                                      const float *__restrict__ pick, uint32_t *__restrict__ out,
                                                      uint32_t *__restrict__ accepted) {
-  const RowGroups<float> rg(d.n, 0u);
+  const RowGroups<float> rg(d.n);
   for (size_t b = blockIdx.x; b < sequences; b += gridDim.x) {
     const uint32_t word = in.taken[b], taken = word & ~kRefused;
     const Weights ws = weights_of(d, b, taken, (word & kRefused) != 0u);

@@ -314,11 +314,12 @@ int anode_gpu_softmax_distill_rows_bf16(uint32_t dim0, uint32_t dim1, uint32_t s
 int anode_gpu_softmax_distill_rows_f16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, float *loss, float *row_max, float *row_sum, ANODE_LAUNCH_TAIL);
 /* Its gradient, from the row_max and row_sum of the forward pass: dx[j] = dy[row] / t * (P q[j] - sum of the p_k whose
  * class is j), P = sum_k p_k (1 where teacher_log_norm is null).  Slots may name a class more than once.  dx lies as
- * x does (same stride) and may be x itself.  A row without a slot has dx = 0. */
+ * x does (same stride) and may be x itself; rows of dx that lie across rows of x are refused (1).  A row without a
+ * slot has dx = 0. */
 int anode_gpu_softmax_distill_bwd_rows_f32(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *dy, const float *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *row_max, const float *row_sum, float *dx, ANODE_LAUNCH_TAIL);
 int anode_gpu_softmax_distill_bwd_rows_bf16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *dy, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *row_max, const float *row_sum, uint16_t *dx, ANODE_LAUNCH_TAIL);
 int anode_gpu_softmax_distill_bwd_rows_f16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *dy, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *row_max, const float *row_sum, uint16_t *dx, ANODE_LAUNCH_TAIL);
-/* dx += ..., added in 32 bits or more and rounded once; dx may not be x.  A row without a slot is left as it is. */
+/* dx += ..., added in 32 bits or more and rounded once.  A row without a slot is left as it is. */
 int anode_gpu_softmax_distill_bwd_rows_accumulate_f32(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *dy, const float *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *row_max, const float *row_sum, float *dx, ANODE_LAUNCH_TAIL);
 int anode_gpu_softmax_distill_bwd_rows_accumulate_bf16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *dy, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *row_max, const float *row_sum, uint16_t *dx, ANODE_LAUNCH_TAIL);
 int anode_gpu_softmax_distill_bwd_rows_accumulate_f16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *dy, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, const float *row_max, const float *row_sum, uint16_t *dx, ANODE_LAUNCH_TAIL);

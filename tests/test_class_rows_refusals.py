@@ -84,6 +84,17 @@ def test_missing_and_misaligned_arrays(call, kind):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("call", [c for c in CALLS if "dx" in CALLS[c][1]])
+def test_gradients_that_lie_across_the_logits(call, kind):
+    name, names = _name(call, kind), CALLS[call][1]
+    size = 4 if kind == "f32" else 2
+    for elements, stride, rows in ((1, 0, 3), (-1, 0, 3), (99, 0, 1), (150, 0, 3), (299, 0, 3), (100, 120, 3), (121, 200, 3),
+                                   (-199, 200, 2), (301, 200, 3), (499, 200, 3), (-499, 200, 3)):
+        at = P + (1 << 20) + elements * size
+        assert _call(name, names, x=P + (1 << 20), dx=at, stride=stride, dim1=rows) == (REFUSED, REFUSED), (elements, stride, rows)
+
+
+@pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("call", CALLS)
 def test_no_rows_is_nothing_to_do(call, kind):
     name, names = _name(call, kind), CALLS[call][1]

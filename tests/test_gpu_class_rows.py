@@ -233,7 +233,14 @@ def check_distill(kind, x, value, index, t, dy, log_norm, mode, stride=0, offset
     rows, n = x.shape
     t = float(F32(t))  # the entry point's argument has 32 bits
     old = rounded(np.random.default_rng(9).standard_normal((rows, n)), kind) if mode == "accumulate" else None
-    loss, top, total, dx = run_distill(kind, x, value, index, t, dy, log_norm, mode, stride, offset, in_place, old, apart)
+    check_results(kind, x, value, index, t, dy, log_norm, mode, old, what,
+                  run_distill(kind, x, value, index, t, dy, log_norm, mode, stride, offset, in_place, old, apart))
+
+
+def check_results(kind, x, value, index, t, dy, log_norm, mode, old, what, got):
+    """Loss, row_max, row_sum and dx against the plain forms, within their bounds."""
+    rows, n = x.shape
+    loss, top, total, dx = got
     want_loss, want_top, want_total = ref.distill(x, value, index, t, log_norm)
     want_dx, q, p = ref.distill_grad(x, value, index, t, dy, log_norm)
     assert np.array_equal(top.astype(np.float64), want_top), what
@@ -294,6 +301,82 @@ def test_distill_of_arrays_that_lie_unlike_each_other(kind, apart):
         value, index = slots(g, 5, n, 9)
         for mode in ("fused", "apart", "accumulate"):
             check_distill(kind, x, value, index, 1.0, g.standard_normal(5).astype(F32), None, mode, n + 3, 1, what="unlike", apart=apart)
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("n,stride", [(130, 261), (130, 260), (9001, 20001)])
+def test_distill_of_a_gradient_between_the_rows_of_the_logits(kind, n, stride):
+    # one array of rows twice as long: the logits and the gradient lie beside each other in it
+    g = np.random.default_rng(n + stride)
+    rows, k = 5, 9
+    x = logits(g, rows, n, kind)
+    value, index = slots(g, rows, n, k)
+    dy = g.standard_normal(rows).astype(F32)
+    for first in (0, stride - n):                  # the gradient before the logits' rows, and behind them
+        both = torch.full((rows * stride + n,), 3.0, dtype=TYPES[kind], device="cuda")
+        grid = both[:rows * stride].view(rows, stride)
+        at = stride - n - first
+        grid[:, at:at + n] = torch.from_numpy(x).to("cuda").to(TYPES[kind])
+        out = [torch.empty(rows, device="cuda") for _ in range(3)]
+        call("anode_gpu_softmax_distill_fused_fwd_bwd_rows_" + kind, n, rows, stride, k, 1.0, both[at:], dev(value), u32(index), None,
+             dev(dy), *out, both[first:])
+        got = grid.float().cpu().numpy()
+        assert np.array_equal(got[:, at:at + n], x)
+        check_results(kind, x, value, index, 1.0, dy, None, "fused", None, f"between {first}",
+                      (*map(host, out), got[:, first:first + n]))
+        left = np.delete(got, np.r_[at:at + n, first:first + n], 1)
+        assert np.all(left == 3.0) and bool((both[rows * stride:] == 3.0).all())
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_distill_accumulates_onto_the_logits_themselves(kind):
+    g = np.random.default_rng(15)
+    for n in (77, 4100, 40000):
+        x = logits(g, 6, n, kind)
+        value, index = slots(g, 6, n, 12)
+        dy = g.standard_normal(6).astype(F32)
+        teacher = (dev(value), u32(index), None)
+        stats = [torch.empty(6, device="cuda") for _ in range(3)]
+        rows = Rows(x, kind)
+        call("anode_gpu_softmax_distill_rows_" + kind, n, 6, 0, 12, 1.0, rows.view, *teacher, *stats)
+        apart = Rows(x, kind)
+        call("anode_gpu_softmax_distill_bwd_rows_accumulate_" + kind, n, 6, 0, 12, 1.0, dev(dy), rows.view, *teacher, *stats[1:], apart.view)
+        call("anode_gpu_softmax_distill_bwd_rows_accumulate_" + kind, n, 6, 0, 12, 1.0, dev(dy), rows.view, *teacher, *stats[1:], rows.view)
+        assert np.array_equal(rows.get(), apart.get())
+        rows.check_surroundings("accumulate in place")
+
+
+# rows that fill the registers they are held in to the last value, and one value more; and the next workgroup's
+HELD = [4096, 18432, 71680, 143360, 276480]
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("row", HELD)
+@pytest.mark.parametrize("more", [-1, 0, 1])
+def test_distill_rows_at_the_borders(kind, row, more):
+    n = row // TYPES[kind].itemsize + more
+    rows = 34                                      # (more than are cut into parts)
+    g = np.random.default_rng(n)
+    x = np.broadcast_to(logits(g, 1, n, kind), (rows, n)).copy()
+    x[:, :3] = rounded(g.standard_normal((rows, 3)), kind)
+    value, index = slots(g, rows, n, 7)
+    for r in range(rows):
+        index[r, :2] = n - 1, (r * 64 + r) % n     # the row's last value, and places of every kind
+    index[:, 2:] = np.where(index[:, 2:] == index[:, :1], ref.NONE, index[:, 2:])
+    dy = g.standard_normal(rows).astype(F32)
+    for stride, offset, in_place in ((0, 0, False), (n + 1, 1, True)):
+        check_distill(kind, x, value, index, 1.0, dy, None, "fused", stride, offset, in_place, "border")
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("mode", ["fused", "apart"])
+@pytest.mark.parametrize("n", [1001, 2600, 4095])
+def test_distill_of_many_short_rows(kind, mode, n):
+    g = np.random.default_rng(n)
+    rows = 1030
+    x = logits(g, rows, n, kind)
+    value, index = slots(g, rows, n, 20)
+    check_distill(kind, x, value, index, 1.5, g.standard_normal(rows).astype(F32), None, mode, what="many")
 
 
 SHAPES = [(1, 3, 1), (2, 5, 3), (7, 4, 7), (8, 3, 2), (9, 2, 9), (63, 5, 10), (255, 3, 64), (257, 2, 0), (1000, 40, 10), (1000, 2, 700),
@@ -458,6 +541,15 @@ def test_verify(n, G, B, point):
         check_verify(target, None if point else draft, token, length, accept, pick, f"[{n}, {G}, {B}] {point} {offset}", offset)
 
 
+@pytest.mark.parametrize("B", [200, 300, 600])
+@pytest.mark.parametrize("n", [500, 8195])
+def test_verify_many_sequences(n, B):
+    g = np.random.default_rng(n + B)
+    target, draft, token = drafts(g, n, 1, B)
+    accept, pick = g.random((B, 1)).astype(F32), g.random(B).astype(F32)
+    check_verify(target, draft, token, None, accept, pick, f"[{n}, 1, {B}]")
+
+
 def test_verify_borders():
     # dyadic probabilities: every sum is exact, and the random numbers lie on the borders
     target = np.zeros((8, 2, 8), F32)
@@ -520,7 +612,7 @@ def test_drawing_follows_the_probabilities():
 
 def test_a_draft_model_is_distilled_and_its_tokens_verified():
     """The chain as it is used: the target's rows give a record, the draft model's head takes gradient steps on it, and
-    its tokens are then verified; the distance to the target falls and more tokens are taken."""
+    its tokens are then verified."""
     g = np.random.default_rng(30)
     n, B, G, k, t = 2000, 64, 2, 64, 1.0
     rows = B * (G + 1)
