@@ -56,20 +56,41 @@ __device__ inline void sort_entries(uint64_t *e, uint32_t size) {
   __syncthreads();
 }
 
-// A key that at least j lanes reach, found bit by bit: its leading 18 bits for floats (those below are 0), exactly for the
-// 16-bit types, whose keys have no more; 0 where fewer lanes hold a key at all.  The comparisons' results are scalar, so a
-// step is a compare, a count and a select.
+// The lowest bit of a key that the searches below look at: 18 leading bits of floats (those below are 0), all of the 16-bit
+// types', whose keys have no more.
+template <typename T>
+struct LowestBit {
+  static constexpr uint32_t value = sizeof(T) == 4 ? 1u << 14 : KeyBits<T>::value == 16 ? 1u << 16 : 1u << 13;
+};
+template <typename T>
+__device__ inline uint32_t whole_key(uint32_t t) {  // (below its bits a key of a 16-bit type repeats its sign, inverted)
+  return sizeof(T) == 2 && t != 0u && (t & 0x80000000u) == 0u ? t | (LowestBit<T>::value - 1u) : t;
+}
+
+// A key that at least j lanes reach, found bit by bit; 0 where fewer lanes hold a key at all.  The comparisons' results are
+// scalar, so a step is a compare, a count and a select.
 template <typename T>
 __device__ inline uint32_t key_reached_by(uint32_t key, uint32_t j) {
-  constexpr int kLow = sizeof(T) == 4 ? 14 : KeyBits<T>::value == 16 ? 16 : 13;
   uint32_t t = 0u;
 #pragma unroll
-  for (int bit = 31; bit >= kLow; --bit) {
-    const uint32_t higher = t | (1u << bit);
-    if (uint32_t(__popcll(__ballot(key >= higher))) >= j) t = higher;
+  for (uint32_t bit = 0x80000000u; bit >= LowestBit<T>::value; bit >>= 1) {
+    if (uint32_t(__popcll(__ballot(key >= (t | bit)))) >= j) t |= bit;
   }
-  if (sizeof(T) == 2 && t != 0u && (t & 0x80000000u) == 0u) t |= (1u << kLow) - 1u;  // (below its bits a key repeats its sign, inverted)
-  return t;
+  return whole_key<T>(t);
+}
+
+constexpr int kSegments = 16;  // of a thread, whose largest values lie in LDS
+
+// Room for `own` items of this lane behind a counter in LDS; the wave's lanes all call it.  (One addition for the wave: given an
+// atomic addition of different amounts the compiler adds the lanes up one after the other, 2 us of a row.)
+__device__ inline uint32_t reserve(uint32_t *counter, uint32_t own) {
+  const uint32_t upto = lanes_upto(own), all = from_lane(upto, kWave - 1);
+  uint32_t at = 0u;
+  if (all != 0u) {
+    if ((threadIdx.x & (kWave - 1)) == 0u) at = atomicAdd(counter, all);
+    at = from_lane(at, 0);
+  }
+  return at + upto - own;
 }
 
 // What the exact selection of k entries needs in LDS.
@@ -252,22 +273,31 @@ __device__ __attribute__((noinline)) uint32_t select_again(const T *xr, uint32_t
   return have;
 }
 
-// The result of a row from its entries in LDS, at least the k largest of them, and empty slots behind.  Up to 256 entries are
-// counted against each other (a thread an entry, the others read two at a time by all lanes alike); more are sorted.
+constexpr uint32_t kCounted = 512;
+// The result of a row from its entries in LDS, at least the k largest of them, and empty slots behind.  Up to 512 entries are
+// counted against each other, each by one to eight neighbouring threads; more are sorted.
 template <int THREADS>
 __device__ inline void write_result(uint64_t *entries, uint32_t count, size_t row, uint32_t k, float *value, uint32_t *index) {
-  if (count <= 256u) {
-    if (threadIdx.x == 0u) entries[count] = 0u;  // (the second of the last pair; the array has room)
+  if (count <= kCounted) {
+    uint32_t sharers = 8u;
+    while (sharers > 1u && sharers * count > uint32_t(THREADS)) sharers >>= 1;
+    // (each reads four pairs at a time: zeros behind the last entry; the array has room)
+    if (threadIdx.x < 64u) entries[count + threadIdx.x] = 0u;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < count; i += THREADS) {
+    const uint32_t part = threadIdx.x & (sharers - 1u);
+    for (uint32_t i = threadIdx.x / sharers; i < count; i += uint32_t(THREADS) / sharers) {
       const uint64_t own = entries[i];
       uint32_t rank = 0u;
-      for (uint32_t j = 0; j < count; j += 2) {
+      for (uint32_t j = 2u * part; j < count; j += 8u * sharers) {
         typedef uint64_t pair __attribute__((ext_vector_type(2)));
-        const pair e = *reinterpret_cast<const pair *>(&entries[j]);
-        rank += (e.x > own ? 1u : 0u) + (e.y > own ? 1u : 0u);
+        pair e[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) e[p] = *reinterpret_cast<const pair *>(&entries[j + 2u * uint32_t(p) * sharers]);
+#pragma unroll
+        for (int p = 0; p < 4; ++p) rank += (e[p].x > own ? 1u : 0u) + (e[p].y > own ? 1u : 0u);
       }
-      if (rank < k) {
+      for (uint32_t d = 1u; d < sharers; d <<= 1) rank += uint32_t(__shfl_xor(int(rank), int(d), kWave));
+      if (part == 0u && rank < k) {
         value[row * k + rank] = value_of(key_in(own));
         index[row * k + rank] = ~uint32_t(own);
       }
@@ -301,26 +331,48 @@ struct PartResults {
   uint32_t quota;
 };
 
-// One workgroup a part of a row, which it reads once.  A threshold that k values seen so far reach -- every wave finds what its
-// share of k reaches among the largest value of each of its lanes, the least of the waves counts -- is renewed after 1, 2, 4,
-// 8 ... tiles; values that reach it are put into a list in LDS, which grows by little more than k between two renewals, whatever
-// the row's length.  What the list holds at the end is thinned the same way, sorted and written.  Rows for which the list
-// is too short (thousands of ties at the threshold, the largest values all in few lanes' places, rising rows) are read again.
-template <typename T, int THREADS, int LIST, bool NORM>
-__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS > 512 ? 8 : THREADS > 256 ? 6 : 5))) void top_k_kernel(
+// A key that at least `share` of a wave's segments reach, from the largest values of each lane's segments in LDS.
+template <typename T, int THREADS>
+__device__ inline uint32_t key_of_segments(const float *segment, uint32_t segments, uint32_t share) {
+  uint32_t key[kSegments];
+#pragma unroll
+  for (int j = 0; j < kSegments; ++j) {
+    key[j] = uint32_t(j) < segments ? key_of(segment[uint32_t(j) * uint32_t(THREADS) + threadIdx.x]) : 0u;
+  }
+  uint32_t t = 0u;
+#pragma unroll 1
+  for (uint32_t bit = 0x80000000u; bit >= LowestBit<T>::value; bit >>= 1) {
+    uint32_t reached = 0u;
+#pragma unroll
+    for (int j = 0; j < kSegments; ++j) reached += uint32_t(__popcll(__ballot(key[j] >= (t | bit))));
+    if (reached >= share) t |= bit;
+  }
+  return whole_key<T>(t);
+}
+
+// One workgroup a part of a row, which it streams once.  A thread leaves the largest value of each of its segments (up to 16: a
+// 16-byte group each, or as many groups as that takes) in LDS.  A threshold that k segments of the row reach -- every wave finds
+// what its share of k reaches, the least of the waves counts -- names the few segments that can hold one of the k
+// largest; these are read again, and of their values those that reach the threshold are ranked and written.  Rows for which
+// there are too many (thousands of ties at the threshold, the largest values all in few threads' segments) are selected from
+// with one or more further passes.
+template <typename T, int THREADS, int SHORT, bool NORM>
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS == 128 && sizeof(T) == 4 ? 5 : 4))) void top_k_kernel(
     uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc, double inv_t, Cut cut, const T *__restrict__ x,
     float *__restrict__ value, uint32_t *__restrict__ index, float *__restrict__ log_norm, PartResults pr) {
   constexpr int W = Group<T>::W;
-  constexpr int U = THREADS > 256 ? 16 / W : 4;  // groups of a thread together
+  constexpr int U = 4;  // groups of a thread together
   constexpr uint32_t WAVES = THREADS / kWave;
   constexpr uint32_t kTile = uint32_t(THREADS) * uint32_t(U);
-  constexpr uint32_t kShort = THREADS > 256 ? 2u * uint32_t(THREADS) : 512u;
-  __shared__ __align__(16) uint64_t list[LIST];
-  __shared__ __align__(16) uint64_t best[kShort];
+  constexpr uint32_t kList = uint32_t(kSegments * THREADS) / 2u, kShort = SHORT;  // (kShort >= k: launch_top_k() sees to it)
+  __shared__ __align__(16) uint64_t list[kList];
+  __shared__ __align__(16) uint64_t best[kShort + 64u];
   __shared__ RadixLds radix;
-  __shared__ uint32_t wave_key[2][WAVES];
-  __shared__ uint32_t listed, taken;
+  __shared__ uint32_t wave_key[WAVES];
+  __shared__ uint32_t named, listed, taken;
   __shared__ SoftmaxSum sums[WAVES];
+  float *const segment = reinterpret_cast<float *>(list);          // [segments, threads]; until the list is filled
+  uint32_t *const names = reinterpret_cast<uint32_t *>(best);      // of segments to be read again
   const uint32_t wave = threadIdx.x / kWave;
   const uint32_t share = (k + WAVES - 1u) / WAVES;
   const uint64_t items = uint64_t(rows) * cut.parts;
@@ -330,87 +382,134 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
     const uint32_t count = min(cut.per, n - from);
     const T *xr = x + r * stride + from;
     const RowSpan<T> span(count, 0u);
-    if (threadIdx.x == 0) listed = 0u;
-    __syncthreads();
-    float top = kMinusInf, least = -__FLT_MAX__;
+    const uint32_t turns = span.groups / uint32_t(THREADS) + (span.groups % uint32_t(THREADS) != 0u);  // groups of a thread
+    const uint32_t tiles = (turns + uint32_t(U) - 1u) / uint32_t(U);
+    const bool fine = turns <= uint32_t(kSegments);  // a segment is one group
+    const uint32_t span_tiles = (tiles + uint32_t(kSegments) - 1u) / uint32_t(kSegments);
+    const uint32_t each = fine ? 1u : span_tiles * uint32_t(U);  // groups of a segment
+    const uint32_t segments = (turns + each - 1u) / each;
+    if (threadIdx.x == 0) named = listed = 0u;
+    float top = kMinusInf;
     SoftmaxSum st = {-sc.limit, 0.0f};
-    bool full = false;  // this thread has seen the list overflow
-    auto put = [&](float v, uint32_t at) {
-      if (v >= least) {
-        const uint32_t place = atomicAdd(&listed, 1u);
-        if (place < uint32_t(LIST)) {
-          list[place] = entry_of(key_of(v), from + at);
-        } else {
-          full = true;
-        }
-      }
-    };
     if (span.groups != 0u) {
       u32x4 q[U];
       load_tile<T, THREADS, U>(span, xr, threadIdx.x, q);
-      uint32_t tile = 0u, turn = 0u;
-      for (uint32_t base = 0;; base += kTile, ++tile) {
+      float segment_top = kMinusInf;
+      uint32_t left = span_tiles;
+      float *own = segment + threadIdx.x;
+      for (uint32_t base = 0;; base += kTile) {
         float v[U * W];
         u32x4 next[U];
         const bool more = span.groups - base > kTile;
         load_tile<T, THREADS, U>(span, xr, base + kTile + threadIdx.x, next);
         unpack_tile<T, U>(q, v);
         if (!more) mask_tile<T, THREADS, U>(span, base + threadIdx.x, kMinusInf, v);
-        const float tile_top = max_of(kMinusInf, v);
+        float tile_top = kMinusInf;
+        if (fine) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            float w[W];
+#pragma unroll
+            for (int j = 0; j < W; ++j) w[j] = v[u * W + j];
+            const float group_top = max_of(kMinusInf, w);
+            if (base / uint32_t(THREADS) + uint32_t(u) < uint32_t(kSegments)) own[u * THREADS] = group_top;
+            tile_top = fmaxf(tile_top, group_top);
+          }
+          own += U * THREADS;
+        } else {
+          tile_top = max_of(kMinusInf, v);
+          segment_top = fmaxf(segment_top, tile_top);
+          if (--left == 0u || !more) {
+            own[0] = segment_top;
+            own += THREADS;
+            segment_top = kMinusInf;
+            left = span_tiles;
+          }
+        }
         top = fmaxf(top, tile_top);
-        if ((tile & (tile - 1u)) == 0u) {
-          const uint32_t t = key_reached_by<T>(key_of(top), share);
-          uint32_t *keys = wave_key[turn];  // (the other half may still be read)
-          turn ^= 1u;
-          if ((threadIdx.x & (kWave - 1)) == 0) keys[wave] = t;
-          __syncthreads();
-          uint32_t low = keys[0];
-#pragma unroll
-          for (uint32_t w = 1; w < WAVES; ++w) low = min(low, keys[w]);
-          least = low < kLowestKey ? -__FLT_MAX__ : value_of(low);
-        }
-        if (tile_top >= least && !full) {  // (rare: the values are marked and fetched again; an indexed register is dearer)
-          uint32_t marked = 0u;
-#pragma unroll
-          for (int i = 0; i < U * W; ++i) marked |= uint32_t(v[i] >= least) << i;
-          do {
-            const uint32_t i = uint32_t(__ffs(int(marked))) - 1u;
-            marked &= marked - 1u;
-            const uint32_t at = span.first(base + threadIdx.x + i / uint32_t(W) * uint32_t(THREADS)) + i % uint32_t(W);
-            put(float(xr[at]), at);
-          } while (marked != 0u);
-        }
         if constexpr (NORM) fold_below(st, fmaxf(top, -sc.limit), v, sc.c);
         if (!more) break;
 #pragma unroll
         for (int u = 0; u < U; ++u) q[u] = next[u];
       }
     }
-    if (span.single(threadIdx.x)) {  // (at most 7: the head is empty)
-      const uint32_t at = span.single_at(threadIdx.x);
-      const float v = float(xr[at]);
-      put(v, at);
-      if constexpr (NORM) fold_one(st, v, sc.c);
+    // (up to half of a wave's lanes: the lanes' largest values instead of the segments', 1.4 times k values reach what they give)
+    const uint32_t t = share <= uint32_t(kWave / 2) ? key_reached_by<T>(key_of(top), share)
+                                                    : key_of_segments<T, THREADS>(segment, segments, share);
+    if ((threadIdx.x & (kWave - 1)) == 0) wave_key[wave] = t;
+    __syncthreads();
+    uint32_t low = wave_key[0];
+#pragma unroll
+    for (uint32_t w = 1; w < WAVES; ++w) low = min(low, wave_key[w]);
+    const float least = low < kLowestKey ? -__FLT_MAX__ : value_of(low);
+    uint32_t marked = 0u;
+#pragma unroll 4
+    for (uint32_t j = 0; j < segments; ++j) marked |= uint32_t(segment[j * uint32_t(THREADS) + threadIdx.x] >= least) << j;
+    uint32_t place = reserve(&named, uint32_t(__popc(marked)));
+    for (; marked != 0u && place < 2u * kShort; marked &= marked - 1u) {
+      names[place++] = (uint32_t(__ffs(int(marked))) - 1u) * each * uint32_t(THREADS) + threadIdx.x;  // its first group
     }
     __syncthreads();
-    uint32_t have = listed;
-    if (have <= uint32_t(LIST)) have = drop_small<T, THREADS>(list, have, k, best, kShort, wave_key[0], &taken);
-    if (have > kShort) have = select_again<T, THREADS>(xr, count, from, top, k, list, uint32_t(LIST), best, kShort, &radix);
+    uint32_t have = named <= 2u * kShort ? 0u : kNoClass;
+    if (have == 0u) {
+      const uint32_t again = named * each;
+      for (uint32_t base = 0; base < again; base += uint32_t(THREADS)) {
+        const uint32_t i = min(base + threadIdx.x, again - 1u);
+        const uint32_t g = names[i / each] + i % each * uint32_t(THREADS);
+        const bool mine = base + threadIdx.x < again && g < span.groups;
+        float v[W];
+        unpack(load_stream<0, int(sizeof(T))>(reinterpret_cast<const u32x4 *>(xr + size_t(span.first(min(g, span.groups - 1u))))), v, x);
+        uint32_t reached = 0u;
+#pragma unroll
+        for (int j = 0; j < W; ++j) reached += mine && v[j] >= least ? 1u : 0u;
+        uint32_t place = reserve(&listed, reached);
+        if (reached != 0u && place + reached <= kList) {
+#pragma unroll
+          for (int j = 0; j < W; ++j) {
+            if (v[j] >= least) list[place++] = entry_of(key_of(v[j]), from + span.first(g) + uint32_t(j));
+          }
+        }
+      }
+      if (span.single(threadIdx.x)) {  // (at most 7: the head is empty)
+        const uint32_t at = span.single_at(threadIdx.x);
+        const float v = float(xr[at]);
+        if (v >= least) {
+          const uint32_t place = atomicAdd(&listed, 1u);
+          if (place < kList) list[place] = entry_of(key_of(v), from + at);
+        }
+        if constexpr (NORM) fold_one(st, v, sc.c);
+      }
+      __syncthreads();
+      have = listed;
+    } else if (NORM && span.single(threadIdx.x)) {
+      fold_one(st, float(xr[span.single_at(threadIdx.x)]), sc.c);
+    }
+    uint64_t *found = list;
+    if (have > kList) {
+      have = select_again<T, THREADS>(xr, count, from, top, k, list, kList, best, kShort, &radix);
+      found = best;
+    } else if (have > kCounted / 2u) {
+      const uint32_t few = drop_small<T, THREADS>(list, have, k, best, kShort, wave_key, &taken);
+      if (few <= kShort) {
+        have = few;
+        found = best;
+      }
+    }
     if (cut.parts > 1u && have > pr.quota) {  // more than the part has room for: the k largest of them
       uint32_t size = 2u;
       while (size < have) size <<= 1;
-      for (uint32_t i = have + threadIdx.x; i < size; i += THREADS) best[i] = 0u;
-      sort_entries<THREADS>(best, size);
+      for (uint32_t i = have + threadIdx.x; i < size; i += THREADS) found[i] = 0u;
+      sort_entries<THREADS>(found, size);
       have = k;
     }
     if (cut.parts == 1u) {
-      write_result<THREADS>(best, have, r, k, value, index);
+      write_result<THREADS>(found, have, r, k, value, index);
       if constexpr (NORM) {
         st = finish_stats<T, THREADS>(st, xr, n, sc, sums);
         if (threadIdx.x == 0) log_norm[r] = float(double(st.m) * inv_t + log(double(st.s)));
       }
     } else {
-      for (uint32_t i = threadIdx.x; i < have; i += THREADS) pr.entries[item * pr.quota + i] = best[i];
+      for (uint32_t i = threadIdx.x; i < have; i += THREADS) pr.entries[item * pr.quota + i] = found[i];
       if (threadIdx.x == 0) pr.count[item] = have;
       if constexpr (NORM) {
         st = block_merge<WAVES>(st, sc.c, sums);
@@ -478,7 +577,8 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
 // Threads of a workgroup: a wave's 64 lanes speak for its share of k, so two or four waves take up to 128, eight up to 256, sixteen
 // more.  Two for short rows: 65536 rows of 1000 floats 100 against 200 us, 8192 of 16000 bf16 62 against 74; 1024 of 32768
 // 35 against 28.  Eight for k = 200: 156 against 203 us with sixteen.
-uint32_t threads_for(uint32_t n, uint32_t k) { return k > 256u ? 1024u : k > 128u ? 512u : n <= 16384u ? 128u : 256u; }
+constexpr uint32_t kFew = 256;
+uint32_t threads_for(uint32_t n, uint32_t k) { return n <= 16384u && k <= kFew ? 128u : 256u; }
 
 // Parts of at least 4096 values, no more than bring the launch to eight waves a CU, and with room for three times k entries
 // each among those that are joined (a part leaves little more than k).
@@ -499,9 +599,10 @@ PartBytes part_bytes(uint32_t rows, const Cut &cut) {
   return PartBytes{items * (kJoined / cut.parts) * sizeof(uint64_t), items * sizeof(SoftmaxSum), items * sizeof(uint32_t)};
 }
 
-template <typename T, int THREADS, int LIST, bool NORM>
+template <typename T, int THREADS, int SHORT, bool NORM>
 int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, uint32_t k, float temperature, const T *x,
                  float *value, uint32_t *index, float *log_norm, hipStream_t st) {
+  if (k > uint32_t(SHORT)) return refuse(symbol, "more slots than the kernel has room for");  // (not reached)
   const Cut cut = cut_row(n, rows, k, THREADS);
   const uint64_t items = uint64_t(rows) * cut.parts;
   const uint32_t most = 1u << 24, grid = items < most ? uint32_t(items) : most;
@@ -509,7 +610,7 @@ int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, u
   const double inv_t = 1.0 / double(temperature);
   PartResults pr = {nullptr, nullptr, nullptr, kJoined / cut.parts};
   if (cut.parts == 1u) {
-    top_k_kernel<T, THREADS, LIST, NORM><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
+    top_k_kernel<T, THREADS, SHORT, NORM><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
   } else {
     const PartBytes bytes = part_bytes(rows, cut);
     const RowsScratch scratch = rows_scratch(st, bytes.entries + bytes.stats + bytes.counts, symbol);
@@ -518,7 +619,7 @@ int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, u
     pr.entries = reinterpret_cast<uint64_t *>(at);
     pr.stats = reinterpret_cast<SoftmaxSum *>(at + bytes.entries);
     pr.count = reinterpret_cast<uint32_t *>(at + bytes.entries + bytes.stats);
-    top_k_kernel<T, THREADS, LIST, NORM><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
+    top_k_kernel<T, THREADS, SHORT, NORM><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
     top_k_join_kernel<T, NORM><<<rows < most ? rows : most, kBlock, 0, st>>>(n, rows, stride, k, sc, inv_t, cut.parts, x, value,
                                                                            index, log_norm, pr);
   }
@@ -537,12 +638,9 @@ int top_k(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, uin
   const hipStream_t st = as_stream(stream);
   auto go = [&](auto norm) {
     constexpr bool NORM = decltype(norm)::value;
-    switch (threads_for(dim0, k)) {
-      case 128u: return launch_top_k<T, 128, 1024, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
-      case 256u: return launch_top_k<T, 256, 1536, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
-      case 512u: return launch_top_k<T, 512, 2560, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
-      default: return launch_top_k<T, 1024, 4096, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
-    }
+    if (k > kFew) return launch_top_k<T, 256, int(kMaxSlots) * 2, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+    if (threads_for(dim0, k) == 128u) return launch_top_k<T, 128, int(kFew) * 2, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+    return launch_top_k<T, 256, int(kFew) * 2, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
   };
   return log_norm != nullptr ? go(std::true_type{}) : go(std::false_type{});
 }
