@@ -273,9 +273,10 @@ __device__ __attribute__((noinline)) uint32_t select_again(const T *xr, uint32_t
   return have;
 }
 
-constexpr uint32_t kCounted = 512;
-// The result of a row from its entries in LDS, at least the k largest of them, and empty slots behind.  Up to 512 entries are
-// counted against each other, each by one to eight neighbouring threads; more are sorted.
+constexpr uint32_t kCounted = 256;
+// The result of a row from its entries in LDS, at least the k largest of them, and empty slots behind.  Up to 256 entries are
+// counted against each other, each by one to eight neighbouring threads; more are sorted (64 rows of which 200 of 131072
+// are kept: 32 us, 36 where up to 512 are counted).
 template <int THREADS>
 __device__ inline void write_result(uint64_t *entries, uint32_t count, size_t row, uint32_t k, float *value, uint32_t *index) {
   if (count <= kCounted) {
@@ -356,6 +357,11 @@ __device__ inline uint32_t key_of_segments(const float *segment, uint32_t segmen
 // largest; these are read again, and of their values those that reach the threshold are ranked and written.  Rows for which
 // there are too many (thousands of ties at the threshold, the largest values all in few threads' segments) are selected from
 // with one or more further passes.
+//
+// Bound by reading: [2048, 131072] bf16 with the norm 95 us (5.6 TB/s) for k = 1, 103 us (5.2) for k = 64, 240 us for k = 1000,
+// whose 1200 candidates are sorted; without the norm 92 us.  With 8 segments a thread the 64 take 111 us and the 1000
+// 1742, with 32 103 and 294; with two groups of a thread on their way together instead of four the 64 take 114.  [512,
+// 131072] f32 49 us of random values, 112 of zeros, 58 in rising order; bf16 29, 75 and 316.
 template <typename T, int THREADS, int SHORT, bool NORM>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS == 128 && sizeof(T) == 4 ? 5 : 4))) void top_k_kernel(
     uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc, double inv_t, Cut cut, const T *__restrict__ x,
@@ -364,7 +370,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
   constexpr int U = 4;  // groups of a thread together
   constexpr uint32_t WAVES = THREADS / kWave;
   constexpr uint32_t kTile = uint32_t(THREADS) * uint32_t(U);
-  constexpr uint32_t kList = uint32_t(kSegments * THREADS) / 2u, kShort = SHORT;  // (kShort >= k: launch_top_k() sees to it)
+  constexpr uint32_t kList = uint32_t(kSegments * THREADS) / 2u, kShort = SHORT;  // (twice the largest k it is launched for)
   __shared__ __align__(16) uint64_t list[kList];
   __shared__ __align__(16) uint64_t best[kShort + 64u];
   __shared__ RadixLds radix;
@@ -488,7 +494,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
     if (have > kList) {
       have = select_again<T, THREADS>(xr, count, from, top, k, list, kList, best, kShort, &radix);
       found = best;
-    } else if (have > kCounted / 2u) {
+    } else if (have > kCounted) {
       const uint32_t few = drop_small<T, THREADS>(list, have, k, best, kShort, wave_key, &taken);
       if (few <= kShort) {
         have = few;
@@ -574,17 +580,16 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
   }
 }
 
-// Threads of a workgroup: a wave's 64 lanes speak for its share of k, so two or four waves take up to 128, eight up to 256, sixteen
-// more.  Two for short rows: 65536 rows of 1000 floats 100 against 200 us, 8192 of 16000 bf16 62 against 74; 1024 of 32768
-// 35 against 28.  Eight for k = 200: 156 against 203 us with sixteen.
+// Threads of a workgroup: two waves for short rows, 8192 of 16000 bf16 64 against 97 us with four; four for long ones, 333 of
+// 50257 halves 18.6 against 27 with two.  k > 256 takes four and more room in LDS.
 constexpr uint32_t kFew = 256;
 uint32_t threads_for(uint32_t n, uint32_t k) { return n <= 16384u && k <= kFew ? 128u : 256u; }
 
-// Parts of at least 4096 values, no more than bring the launch to eight waves a CU, and with room for three times k entries
+// Parts of at least 8192 values, no more than bring the launch to eight waves a CU, and with room for three times k entries
 // each among those that are joined (a part leaves little more than k).
 Cut cut_row(uint32_t n, uint32_t rows, uint32_t k, uint32_t threads) {
   uint64_t parts = uint64_t(device_cu_count()) * (512u / threads) / rows;
-  if (parts > n / 4096u) parts = n / 4096u;
+  if (parts > n / 8192u) parts = n / 8192u;
   if (parts > 64u) parts = 64u;
   if (k != 0u && parts > kJoined / (3u * k)) parts = kJoined / (3u * k);
   if (parts <= 1u) return Cut{1u, n};
@@ -602,7 +607,6 @@ PartBytes part_bytes(uint32_t rows, const Cut &cut) {
 template <typename T, int THREADS, int SHORT, bool NORM>
 int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, uint32_t k, float temperature, const T *x,
                  float *value, uint32_t *index, float *log_norm, hipStream_t st) {
-  if (k > uint32_t(SHORT)) return refuse(symbol, "more slots than the kernel has room for");  // (not reached)
   const Cut cut = cut_row(n, rows, k, THREADS);
   const uint64_t items = uint64_t(rows) * cut.parts;
   const uint32_t most = 1u << 24, grid = items < most ? uint32_t(items) : most;
@@ -638,9 +642,13 @@ int top_k(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, uin
   const hipStream_t st = as_stream(stream);
   auto go = [&](auto norm) {
     constexpr bool NORM = decltype(norm)::value;
-    if (k > kFew) return launch_top_k<T, 256, int(kMaxSlots) * 2, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
-    if (threads_for(dim0, k) == 128u) return launch_top_k<T, 128, int(kFew) * 2, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
-    return launch_top_k<T, 256, int(kFew) * 2, NORM>(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
+    auto *launch = &launch_top_k<T, 256, int(kFew) * 2, NORM>;
+    if (k > kFew) {
+      launch = &launch_top_k<T, 256, int(kMaxSlots) * 2, NORM>;
+    } else if (threads_for(dim0, k) == 128u) {
+      launch = &launch_top_k<T, 128, int(kFew) * 2, NORM>;
+    }
+    return launch(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
   };
   return log_norm != nullptr ? go(std::true_type{}) : go(std::false_type{});
 }
