@@ -322,6 +322,7 @@ __device__ inline void write_result(uint64_t *entries, uint32_t count, size_t ro
 // A part of a row: rows are cut into `parts` of `per` values where there are too few to fill the GPU.
 struct Cut {
   uint32_t parts, per;
+  bool near;
 };
 
 // What the parts of a row leave for the kernel that joins them.
@@ -331,6 +332,16 @@ struct PartResults {
   SoftmaxSum *stats;  // [parts, rows]
   uint32_t quota;
 };
+
+// U groups of a thread, `step` apart from g on: what load_tile() does for groups that lie THREADS apart.
+template <typename T, int U>
+__device__ inline void load_apart(const RowSpan<T> &span, const T *row, uint32_t g, uint32_t step, u32x4 (&q)[U]) {
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t at = min(g + uint32_t(u) * step, span.groups - 1u);
+    q[u] = load_stream<0, int(sizeof(T))>(reinterpret_cast<const u32x4 *>(row + size_t(span.first(at))));
+  }
+}
 
 // A key that at least `share` of a wave's segments reach, from the largest values of each lane's segments in LDS.
 template <typename T, int THREADS>
@@ -351,17 +362,37 @@ __device__ inline uint32_t key_of_segments(const float *segment, uint32_t segmen
   return whole_key<T>(t);
 }
 
+// The largest key, but for its low bits, that k of the threads reach, by every wave alike; 0 where fewer hold a key.
+template <typename T, int THREADS>
+__device__ inline uint32_t key_of_threads(const uint32_t *thread_key, uint32_t k) {
+  constexpr int EACH = THREADS / kWave;
+  uint32_t key[EACH], t = 0u;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) key[i] = thread_key[(threadIdx.x & (kWave - 1)) + uint32_t(i * kWave)];
+#pragma unroll
+  for (uint32_t bit = 0x80000000u; bit >= LowestBit<T>::value; bit >>= 1) {
+    uint32_t reached = 0u;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) reached += uint32_t(__popcll(__ballot(key[i] >= (t | bit))));
+    if (reached >= k) t |= bit;
+  }
+  return whole_key<T>(t);
+}
+
 // One workgroup a part of a row, which it streams once.  A thread leaves the largest value of each of its segments (up to 16: a
-// 16-byte group each, or as many groups as that takes) in LDS.  A threshold that k segments of the row reach -- every wave finds
-// what its share of k reaches, the least of the waves counts -- names the few segments that can hold one of the k
-// largest; these are read again, and of their values those that reach the threshold are ranked and written.  Rows for which
-// there are too many (thousands of ties at the threshold, the largest values all in few threads' segments) are selected from
-// with one or more further passes.
+// 16-byte group each, or as many groups as that takes) in LDS.  A threshold that k of the threads' largest values reach (of long
+// rows; of short ones every wave finds what its share of k reaches, the least of the waves counts; for large k the
+// segments count, not the threads) names the few segments that can hold one of the k largest; these are read again,
+// and of their values those that reach the threshold are ranked and written.  Rows for which there are too many
+// (thousands of ties at the threshold, the largest values all in few segments) are selected from with further passes.
 //
-// Bound by reading: [2048, 131072] bf16 with the norm 95 us (5.6 TB/s) for k = 1, 103 us (5.2) for k = 64, 240 us for k = 1000,
-// whose 1200 candidates are sorted; without the norm 92 us.  With 8 segments a thread the 64 take 111 us and the 1000
-// 1742, with 32 103 and 294; with two groups of a thread on their way together instead of four the 64 take 114.  [512,
-// 131072] f32 49 us of random values, 112 of zeros, 58 in rising order; bf16 29, 75 and 316.
+// Bound by reading: [2048, 131072] bf16 with the norm 95 us (5.6 TB/s) for k = 1, 99 us (5.4) for k = 64, 228 us for k = 1000,
+// whose 1200 candidates are sorted.  A threshold held while the row streams, with a list of what reaches it, took 114 us:
+// its branches, barriers and LDS additions cost more than the 75 segments that are read again here.  With 8 segments a
+// thread the 64 take 111 us and the 1000 1742, with 32 103 and 294; with two groups of a thread on their way together
+// instead of four the 64 take 114.  The threads' threshold instead of the waves' is as quick for random values and eight
+// times as quick for rows in falling order.  [512, 131072] f32 47 us of random values, 111 of zeros, 79 in rising order;
+// bf16 29, 75 and 46.
 template <typename T, int THREADS, int SHORT, bool NORM>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS == 128 && sizeof(T) == 4 ? 5 : 4))) void top_k_kernel(
     uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc, double inv_t, Cut cut, const T *__restrict__ x,
@@ -379,6 +410,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
   __shared__ SoftmaxSum sums[WAVES];
   float *const segment = reinterpret_cast<float *>(list);          // [segments, threads]; until the list is filled
   uint32_t *const names = reinterpret_cast<uint32_t *>(best);      // of segments to be read again
+  uint32_t *const thread_key = names + kShort;                     // (behind them in the same place)
   const uint32_t wave = threadIdx.x / kWave;
   const uint32_t share = (k + WAVES - 1u) / WAVES;
   const uint64_t items = uint64_t(rows) * cut.parts;
@@ -394,12 +426,14 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
     const uint32_t span_tiles = (tiles + uint32_t(kSegments) - 1u) / uint32_t(kSegments);
     const uint32_t each = fine ? 1u : span_tiles * uint32_t(U);  // groups of a segment
     const uint32_t segments = (turns + each - 1u) / each;
+    const bool near = THREADS > 128 && cut.near && !fine;  // a thread's groups of a tile lie side by side, not THREADS apart
+    const uint32_t step = near ? 1u : uint32_t(THREADS), own_first = near ? threadIdx.x * uint32_t(U) : threadIdx.x;
     if (threadIdx.x == 0) named = listed = 0u;
     float top = kMinusInf;
     SoftmaxSum st = {-sc.limit, 0.0f};
     if (span.groups != 0u) {
       u32x4 q[U];
-      load_tile<T, THREADS, U>(span, xr, threadIdx.x, q);
+      load_apart<T, U>(span, xr, own_first, step, q);
       float segment_top = kMinusInf;
       uint32_t left = span_tiles;
       float *own = segment + threadIdx.x;
@@ -407,9 +441,12 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
         float v[U * W];
         u32x4 next[U];
         const bool more = span.groups - base > kTile;
-        load_tile<T, THREADS, U>(span, xr, base + kTile + threadIdx.x, next);
+        load_apart<T, U>(span, xr, base + kTile + own_first, step, next);
         unpack_tile<T, U>(q, v);
-        if (!more) mask_tile<T, THREADS, U>(span, base + threadIdx.x, kMinusInf, v);
+        if (!more) {
+#pragma unroll
+          for (int i = 0; i < U * W; ++i) v[i] = base + own_first + uint32_t(i / W) * step < span.groups ? v[i] : kMinusInf;
+        }
         float tile_top = kMinusInf;
         if (fine) {
 #pragma unroll
@@ -439,29 +476,38 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
         for (int u = 0; u < U; ++u) q[u] = next[u];
       }
     }
-    // (up to half of a wave's lanes: the lanes' largest values instead of the segments', 1.4 times k values reach what they give)
-    const uint32_t t = share <= uint32_t(kWave / 2) ? key_reached_by<T>(key_of(top), share)
-                                                    : key_of_segments<T, THREADS>(segment, segments, share);
-    if ((threadIdx.x & (kWave - 1)) == 0) wave_key[wave] = t;
-    __syncthreads();
-    uint32_t low = wave_key[0];
+    // (up to half of the threads: their largest values instead of the segments', 1.4 times k values reach what they give)
+    uint32_t low;
+    if (THREADS > 128 && k <= uint32_t(THREADS) / 2u) {
+      thread_key[threadIdx.x] = key_of(top);
+      __syncthreads();
+      low = key_of_threads<T, THREADS>(thread_key, k);
+    } else {
+      const uint32_t t = share <= uint32_t(kWave / 2) ? key_reached_by<T>(key_of(top), share)
+                                                      : key_of_segments<T, THREADS>(segment, segments, share);
+      if ((threadIdx.x & (kWave - 1)) == 0) wave_key[wave] = t;
+      __syncthreads();
+      low = wave_key[0];
 #pragma unroll
-    for (uint32_t w = 1; w < WAVES; ++w) low = min(low, wave_key[w]);
+      for (uint32_t w = 1; w < WAVES; ++w) low = min(low, wave_key[w]);
+    }
     const float least = low < kLowestKey ? -__FLT_MAX__ : value_of(low);
     uint32_t marked = 0u;
 #pragma unroll 4
     for (uint32_t j = 0; j < segments; ++j) marked |= uint32_t(segment[j * uint32_t(THREADS) + threadIdx.x] >= least) << j;
     uint32_t place = reserve(&named, uint32_t(__popc(marked)));
-    for (; marked != 0u && place < 2u * kShort; marked &= marked - 1u) {
-      names[place++] = (uint32_t(__ffs(int(marked))) - 1u) * each * uint32_t(THREADS) + threadIdx.x;  // its first group
+    for (; marked != 0u && place < kShort; marked &= marked - 1u) {
+      names[place++] = (uint32_t(__ffs(int(marked))) - 1u) * uint32_t(THREADS) + threadIdx.x;
     }
     __syncthreads();
-    uint32_t have = named <= 2u * kShort ? 0u : kNoClass;
+    uint32_t have = named <= kShort ? 0u : kNoClass;
     if (have == 0u) {
       const uint32_t again = named * each;
       for (uint32_t base = 0; base < again; base += uint32_t(THREADS)) {
         const uint32_t i = min(base + threadIdx.x, again - 1u);
-        const uint32_t g = names[i / each] + i % each * uint32_t(THREADS);
+        const uint32_t name = names[i / each], turn = name / uint32_t(THREADS) * each + i % each;
+        const uint32_t thread = name % uint32_t(THREADS), tile = turn / uint32_t(U), u = turn % uint32_t(U);
+        const uint32_t g = tile * kTile + (near ? thread * uint32_t(U) + u : thread + u * uint32_t(THREADS));
         const bool mine = base + threadIdx.x < again && g < span.groups;
         float v[W];
         unpack(load_stream<0, int(sizeof(T))>(reinterpret_cast<const u32x4 *>(xr + size_t(span.first(min(g, span.groups - 1u))))), v, x);
@@ -585,16 +631,22 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
 constexpr uint32_t kFew = 256;
 uint32_t threads_for(uint32_t n, uint32_t k) { return n <= 16384u && k <= kFew ? 128u : 256u; }
 
+// Arrays from this size on, which memory and not the last cache delivers, are read with a thread's four groups side by side: the
+// segments read again lie in a quarter of the lines (86 MB of [2048, 131072] bf16, 103 against 99 us; [512, 131072] f32
+// 54.8 against 52.0), below it THREADS apart (512 rows of bf16 30.8 against 33.4).
+constexpr uint64_t kNearBytes = uint64_t(192) << 20;
+
 // Parts of at least 8192 values, no more than bring the launch to eight waves a CU, and with room for three times k entries
 // each among those that are joined (a part leaves little more than k).
-Cut cut_row(uint32_t n, uint32_t rows, uint32_t k, uint32_t threads) {
+Cut cut_row(uint32_t n, uint32_t rows, uint32_t k, uint32_t threads, uint32_t size) {
+  const bool near = uint64_t(n) * rows * size >= kNearBytes;
   uint64_t parts = uint64_t(device_cu_count()) * (512u / threads) / rows;
   if (parts > n / 8192u) parts = n / 8192u;
   if (parts > 64u) parts = 64u;
   if (k != 0u && parts > kJoined / (3u * k)) parts = kJoined / (3u * k);
-  if (parts <= 1u) return Cut{1u, n};
+  if (parts <= 1u) return Cut{1u, n, near};
   const uint64_t per = ((uint64_t(n) + parts - 1u) / parts + 1023u) / 1024u * 1024u;
-  return Cut{uint32_t((n + per - 1u) / per), uint32_t(per)};
+  return Cut{uint32_t((n + per - 1u) / per), uint32_t(per), near};
 }
 struct PartBytes {
   size_t entries, stats, counts;
@@ -607,7 +659,7 @@ PartBytes part_bytes(uint32_t rows, const Cut &cut) {
 template <typename T, int THREADS, int SHORT, bool NORM>
 int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, uint32_t k, float temperature, const T *x,
                  float *value, uint32_t *index, float *log_norm, hipStream_t st) {
-  const Cut cut = cut_row(n, rows, k, THREADS);
+  const Cut cut = cut_row(n, rows, k, THREADS, uint32_t(sizeof(T)));
   const uint64_t items = uint64_t(rows) * cut.parts;
   const uint32_t most = 1u << 24, grid = items < most ? uint32_t(items) : most;
   const Scale sc = scale_for(temperature);
@@ -657,7 +709,7 @@ int top_k(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, uin
 
 size_t top_k_scratch(uint32_t classes, uint32_t rows, uint32_t k) {
   if (rows == 0u || k > kMaxSlots) return 0u;
-  const Cut cut = cut_row(classes, rows, k, threads_for(classes, k));
+  const Cut cut = cut_row(classes, rows, k, threads_for(classes, k), 1u);
   if (cut.parts == 1u) return 0u;
   const PartBytes b = part_bytes(rows, cut);
   return b.entries + b.stats + b.counts;

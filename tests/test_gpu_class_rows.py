@@ -170,6 +170,47 @@ def test_top_k_masks(kind):
             check_top_k(kind, x, k, what=f"{kind} n={n} k={k}")
 
 
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("k", [1, 64, 200, 1000])
+def test_top_k_of_large_arrays(kind, k):
+    # more than the last cache holds: 800 rows (400 of floats) of an odd length, and rows in order, of ties and of masks
+    n, stride = 131071, 131075
+    rows = 800 if kind != "f32" else 400
+    g = torch.Generator("cuda").manual_seed(k)
+    buf = torch.randn(1 + rows * stride, generator=g, device="cuda").mul_(3.0).to(TYPES[kind])
+    grid = buf[1:].view(rows, stride)
+    ramp = torch.arange(n, device="cuda") / 1024.0 - 60.0
+    grid[0, :n], grid[1, :n] = ramp.to(TYPES[kind]), ramp.flip(0).to(TYPES[kind])
+    grid[2], grid[3] = 0.0, torch.finfo(TYPES[kind]).min
+    grid[3, 5::9001] = 1.0
+    grid[4] = -float("inf")
+    grid[4, 7::30011] = -2.0
+    grid[5, ::256] += 20.0                         # the largest all in a few threads' places
+    grid[6, 1000:1300] += 20.0                     # ... and all in one place
+    x = grid[:, :n].float()
+    grid[:, n:] = float("inf")                     # what lies behind a row is not looked at
+    value, check_v = guarded(rows * k)
+    index, check_i = guarded(rows * k, torch.int32)
+    norm, check_n = guarded(rows)
+    call("anode_gpu_top_k_rows_" + kind, n, rows, stride, k, 2.0, buf[1:], value, index, norm)
+    for c in (check_v, check_i, check_n):
+        c("top_k of a large array")
+    v, i = value.view(rows, k), index.view(rows, k)
+    want, _ = torch.sort(x, dim=1, descending=True)
+    want = want[:, :k]
+    assert bool((v == want).all())
+    found = want > -float("inf")
+    assert bool((x.gather(1, i.long().clamp(0, n - 1))[found] == want[found]).all()) and bool((i[~found] == -1).all())
+    tied = (v[:, 1:] == v[:, :-1]) & found[:, 1:]
+    assert bool((i[:, 1:] > i[:, :-1])[tied].all())  # of equal values the lower class first: so all differ
+    for r in (0, 2, 3, 4, 5, 6, rows - 1):
+        row = x[r:r + 1].cpu().numpy()
+        assert np.array_equal(host(i[r]).view(np.uint32), ref.top_k(row, k)[1][0]), r
+        top, total = ref.stats(row, 2.0)
+        norm_want = top[0] / 2.0 + np.log(total[0])
+        assert abs(float(norm[r]) - norm_want) <= ref.sum_bound(row[0], 2.0) + U * abs(norm_want), r
+
+
 def test_top_k_without_norm_and_with_norm_alone():
     g = np.random.default_rng(5)
     x = logits(g, 4, 3000, "f32")
