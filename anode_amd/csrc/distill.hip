@@ -23,10 +23,9 @@ struct Teacher {
   __device__ bool counts(size_t at, uint32_t n) const { return index[at] < n && value[at] > kMinusInf; }
 };
 
-// A row's teacher as the wave knows it that looked at the slots: the log of slot j's probability is
-// value * inv_t - shift + log_scale.
+// A row's teacher as the wave knows it that looked at the slots: slot j's probability is exp(value * inv_t - shift) * scale.
 struct TeacherRow {
-  double shift, log_scale, mass;
+  double shift, scale, mass;
   bool any;  // a slot counts
 };
 
@@ -40,15 +39,15 @@ struct Slots {
   uint32_t *next;   // [k]: the next slot of the same thread, or kNoClass
   uint32_t *head;   // [threads]: a thread's first slot, or kNoClass
   uint32_t *turns;  // [threads]: bit i for a slot in the thread's groups of turn i, i + 32, ...
-  uint32_t *seen;   // [kSeen], for k > 64: the classes met so far
+  volatile uint16_t *seen;  // [kSeen]: slots' numbers, at the places that their classes give
 };
-constexpr uint32_t kSeen = 2u * kMaxSlots;
+constexpr uint32_t kSeen = 2048;  // (the leading 11 bits of a product)
 __device__ inline Slots slots_in(uint32_t *lds, uint32_t k, uint32_t threads) {
   float *f = reinterpret_cast<float *>(lds);
   uint32_t *t = lds + 5u * k;
-  return Slots{f, f + k, f + 2u * k, lds + 3u * k, lds + 4u * k, t, t + threads, t + 2u * threads};
+  return Slots{f, f + k, f + 2u * k, lds + 3u * k, lds + 4u * k, t, t + threads, reinterpret_cast<volatile uint16_t *>(t + 2u * threads)};
 }
-uint32_t slot_bytes(uint32_t k, uint32_t threads) { return 20u * k + 8u * threads + (k > uint32_t(kWave) ? 4u * kSeen : 0u); }
+uint32_t slot_bytes(uint32_t k, uint32_t threads) { return 20u * k + 8u * threads + 2u * kSeen; }
 
 // Reads the slots of a row, by one whole wave: x is the row, n its length.  LOSS: the student's logits too, which the loss asks for
 // and the gradient does not.
@@ -56,7 +55,7 @@ template <bool LOSS, typename T>
 __device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x, uint32_t n, double inv_t, const Slots &s) {
   const uint32_t lane = threadIdx.x & (kWave - 1);
   const size_t first = row * t.k;
-  TeacherRow r = {0.0, 0.0, 0.0, false};
+  TeacherRow r = {0.0, 1.0, 0.0, false};
   float top = kMinusInf;
   for (uint32_t j = lane; j < t.k; j += kWave) {
     const uint32_t at = t.index[first + j];
@@ -80,39 +79,39 @@ __device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x
   sum = lanes_sum(sum);
   r.mass = sum;
   if (t.log_norm == nullptr) {
-    const float scale = float(1.0 / sum);
-    for (uint32_t j = lane; j < t.k; j += kWave) s.p[j] *= scale;
+    r.scale = 1.0 / sum;
+    for (uint32_t j = lane; j < t.k; j += kWave) s.p[j] *= float(r.scale);
     r.mass = 1.0;
-    r.log_scale = -log(sum);
   }
   return r;
 }
 
-// Whether a class is named twice, by the wave that read the slots: among 64 slots by comparing, beyond in a table.
+// Whether a class is named twice, by the wave that read the slots: every slot leaves its number at a place of a table that the class
+// gives, and looks whose number is there.  Another one's of the same class: twice.  Another class's: once more, at
+// another place (the slot whose number stands is done each time, so this ends).  What the table held before does not matter.
 __device__ inline bool repeated_slots(uint32_t k, const Slots &s) {
   const uint32_t lane = threadIdx.x & (kWave - 1);
-  bool twice = false;
-  if (k <= uint32_t(kWave)) {
-    const uint32_t mine = lane < k ? s.index[lane] : kNoClass;
-    for (uint32_t i = 0; i < k; ++i) twice |= from_lane(mine, int(i)) == mine && i != lane;
-    return __any(twice && mine != kNoClass);
-  }
-  for (uint32_t i = lane; i < kSeen; i += kWave) s.seen[i] = kNoClass;
-  for (uint32_t j = lane; j < k; j += kWave) {
-    const uint32_t mine = s.index[j];
-    if (mine == kNoClass) continue;
-    uint32_t at = (mine * 2654435761u) >> 21;  // (kSeen = 2^11 places, at most half of them taken)
-    for (;;) {
-      const uint32_t held = atomicCAS(&s.seen[at], kNoClass, mine);
-      if (held == kNoClass) break;
-      if (held == mine) {
-        twice = true;
-        break;
-      }
-      at = (at + 1u) & (kSeen - 1u);
+  uint32_t open = 0u;  // bit i: slot lane + 64 i has not found its place
+  for (uint32_t j = lane, bit = 1u; j < k; j += kWave, bit <<= 1) open |= s.index[j] != kNoClass ? bit : 0u;
+  for (uint32_t factor = 2654435761u;; factor = factor * 0x9e3779b1u + 0x7f4a7c16u | 1u) {
+    for (uint32_t j = lane, bit = 1u; j < k; j += kWave, bit <<= 1) {
+      if ((open & bit) != 0u) s.seen[(s.index[j] * factor) >> 21] = uint16_t(j);
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    bool twice = false;
+    for (uint32_t j = lane, bit = 1u; j < k; j += kWave, bit <<= 1) {
+      if ((open & bit) == 0u) continue;
+      const uint32_t mine = s.index[j], there = s.seen[(mine * factor) >> 21];
+      if (there == j) {
+        open &= ~bit;
+      } else {
+        twice |= s.index[there] == mine;
+      }
+    }
+    if (__any(twice)) return true;
+    if (!__any(open != 0u)) return false;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
-  return __any(twice);
 }
 
 // Deals the slots that lie in [from, from + n of the span) of the row to the streaming threads, w times their
@@ -165,13 +164,13 @@ __device__ inline void take_slots(const Slots &s, uint32_t first, float (&v)[W])
 // The row's loss from its slots in LDS, by the wave that read them.
 __device__ inline float slots_loss(const Teacher &t, size_t row, SoftmaxSum st, double inv_t, const TeacherRow &tr, const Slots &s) {
   if (!tr.any) return 0.0f;
-  const double log_s = log(double(st.s));
+  const double logs = log(double(st.s) * tr.scale);  // ln S and the logarithm of the probabilities' scale
   double loss = 0.0;
   for (uint32_t j = threadIdx.x & (kWave - 1); j < t.k; j += kWave) {
     const float p = s.p[j];
     if (s.index[j] == kNoClass || p == 0.0f) continue;  // (a slot without mass adds nothing, whatever the student says)
-    const double lp = double(t.value[row * t.k + j]) * inv_t - tr.shift + tr.log_scale;
-    loss += double(p) * (lp - ((double(s.x[j]) - double(st.m)) * inv_t - log_s));
+    const double lp = double(t.value[row * t.k + j]) * inv_t - tr.shift;
+    loss += double(p) * (lp - (double(s.x[j]) - double(st.m)) * inv_t + logs);
   }
   return float(lanes_sum(loss));
 }
@@ -204,24 +203,22 @@ __device__ inline float row_loss(const Teacher &t, size_t row, const T *x, uint3
   }
   top = wave_max(top);
   if (!(top > kMinusInf)) return 0.0f;
-  // with e_k = exp(a_k): loss = sum e_k (a_k - ln q_k) where the norm is given, else that over sum e_k, less its log
+  // with e_k = exp(a_k), M = sum e_k: loss = sum e_k (a_k - (x_k - m) / T) + M ln S where the norm is given, else the sum over M,
+  // and ln (S / M)
   const double shift = t.log_norm != nullptr ? double(t.log_norm[row]) : double(top) * inv_t;
-  const double log_s = log(double(st.s));
   double mass = 0.0, loss = 0.0;
   for (uint32_t j = lane; j < t.k; j += kWave) {
     const LaneSlot s = j == lane ? mine : lane_slot(t, row, x, n, j);
     if (!s.counts) continue;
     const double a = double(s.value) * inv_t - shift, e = exp(a);
-    const double lq = (double(s.x) - double(st.m)) * inv_t - log_s;
-    if (e != 0.0) loss += e * (a - lq);  // (a slot without mass adds nothing, whatever the student says)
+    if (e != 0.0) loss += e * (a - (double(s.x) - double(st.m)) * inv_t);  // (a slot without mass adds nothing, whatever the student says)
     mass += e;
   }
   loss = lanes_sum(loss);
-  if (t.log_norm == nullptr) {
-    mass = lanes_sum(mass);
-    loss = loss / mass - log(mass);
-  }
-  return float(loss);
+  mass = lanes_sum(mass);
+  if (mass == 0.0) return 0.0f;
+  const double share = t.log_norm != nullptr ? 1.0 : 1.0 / mass, logs = log(double(st.s) * share);
+  return float((loss + mass * logs) * share);
 }
 
 constexpr int kUnroll = 4;  // 16-byte groups of a thread on their way together
