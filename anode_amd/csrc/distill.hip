@@ -232,7 +232,7 @@ struct Parts {
 };
 
 // One workgroup a row: statistics and loss.
-template <typename T, int THREADS>
+template <typename T, int THREADS, int U>
 __global__ __launch_bounds__(THREADS) void distill_kernel(uint32_t n, uint32_t rows, size_t stride, Scale sc, double inv_t,
                                                           const T *__restrict__ x, Teacher t, float *__restrict__ loss,
                                                           float *__restrict__ row_max, float *__restrict__ row_sum) {
@@ -242,7 +242,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(uint32_t n, uint32_t r
     LaneSlot slot = {};
     if (threadIdx.x < uint32_t(kWave)) slot = lane_slot(t, r, xr, n, threadIdx.x);
     const SoftmaxSum st =
-        finish_stats<T, THREADS>(stream_stats<T, THREADS, kUnroll>(RowSpan<T>(n, 0u), xr, sc), xr, n, sc, lds);
+        finish_stats<T, THREADS>(stream_stats<T, THREADS, U>(RowSpan<T>(n, 0u), xr, sc), xr, n, sc, lds);
     if (threadIdx.x < uint32_t(kWave)) {
       const float l = row_loss(t, r, xr, n, st, inv_t, slot);
       if (threadIdx.x == 0) {
@@ -384,7 +384,7 @@ struct Joined {
 
 // One workgroup a part of a row.  JOIN: the row's statistics are put together from its parts by every workgroup for itself, and
 // the first part's writes them and the loss.
-template <typename T, int THREADS, bool ACC, bool JOIN, int NT>
+template <typename T, int THREADS, int U, bool ACC, bool JOIN, int NT>
 __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32_t rows, size_t stride, Scale sc, double inv_t,
                                                               Parts ps, const float *__restrict__ dy, const T *x, Teacher t,
                                                               Joined jn, T *dx) {
@@ -400,8 +400,8 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32
     const T *xr = x + r * stride;
     T *dxr = dx + r * stride;
     const RowSpan<T> span(count, values_to_line(dxr + from));
-    u32x4 q[kUnroll];
-    if (span.groups != 0u) load_tile<T, THREADS, kUnroll>(span, xr + from, threadIdx.x, q);
+    u32x4 q[U];
+    if (span.groups != 0u) load_tile<T, THREADS, U>(span, xr + from, threadIdx.x, q);
     SoftmaxSum st;
     if (JOIN) {
       st = join_parts<T, THREADS>(jn.partial + r * ps.parts, ps.parts, xr, n, sc, plain_lds);
@@ -427,9 +427,9 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32
     if (!ACC || d.any) {
       single_grad<T, THREADS, ACC>(span, xr + from, dxr + from, from, d, slots);
       if (d.fast) {
-        stream_groups<T, THREADS, kUnroll, ACC, NT, true>(span, xr + from, dxr + from, from, d, slots, q);
+        stream_groups<T, THREADS, U, ACC, NT, true>(span, xr + from, dxr + from, from, d, slots, q);
       } else {
-        stream_groups<T, THREADS, kUnroll, ACC, 0, false>(span, xr + from, dxr + from, from, d, slots, q);
+        stream_groups<T, THREADS, U, ACC, 0, false>(span, xr + from, dxr + from, from, d, slots, q);
       }
     }
     __syncthreads();
@@ -641,6 +641,10 @@ int check_arrays(const char *symbol, const Shape &s, const T *x, const Teacher &
 // do not fill the GPU the gradient takes four waves from 4 KB on: 1024 rows of 16 KB 15.6 against 22 us, 2048 rows
 // 27.5 against 25.8.
 constexpr size_t kWaveRow = 16384;
+// Up to here it has two groups of a thread on their way together, and room for more waves on the SIMD: 65536 rows of 1000 bf16 61.6
+// against 77 us for the loss and 133 against 170 with the gradient, of 1000 floats 73 and 80, 165 and 189; rows of 8000
+// bytes 17.4 against 16.7.  (The fused call holds two groups a thread up to half of it: 118 against 144 us.)
+constexpr size_t kShortRow = 4096;
 
 // Bytes of a row that the workgroups of the fused call hold in registers: those of a wave, and of the three smaller of
 // distill_held_kernel.  At each border the smaller one is the quicker: 94.8 against 182 us (32768 rows of 4 KB), 66.5
@@ -689,10 +693,18 @@ int distill(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, f
     part_stats_kernel<T><<<grid_for(uint64_t(s.rows) * ps.parts), kBlock, 0, st>>>(s.n, s.rows, s.stride, s.sc, ps, x, partial);
     distill_join_kernel<T><<<grid_for(s.rows), kWave, 0, st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, ps.parts, x, t, partial, loss,
                                                              row_max, row_sum);
-  } else if (size_t(s.n) * sizeof(T) <= kWaveRow) {
-    distill_kernel<T, kWave><<<grid_for(s.rows), kWave, 0, st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, loss, row_max, row_sum);
   } else {
-    distill_kernel<T, kBlock><<<grid_for(s.rows), kBlock, 0, st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, loss, row_max, row_sum);
+    auto go = [&](auto kernel, uint32_t threads) {
+      kernel<<<grid_for(s.rows), threads, 0, st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, loss, row_max, row_sum);
+    };
+    const size_t row = size_t(s.n) * sizeof(T);
+    if (row <= kShortRow) {
+      go(distill_kernel<T, kWave, 2>, kWave);
+    } else if (row <= kWaveRow) {
+      go(distill_kernel<T, kWave, kUnroll>, kWave);
+    } else {
+      go(distill_kernel<T, kBlock, kUnroll>, kBlock);
+    }
   }
   note_launch(symbol);
   return 0;
@@ -704,13 +716,16 @@ void launch_bwd(const Shape &s, const float *dy, const T *x, const Teacher &t, c
   const Parts ps = cut_rows<T>(s);
   const uint32_t grid = grid_for(uint64_t(s.rows) * ps.parts);
   const Joined jn = {nullptr, nullptr, const_cast<float *>(row_max), const_cast<float *>(row_sum)};  // (read only)
+  auto go = [&](auto kernel, uint32_t threads) {
+    kernel<<<grid, threads, slot_bytes(t.k, threads), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, ps, dy, x, t, jn, dx);
+  };
   const size_t row = size_t(s.n) * sizeof(T);
-  if (row <= kHeldByWave || (row <= kWaveRow && s.rows > kWanted)) {
-    distill_bwd_kernel<T, kWave, ACC, false, NT><<<grid, kWave, slot_bytes(t.k, kWave), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t,
-                                                                                             ps, dy, x, t, jn, dx);
+  if (row <= kShortRow) {
+    go(distill_bwd_kernel<T, kWave, 2, ACC, false, NT>, kWave);
+  } else if (row <= kWaveRow && s.rows > kWanted) {
+    go(distill_bwd_kernel<T, kWave, kUnroll, ACC, false, NT>, kWave);
   } else {
-    distill_bwd_kernel<T, kBlock, ACC, false, NT><<<grid, kBlock, slot_bytes(t.k, kBlock), st>>>(s.n, s.rows, s.stride, s.sc,
-                                                                                                s.inv_t, ps, dy, x, t, jn, dx);
+    go(distill_bwd_kernel<T, kBlock, kUnroll, ACC, false, NT>, kBlock);
   }
 }
 
@@ -741,7 +756,9 @@ void launch_fused(const Shape &s, const T *x, const Teacher &t, const float *dy,
     kernel<<<grid_for(s.rows), threads, slot_bytes(t.k, streaming), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, dy, loss, row_max,
                                                               row_sum, dx);
   };
-  if (row <= kHeldByWave) {
+  if (row <= kHeldByWave / 2u) {
+    go(distill_wave_kernel<T, 2, NT>, kWave);
+  } else if (row <= kHeldByWave) {
     go(distill_wave_kernel<T, 4, NT>, kWave);
   } else if (row <= kHeldBySmall) {
     go(distill_held_kernel<T, 192, 6, NT>, 256u);
@@ -777,7 +794,7 @@ int distill_fused(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t str
     SoftmaxSum *partial = static_cast<SoftmaxSum *>(scratch.lease.ptr);
     const uint32_t grid = grid_for(uint64_t(s.rows) * ps.parts);
     part_stats_kernel<T><<<grid, kBlock, 0, st>>>(s.n, s.rows, s.stride, s.sc, ps, x, partial);
-    distill_bwd_kernel<T, kBlock, false, true, 0><<<grid, kBlock, slot_bytes(t.k, kBlock), st>>>(
+    distill_bwd_kernel<T, kBlock, kUnroll, false, true, 0><<<grid, kBlock, slot_bytes(t.k, kBlock), st>>>(
         s.n, s.rows, s.stride, s.sc, s.inv_t, ps, dy, x, t, Joined{partial, loss, row_max, row_sum}, dx);
     note_launch(symbol);
     return 0;
