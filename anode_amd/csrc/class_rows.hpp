@@ -110,6 +110,17 @@ __device__ inline V lanes_sum(V v) {
   return from_lane(lanes_upto(v), kWave - 1);
 }
 
+// The largest of the lanes' values, the same in every lane.
+__device__ inline float lanes_max(float v) {
+  v = fmaxf(v, lane_before<0>(v, v));
+  v = fmaxf(v, lane_before<1>(v, v));
+  v = fmaxf(v, lane_before<2>(v, v));
+  v = fmaxf(v, lane_before<3>(v, v));
+  v = fmaxf(v, lane_before<4>(v, v));
+  v = fmaxf(v, lane_before<5>(v, v));
+  return __shfl(v, kWave - 1, kWave);
+}
+
 // One 16-byte group of a row: W values.
 template <typename T>
 struct Group {
@@ -270,20 +281,14 @@ __device__ inline SoftmaxSum merge(SoftmaxSum a, SoftmaxSum b, float c) {
   r.s = a.s * __builtin_amdgcn_exp2f(a.m * c - shift) + b.s * __builtin_amdgcn_exp2f(b.m * c - shift);
   return r;
 }
-template <int STEP>
-__device__ inline SoftmaxSum merge_before(SoftmaxSum t, float c) {
-  return merge(t, SoftmaxSum{lane_before<STEP>(t.m, t.m), lane_before<STEP>(0.0f, t.s)}, c);
-}
-// The same in every lane of the wave, merged in a fixed order.
+// The same in every lane of the wave, added in a fixed order: first the maximum of all, then each lane's sum about it.  (Merging
+// pairs at every step takes two exponentials each.)
 __device__ inline SoftmaxSum wave_merge(SoftmaxSum t, float c) {
-  t = merge_before<0>(t, c);
-  t = merge_before<1>(t, c);
-  t = merge_before<2>(t, c);
-  t = merge_before<3>(t, c);
-  t = merge_before<4>(t, c);
-  t = merge_before<5>(t, c);
+  SoftmaxSum r = {lanes_max(t.m), 0.0f};
+  r.s = lanes_upto(t.s * __builtin_amdgcn_exp2f(t.m * c - r.m * c));
   // (an exchange, not from_lane(): results in scalar registers push the held rows of distill.hip out of the vector ones)
-  return SoftmaxSum{__shfl(t.m, kWave - 1, kWave), __shfl(t.s, kWave - 1, kWave)};
+  r.s = __shfl(r.s, kWave - 1, kWave);
+  return r;
 }
 // COUNT <= 16 entries in LDS merged, the same in every lane.
 template <int COUNT>
@@ -292,11 +297,19 @@ __device__ inline SoftmaxSum lane_merge(const SoftmaxSum *lds, float c) {
   const uint32_t lane = threadIdx.x & 15u;
   SoftmaxSum t = lds[lane < uint32_t(COUNT) ? lane : 0u];
   if (lane >= uint32_t(COUNT)) t.s = 0.0f;  // (an entry again, of which nothing is added)
-  t = merge_before<0>(t, c);
-  t = merge_before<1>(t, c);
-  t = merge_before<2>(t, c);
-  t = merge_before<3>(t, c);
-  return SoftmaxSum{__shfl(t.m, 15, 16), __shfl(t.s, 15, 16)};
+  SoftmaxSum r = {t.m, 0.0f};
+  r.m = fmaxf(r.m, lane_before<0>(r.m, r.m));
+  r.m = fmaxf(r.m, lane_before<1>(r.m, r.m));
+  r.m = fmaxf(r.m, lane_before<2>(r.m, r.m));
+  r.m = fmaxf(r.m, lane_before<3>(r.m, r.m));
+  r.m = __shfl(r.m, 15, 16);
+  r.s = t.s * __builtin_amdgcn_exp2f(t.m * c - r.m * c);
+  r.s += lane_before<0>(0.0f, r.s);
+  r.s += lane_before<1>(0.0f, r.s);
+  r.s += lane_before<2>(0.0f, r.s);
+  r.s += lane_before<3>(0.0f, r.s);
+  r.s = __shfl(r.s, 15, 16);
+  return r;
 }
 // The same in every thread of the workgroup; `lds` holds one entry a wave.  Ends with a barrier.
 template <int WAVES>

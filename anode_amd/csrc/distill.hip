@@ -66,7 +66,7 @@ __device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x
     if (LOSS) s.x[j] = counts ? float(x[at]) : 0.0f;
     if (counts) top = fmaxf(top, v);
   }
-  top = wave_max(top);
+  top = lanes_max(top);
   r.any = top > kMinusInf;
   if (!r.any) return r;
   r.shift = t.log_norm != nullptr ? double(t.log_norm[row]) : double(top) * inv_t;
@@ -201,7 +201,7 @@ __device__ inline float row_loss(const Teacher &t, size_t row, const T *x, uint3
   for (uint32_t j = lane + kWave; j < t.k; j += kWave) {
     if (t.counts(row * t.k + j, n)) top = fmaxf(top, t.value[row * t.k + j]);
   }
-  top = wave_max(top);
+  top = lanes_max(top);
   if (!(top > kMinusInf)) return 0.0f;
   // with e_k = exp(a_k), M = sum e_k: loss = sum e_k (a_k - (x_k - m) / T) + M ln S where the norm is given, else the sum over M,
   // and ln (S / M)
