@@ -343,12 +343,12 @@ __device__ inline void load_apart(const RowSpan<T> &span, const T *row, uint32_t
   }
 }
 
-// A key that at least `share` of a wave's segments reach, from the largest values of each lane's segments in LDS.
-template <typename T, int THREADS>
+// A key that at least `share` of a wave's segments reach, from the largest values of each lane's segments, MOST at most, in LDS.
+template <typename T, int THREADS, int MOST>
 __device__ inline uint32_t key_of_segments(const float *segment, uint32_t segments, uint32_t share) {
-  uint32_t key[kSegments];
+  uint32_t key[MOST];
 #pragma unroll
-  for (int j = 0; j < kSegments; ++j) {
+  for (int j = 0; j < MOST; ++j) {
     key[j] = uint32_t(j) < segments ? key_of(segment[uint32_t(j) * uint32_t(THREADS) + threadIdx.x]) : 0u;
   }
   uint32_t t = 0u;
@@ -356,7 +356,7 @@ __device__ inline uint32_t key_of_segments(const float *segment, uint32_t segmen
   for (uint32_t bit = 0x80000000u; bit >= LowestBit<T>::value; bit >>= 1) {
     uint32_t reached = 0u;
 #pragma unroll
-    for (int j = 0; j < kSegments; ++j) reached += uint32_t(__popcll(__ballot(key[j] >= (t | bit))));
+    for (int j = 0; j < MOST; ++j) reached += uint32_t(__popcll(__ballot(key[j] >= (t | bit))));
     if (reached >= share) t |= bit;
   }
   return whole_key<T>(t);
@@ -394,7 +394,7 @@ __device__ inline uint32_t key_of_threads(const uint32_t *thread_key, uint32_t k
 // times as quick for rows in falling order.  [512, 131072] f32 47 us of random values, 111 of zeros, 79 in rising order;
 // bf16 29, 75 and 46.
 template <typename T, int THREADS, int SHORT, bool NORM>
-__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS == 128 && sizeof(T) == 4 ? 5 : 4))) void top_k_kernel(
+__global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS <= 128 && sizeof(T) == 4 ? 5 : 4))) void top_k_kernel(
     uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc, double inv_t, Cut cut, const T *__restrict__ x,
     float *__restrict__ value, uint32_t *__restrict__ index, float *__restrict__ log_norm, PartResults pr) {
   constexpr int W = Group<T>::W;
@@ -484,7 +484,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
       low = key_of_threads<T, THREADS>(thread_key, k);
     } else {
       const uint32_t t = share <= uint32_t(kWave / 2) ? key_reached_by<T>(key_of(top), share)
-                                                      : key_of_segments<T, THREADS>(segment, segments, share);
+                                                      : key_of_segments<T, THREADS, THREADS == 64 ? U : kSegments>(segment, segments, share);
       if ((threadIdx.x & (kWave - 1)) == 0) wave_key[wave] = t;
       __syncthreads();
       low = wave_key[0];
@@ -629,7 +629,10 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
 // Threads of a workgroup: two waves for short rows, 8192 of 16000 bf16 64 against 97 us with four; four for long ones, 333 of
 // 50257 halves 18.6 against 27 with two.  k > 256 takes four and more room in LDS.
 constexpr uint32_t kFew = 256;
-uint32_t threads_for(uint32_t n, uint32_t k) { return n <= 16384u && k <= kFew ? 128u : 256u; }
+uint32_t threads_for(uint32_t n, uint32_t k, uint32_t size) {
+  if (k <= 64u && uint64_t(n) * size <= 4096u) return 64u;
+  return n <= 16384u && k <= kFew ? 128u : 256u;
+}
 
 // Arrays from this size on, which memory and not the last cache delivers, are read with a thread's four groups side by side: the
 // segments read again lie in a quarter of the lines (86 MB of [2048, 131072] bf16, 103 against 99 us; [512, 131072] f32
@@ -697,7 +700,9 @@ int top_k(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, uin
     auto *launch = &launch_top_k<T, 256, int(kFew) * 2, NORM>;
     if (k > kFew) {
       launch = &launch_top_k<T, 256, int(kMaxSlots) * 2, NORM>;
-    } else if (threads_for(dim0, k) == 128u) {
+    } else if (threads_for(dim0, k, uint32_t(sizeof(T))) == 64u) {
+      launch = &launch_top_k<T, 64, int(kFew) * 2, NORM>;
+    } else if (threads_for(dim0, k, uint32_t(sizeof(T))) == 128u) {
       launch = &launch_top_k<T, 128, int(kFew) * 2, NORM>;
     }
     return launch(symbol, dim0, dim1, pitch, k, temperature, x, value, index, log_norm, st);
@@ -709,7 +714,7 @@ int top_k(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, uin
 
 size_t top_k_scratch(uint32_t classes, uint32_t rows, uint32_t k) {
   if (rows == 0u || k > kMaxSlots) return 0u;
-  const Cut cut = cut_row(classes, rows, k, threads_for(classes, k), 1u);
+  const Cut cut = cut_row(classes, rows, k, threads_for(classes, k, 1u), 1u);
   if (cut.parts == 1u) return 0u;
   const PartBytes b = part_bytes(rows, cut);
   return b.entries + b.stats + b.counts;
