@@ -484,7 +484,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
       low = key_of_threads<T, THREADS>(thread_key, k);
     } else {
       const uint32_t t = share <= uint32_t(kWave / 2) ? key_reached_by<T>(key_of(top), share)
-                                                      : key_of_segments<T, THREADS, THREADS == 64 ? U : kSegments>(segment, segments, share);
+                                                      : key_of_segments<T, THREADS, THREADS == 64 ? 2 * U : kSegments>(segment, segments, share);
       if ((threadIdx.x & (kWave - 1)) == 0) wave_key[wave] = t;
       __syncthreads();
       low = wave_key[0];
@@ -626,11 +626,13 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
   }
 }
 
-// Threads of a workgroup: two waves for short rows, 8192 of 16000 bf16 64 against 97 us with four; four for long ones, 333 of
-// 50257 halves 18.6 against 27 with two.  k > 256 takes four and more room in LDS.
+// Threads of a workgroup: one wave for rows of up to 8 KB (16 where its lanes' largest values give the threshold, k <= 32), 65536
+// rows of 1000 bf16, k = 10, 97 us, with two 166; 16384 of 16000 bytes, k = 50, 70 against 64, k = 10 of 8192 32 against 35.
+// Two waves for short rows, 8192 of 16000 bf16 64 against 97 us with four; four for long ones, 333 of 50257 halves 18.6
+// against 27 with two.  k > 256 takes four and more room in LDS.
 constexpr uint32_t kFew = 256;
 uint32_t threads_for(uint32_t n, uint32_t k, uint32_t size) {
-  if (k <= 64u && uint64_t(n) * size <= 4096u) return 64u;
+  if (k <= uint32_t(kWave) && uint64_t(n) * size <= (k <= uint32_t(kWave / 2) ? 16384u : 8192u)) return 64u;
   return n <= 16384u && k <= kFew ? 128u : 256u;
 }
 
@@ -714,10 +716,13 @@ int top_k(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, uin
 
 size_t top_k_scratch(uint32_t classes, uint32_t rows, uint32_t k) {
   if (rows == 0u || k > kMaxSlots) return 0u;
-  const Cut cut = cut_row(classes, rows, k, threads_for(classes, k, 1u), 1u);
-  if (cut.parts == 1u) return 0u;
-  const PartBytes b = part_bytes(rows, cut);
-  return b.entries + b.stats + b.counts;
+  size_t most = 0u;
+  for (uint32_t size : {2u, 4u}) {
+    const Cut cut = cut_row(classes, rows, k, threads_for(classes, k, size), size);
+    const PartBytes b = part_bytes(rows, cut);
+    if (cut.parts > 1u && b.entries + b.stats + b.counts > most) most = b.entries + b.stats + b.counts;
+  }
+  return most;
 }
 }  // namespace anode
 

@@ -171,6 +171,20 @@ def test_top_k_masks(kind):
 
 
 @pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("row", [4096, 8192, 16384, 32768, 65536])
+@pytest.mark.parametrize("k", [32, 33, 64, 65, 256, 257])
+def test_top_k_rows_at_the_borders(kind, row, k):
+    # where the number of threads and of groups in a segment changes
+    g = np.random.default_rng(row + k)
+    for n in (row // TYPES[kind].itemsize + more for more in (-1, 0, 1)):
+        x = logits(g, 4, n, kind)
+        x[1] = np.sort(x[1])
+        x[2, g.random(n) < 0.9] = -np.inf
+        x[3] = 0.5
+        check_top_k(kind, x, k, 1.0, n + 1, 1, what=f"border {n}")
+
+
+@pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("k", [1, 64, 200, 1000])
 def test_top_k_of_large_arrays(kind, k):
     # more than the last cache holds: 800 rows (400 of floats) of an odd length, and rows in order, of ties and of masks
