@@ -646,11 +646,13 @@ constexpr size_t kWaveRow = 16384;
 // bytes 17.4 against 16.7.  (The fused call holds two groups a thread up to half of it: 118 against 144 us.)
 constexpr size_t kShortRow = 4096;
 
-// Bytes of a row that the workgroups of the fused call hold in registers: those of a wave, and of the three smaller of
-// distill_held_kernel.  At each border the smaller one is the quicker: 94.8 against 182 us (32768 rows of 4 KB), 66.5
-// against 143 (8192 of 18 KB), 62 against 66 (2048 of 70 KB), 58.6 against 67.9 (1024 of 140 KB).
+// Bytes of a row that the workgroups of the fused call hold in registers: those of a wave, and of five of distill_held_kernel; a
+// sixth, the widest, takes the rest.  At each border the smaller one is the quicker, with rows of bf16: 77 against 182 us
+// (32768 rows of 4 KB), 82 against 86 (16384 of 12 KB), 57 against 143 (8192 of 18 KB), 62 against 74 (4096 of 40 KB),
+// 58 against 66 (2048 of 70 KB), 59 against 68 (1024 of 140 KB).
 constexpr size_t kHeldByWave = size_t(kWave) * 4u * 16u;
-constexpr size_t kHeldBySmall = 192u * 6u * 16u, kHeldByMiddle = 448u * 10u * 16u, kHeldByLarge = 448u * 20u * 16u;
+constexpr size_t kHeldBy64 = 64u * 12u * 16u, kHeldBy192 = 192u * 6u * 16u;
+constexpr size_t kHeldBy448[3] = {448u * 6u * 16u, 448u * 10u * 16u, 448u * 20u * 16u};
 
 // Few rows that only the widest workgroup would hold go in parts, each read a second time for the gradient: 14.8 against 18.7
 // us for 24 rows of 131072 bf16 logits.  At 64 rows the two are even, and shorter rows are quicker on one CU each (16
@@ -760,11 +762,15 @@ void launch_fused(const Shape &s, const T *x, const Teacher &t, const float *dy,
     go(distill_wave_kernel<T, 2, NT>, kWave);
   } else if (row <= kHeldByWave) {
     go(distill_wave_kernel<T, 4, NT>, kWave);
-  } else if (row <= kHeldBySmall) {
+  } else if (row <= kHeldBy64) {
+    go(distill_held_kernel<T, 64, 12, NT>, 128u);
+  } else if (row <= kHeldBy192) {
     go(distill_held_kernel<T, 192, 6, NT>, 256u);
-  } else if (row <= kHeldByMiddle) {
+  } else if (row <= kHeldBy448[0]) {
+    go(distill_held_kernel<T, 448, 6, NT>, 512u);
+  } else if (row <= kHeldBy448[1]) {
     go(distill_held_kernel<T, 448, 10, NT>, 512u);
-  } else if (row <= kHeldByLarge) {
+  } else if (row <= kHeldBy448[2]) {
     go(distill_held_kernel<T, 448, 20, NT>, 512u);
   } else {
     go(distill_held_kernel<T, 960, 18, NT>, 1024u);
@@ -787,7 +793,7 @@ int distill_fused(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t str
   }
   const Parts ps = cut_rows<T>(s);
   // (not where dx is x: a part would overwrite logits that the other parts' workgroups still gather)
-  if (s.rows <= kFewRows && size_t(s.n) * sizeof(T) > kHeldByLarge && ps.parts > 1u && x != dx) {
+  if (s.rows <= kFewRows && size_t(s.n) * sizeof(T) > kHeldBy448[2] && ps.parts > 1u && x != dx) {
     const hipStream_t st = as_stream(stream);
     const RowsScratch scratch = rows_scratch(st, partial_bytes(s.rows, ps), symbol);
     if (scratch.error != 0) return scratch.error;

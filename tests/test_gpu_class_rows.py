@@ -402,7 +402,7 @@ def test_distill_accumulates_onto_the_logits_themselves(kind):
 
 
 # rows that fill the registers they are held in to the last value, and one value more; and the next workgroup's
-HELD = [4096, 18432, 71680, 143360, 276480]
+HELD = [2048, 4096, 12288, 18432, 43008, 71680, 143360, 276480]
 
 
 @pytest.mark.parametrize("kind", TYPES)
