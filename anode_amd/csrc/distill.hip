@@ -32,22 +32,23 @@ struct TeacherRow {
 // The slots of a row in LDS.  A streaming thread finds those that lie in its groups by a list of its own, and the turns of its
 // that have one by a bit mask, so that it takes their part off the values while it still has them in registers.
 struct Slots {
+  double *sum;      // [k]: where a class is named twice, the probabilities of a leader and of the slots that follow it
   float *p;         // [k]: the probability
   float *x;         // [k]: the student's logit
   float *off;       // [k]: what is taken off the gradient of its class
   uint32_t *index;  // [k]: the class; kNoClass for a slot that does not count
-  uint32_t *next;   // [k]: the next slot of the same thread, or kNoClass
+  uint32_t *next;   // [k]: a slot's leader; then the next slot of the same thread, or kNoClass
   uint32_t *head;   // [threads]: a thread's first slot, or kNoClass
   uint32_t *turns;  // [threads]: bit i for a slot in the thread's groups of turn i, i + 32, ...
   volatile uint16_t *seen;  // [kSeen]: slots' numbers, at the places that their classes give
 };
 constexpr uint32_t kSeen = 2048;  // (the leading 11 bits of a product)
-__device__ inline Slots slots_in(uint32_t *lds, uint32_t k, uint32_t threads) {
-  float *f = reinterpret_cast<float *>(lds);
-  uint32_t *t = lds + 5u * k;
-  return Slots{f, f + k, f + 2u * k, lds + 3u * k, lds + 4u * k, t, t + threads, reinterpret_cast<volatile uint16_t *>(t + 2u * threads)};
+__device__ inline Slots slots_in(double *lds, uint32_t k, uint32_t threads) {
+  float *f = reinterpret_cast<float *>(lds + k);
+  uint32_t *u = reinterpret_cast<uint32_t *>(f + 3u * k), *t = u + 2u * k;
+  return Slots{lds, f, f + k, f + 2u * k, u, u + k, t, t + threads, reinterpret_cast<volatile uint16_t *>(t + 2u * threads)};
 }
-uint32_t slot_bytes(uint32_t k, uint32_t threads) { return 20u * k + 8u * threads + 2u * kSeen; }
+uint32_t slot_bytes(uint32_t k, uint32_t threads) { return 28u * k + 8u * threads + 2u * kSeen; }
 
 // Reads the slots of a row, by one whole wave: x is the row, n its length.  LOSS: the student's logits too, which the loss asks for
 // and the gradient does not.
@@ -86,37 +87,54 @@ __device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x
   return r;
 }
 
-// Whether a class is named twice, by the wave that read the slots: every slot leaves its number at a place of a table that the class
-// gives, and looks whose number is there.  Another one's of the same class: twice.  Another class's: once more, at
-// another place (the slot whose number stands is done each time, so this ends).  What the table held before does not matter.
-__device__ inline bool repeated_slots(uint32_t k, const Slots &s) {
+// Finds the leader of every slot that counts, one slot of those that name its class, by the wave that read them, and tells whether
+// there is one with followers.  A slot leaves its number at a place of a table that its class gives, and looks whose number
+// is there: its leader's, if that names its class.  If not, once more at another place (the slots whose number stands
+// are done each time, so this ends).  What the table held before does not matter.
+__device__ inline bool find_leaders(uint32_t k, const Slots &s) {
   const uint32_t lane = threadIdx.x & (kWave - 1);
-  uint32_t open = 0u;  // bit i: slot lane + 64 i has not found its place
+  bool repeated = false;
+  uint32_t open = 0u;  // bit i: slot lane + 64 i has no leader yet
   for (uint32_t j = lane, bit = 1u; j < k; j += kWave, bit <<= 1) open |= s.index[j] != kNoClass ? bit : 0u;
-  for (uint32_t factor = 2654435761u;; factor = factor * 0x9e3779b1u + 0x7f4a7c16u | 1u) {
+  for (uint32_t factor = 2654435761u; __any(open != 0u); factor = (factor * 0x9e3779b1u + 0x7f4a7c16u) | 1u) {
     for (uint32_t j = lane, bit = 1u; j < k; j += kWave, bit <<= 1) {
       if ((open & bit) != 0u) s.seen[(s.index[j] * factor) >> 21] = uint16_t(j);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    bool twice = false;
     for (uint32_t j = lane, bit = 1u; j < k; j += kWave, bit <<= 1) {
       if ((open & bit) == 0u) continue;
       const uint32_t mine = s.index[j], there = s.seen[(mine * factor) >> 21];
-      if (there == j) {
+      if (s.index[there] == mine) {
         open &= ~bit;
-      } else {
-        twice |= s.index[there] == mine;
+        s.next[j] = there;
+        repeated |= there != j;
       }
     }
-    if (__any(twice)) return true;
-    if (!__any(open != 0u)) return false;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
+  return __any(repeated);
+}
+
+// The probabilities of a class that is named more than once, at its leader; added one follower after the other, in slot order.
+__device__ inline void add_followers(uint32_t k, const Slots &s) {
+  const uint32_t lane = threadIdx.x & (kWave - 1);
+  for (uint32_t j = lane; j < k; j += kWave) s.sum[j] = double(s.p[j]);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  for (uint32_t base = 0; base < k; base += kWave) {
+    const uint32_t j = base + lane;
+    const bool counts = j < k && s.index[min(j, k - 1u)] != kNoClass;
+    const uint32_t leader = counts ? s.next[j] : j;
+    for (uint64_t rest = __ballot(leader != j); rest != 0u; rest &= rest - 1u) {
+      const int at = __ffsll((unsigned long long)rest) - 1;
+      const uint32_t to = from_lane(leader, at);
+      if (lane == 0u) s.sum[to] += double(s.p[base + uint32_t(at)]);
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 // Deals the slots that lie in [from, from + n of the span) of the row to the streaming threads, w times their
-// probability each; by the wave that read them.  A class that is named more than once gets all of its mass from the first
-// slot that names it, added in slot order.
+// probability each; by the wave that read them.  A class that is named more than once gets all of its mass from one slot.
 template <typename T, int THREADS>
 __device__ inline void deal_slots(uint32_t k, bool any, const RowSpan<T> &span, uint32_t from, double w, const Slots &s) {
   const uint32_t lane = threadIdx.x & (kWave - 1);
@@ -126,21 +144,13 @@ __device__ inline void deal_slots(uint32_t k, bool any, const RowSpan<T> &span, 
     s.turns[i] = 0u;
   }
   if (!any) return;
-  const bool repeated = repeated_slots(k, s);
+  const bool repeated = find_leaders(k, s);
+  if (repeated) add_followers(k, s);
   for (uint32_t j = lane; j < k; j += kWave) {
     const uint32_t at = s.index[j] - from;
+    const bool mine = s.index[j] != kNoClass && at < end + span.tail && s.next[j] == j;  // (a class below `from` wraps)
     s.next[j] = kNoClass;
-    double p = double(s.p[j]);
-    bool mine = s.index[j] != kNoClass && at < end + span.tail;  // (a class below `from` wraps)
-    if (repeated && mine) {
-      p = 0.0;
-      for (uint32_t i = 0; i < k; ++i) {
-        if (s.index[i] != s.index[j]) continue;
-        if (i < j) mine = false;
-        p += double(s.p[i]);
-      }
-    }
-    s.off[j] = float(w * p);
+    s.off[j] = float(w * (repeated ? s.sum[j] : double(s.p[j])));
     if (!mine) continue;
     const bool single = at < span.head || at >= end;
     const uint32_t place = single ? (at < span.head ? at : at - end + span.head) : (at - span.head) / uint32_t(RowSpan<T>::W);
@@ -388,7 +398,7 @@ template <typename T, int THREADS, int U, bool ACC, bool JOIN, int NT>
 __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32_t rows, size_t stride, Scale sc, double inv_t,
                                                               Parts ps, const float *__restrict__ dy, const T *x, Teacher t,
                                                               Joined jn, T *dx) {
-  extern __shared__ uint32_t slot_lds[];
+  extern __shared__ double slot_lds[];
   __shared__ RowShared rs;
   __shared__ float plain_lds[THREADS / kWave];
   const Slots slots = slots_in(slot_lds, t.k, THREADS);
@@ -449,7 +459,7 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
   constexpr int WAVES = S / kWave;
   constexpr uint32_t kHeld = uint32_t(S) * uint32_t(G);
   static_assert(G % 2 == 0 && G <= 32, "two groups are folded together; a bit of Slots::turns for each");
-  extern __shared__ uint32_t slot_lds[];
+  extern __shared__ double slot_lds[];
   __shared__ SoftmaxSum parts[WAVES];
   __shared__ float plain_lds[WAVES + 1];
   __shared__ RowShared rs;
@@ -554,7 +564,7 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(4))) void
     uint32_t n, uint32_t rows, size_t stride, Scale sc, double inv_t, const T *x, Teacher t, const float *__restrict__ dy,
     float *__restrict__ loss, float *__restrict__ row_max, float *__restrict__ row_sum, T *dx) {
   constexpr int W = Group<T>::W;
-  extern __shared__ uint32_t slot_lds[];
+  extern __shared__ double slot_lds[];
   __shared__ SoftmaxSum lds[1];
   const Slots slots = slots_in(slot_lds, t.k, kWave);
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {

@@ -456,6 +456,26 @@ def test_distill(kind, n, rows, k):
 
 @pytest.mark.parametrize("kind", TYPES)
 @pytest.mark.parametrize("mode", ["fused", "apart", "accumulate"])
+@pytest.mark.parametrize("n,k", [(30, 64), (3, 200), (700, 333), (5000, 1024), (40000, 1024)])
+def test_distill_of_classes_named_many_times(kind, mode, n, k):
+    g = np.random.default_rng(n + k)
+    rows = 6
+    x = logits(g, rows, n, kind)
+    index = g.integers(0, n, (rows, k)).astype(np.uint32)      # drawn with replacement
+    index[1] = index[1, 0]                                     # one class in every slot
+    index[2] = g.integers(0, 2, k) * (n - 1)                   # the row's ends in turn
+    index[3, ::2] = index[3, 1]
+    index[4] = (np.arange(k) * 2048 % n).astype(np.uint32)     # classes that lie alike
+    value = (4.0 + 2.0 * g.standard_normal((rows, k))).astype(F32)
+    value[5, g.random(k) < 0.9] = -np.inf
+    norm = np.array([np.logaddexp.reduce(v.astype(np.float64)) + 0.1 for v in value], F32)
+    dy = g.standard_normal(rows).astype(F32)
+    check_distill(kind, x, value, index, 1.0, dy, None, mode, what="repeated")
+    check_distill(kind, x, value, index, 1.0, dy, norm, mode, n + 3, 1, what="repeated, norm")
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("mode", ["fused", "apart", "accumulate"])
 def test_distill_masks_and_special_values(kind, mode):
     g = np.random.default_rng(11)
     n, k = 5000, 6
