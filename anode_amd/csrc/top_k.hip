@@ -96,7 +96,7 @@ __device__ inline uint32_t reserve(uint32_t *counter, uint32_t own) {
 // What the exact selection of k entries needs in LDS.
 struct RadixLds {
   uint32_t digits[256];
-  uint32_t wave_count[16];
+  uint32_t wave_count[16];  // (two for each of eight waves)
   uint32_t found, above, taken;
 };
 
@@ -221,6 +221,8 @@ __device__ inline uint32_t radix_select(const T *xr, uint32_t n, uint32_t from, 
   return collect<T, THREADS>(xr, n, from, kth, k, entries, k, l);
 }
 
+constexpr uint32_t kCounted = 256;  // entries that are ranked by counting, at most
+
 // The entries in LDS that can be among the k largest, to `out` (room for `most`): those that reach a key which k of them
 // reach, and few more.  Returns their number, which may be above `most` (then `out` is incomplete).
 template <typename T, int THREADS>
@@ -247,6 +249,66 @@ __device__ inline uint32_t drop_small(const uint64_t *entries, uint32_t count, u
   return *taken;
 }
 
+// The same, of at most MOST entries, by the k-th largest key itself but for its low bits: no more than k and those that equal it.
+// A thread holds its share of the entries in registers; the key is found bit by bit, the waves' counts meet in LDS.
+template <typename T, int THREADS, int MOST>
+__device__ inline uint32_t drop_all_but(const uint64_t *entries, uint32_t count, uint32_t k, uint64_t *out, uint32_t most,
+                                      uint32_t *wave_count, uint32_t *taken) {
+  constexpr uint32_t WAVES = THREADS / kWave;
+  constexpr int EACH = MOST / THREADS;
+  static_assert(MOST % THREADS == 0, "a thread's share");
+  const uint32_t wave = threadIdx.x / kWave;
+  uint64_t own[EACH];
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    const uint32_t i = threadIdx.x + uint32_t(e * THREADS);
+    own[e] = i < count ? entries[i] : 0u;
+  }
+  if (threadIdx.x == 0) *taken = 0u;
+  uint32_t least = 0u, turn = 0u;
+#pragma unroll 1
+  for (uint32_t bit = 0x80000000u; bit >= LowestBit<T>::value; bit >>= 1) {
+    uint32_t reached = 0u;
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+      if (uint32_t(e * THREADS) < count) reached += uint32_t(__popcll(__ballot(key_in(own[e]) >= (least | bit))));
+    }
+    if constexpr (WAVES > 1) {
+      // (two halves in turn, so that one barrier a bit is enough)
+      if ((threadIdx.x & (kWave - 1)) == 0) wave_count[turn + wave] = reached;
+      __syncthreads();
+      reached = 0u;
+#pragma unroll
+      for (uint32_t w = 0; w < WAVES; ++w) reached += wave_count[turn + w];
+      turn ^= WAVES;
+    }
+    if (reached >= k) least |= bit;
+  }
+  least = whole_key<T>(least);
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < EACH; ++e) {
+    if (uint32_t(e * THREADS) >= count) break;
+    const bool in = key_in(own[e]) != 0u && key_in(own[e]) >= least;
+    const uint32_t at = reserve(taken, in ? 1u : 0u);
+    if (in && at < most) out[at] = own[e];
+  }
+  __syncthreads();
+  return *taken;
+}
+
+// Entries thinned until they fit in `out`, the quick way first: 8 rows of 1024 halves, of which 165 are kept, 22 against 37 us that
+// sorting all of them takes.  (Where the quick way is enough it is the quicker: 8192 rows of 16000 bf16, k = 200, 109
+// against 116 us.)
+template <typename T, int THREADS, int MOST>
+__device__ inline uint32_t thin_out(const uint64_t *entries, uint32_t count, uint32_t k, uint64_t *out, uint32_t most, uint32_t *waves,
+                                    uint32_t *taken) {
+  const uint32_t few = drop_small<T, THREADS>(entries, count, k, out, most, waves, taken);
+  if (few <= most) return few;
+  __syncthreads();
+  return drop_all_but<T, THREADS, MOST>(entries, count, k, out, most, waves, taken);
+}
+
 // The selection where the list was too short, out of line: inlined it costs the streaming loop registers (119 against 114 us).  With
 // the threshold that the whole row gives -- `top` is the thread's largest value -- it reads the row once more; that settles
 // rising rows, and ties at the threshold itself (zeros, a mask's lowest value), of which the first in order are
@@ -264,7 +326,7 @@ __device__ __attribute__((noinline)) uint32_t select_again(const T *xr, uint32_t
   uint32_t have = collect<T, THREADS>(xr, n, from, border, k, list, room, *l);
   __syncthreads();
   if (have != kNoClass) {
-    have = drop_small<T, THREADS>(list, have, k, best, most, l->wave_count, &l->taken);
+    have = thin_out<T, THREADS, kSegments * THREADS / 2>(list, have, k, best, most, l->wave_count, &l->taken);
     if (have <= most) return have;
   }
   __syncthreads();
@@ -273,7 +335,6 @@ __device__ __attribute__((noinline)) uint32_t select_again(const T *xr, uint32_t
   return have;
 }
 
-constexpr uint32_t kCounted = 256;
 // The result of a row from its entries in LDS, at least the k largest of them, and empty slots behind.  Up to 256 entries are
 // counted against each other, each by one to eight neighbouring threads; more are sorted (64 rows of which 200 of 131072
 // are kept: 32 us, 36 where up to 512 are counted).
@@ -541,7 +602,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
       have = select_again<T, THREADS>(xr, count, from, top, k, list, kList, best, kShort, &radix);
       found = best;
     } else if (have > kCounted) {
-      const uint32_t few = drop_small<T, THREADS>(list, have, k, best, kShort, wave_key, &taken);
+      const uint32_t few = thin_out<T, THREADS, int(kList)>(list, have, k, best, kShort, radix.wave_count, &taken);
       if (few <= kShort) {
         have = few;
         found = best;
@@ -583,7 +644,7 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
   __shared__ __align__(16) uint64_t list[kJoined];
   __shared__ __align__(16) uint64_t best[kShort];
   __shared__ uint32_t first[65];
-  __shared__ uint32_t wave_key[kBlock / kWave];
+  __shared__ uint32_t wave_count[2 * kBlock / kWave];
   __shared__ uint32_t taken;
   __shared__ float plain_lds[kBlock / kWave];
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -607,7 +668,7 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
       list[i] = pr.entries[(r * parts + part) * pr.quota + (i - first[part])];
     }
     __syncthreads();
-    const uint32_t few = drop_small<T, kBlock>(list, have, k, best, kShort, wave_key, &taken);
+    const uint32_t few = thin_out<T, kBlock, int(kJoined)>(list, have, k, best, kShort, wave_count, &taken);
     if (few <= kShort) {
       write_result<kBlock>(best, few, r, k, value, index);
     } else {
