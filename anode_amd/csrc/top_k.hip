@@ -250,9 +250,9 @@ __device__ inline uint32_t drop_small(const uint64_t *entries, uint32_t count, u
 }
 
 // The same, of at most MOST entries, by the k-th largest key itself but for its low bits: no more than k and those that equal it.
-// A thread holds its share of the entries in registers; the key is found bit by bit, the waves' counts meet in LDS.
+// A thread holds its share of the entries in registers; the key is found bit by bit, the waves' counts meet in LDS.  (Out of line: few rows need it.)
 template <typename T, int THREADS, int MOST>
-__device__ inline uint32_t drop_all_but(const uint64_t *entries, uint32_t count, uint32_t k, uint64_t *out, uint32_t most,
+__device__ __attribute__((noinline)) uint32_t drop_all_but(const uint64_t *entries, uint32_t count, uint32_t k, uint64_t *out, uint32_t most,
                                       uint32_t *wave_count, uint32_t *taken) {
   constexpr uint32_t WAVES = THREADS / kWave;
   constexpr int EACH = MOST / THREADS;
