@@ -455,7 +455,7 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32
 // their own: their 64-bit exponentials and logarithms would spill the held registers of a wave that streams, and take
 // about as long as a small row.  [4096, 131072] bf16 402 us, [2048, 32768] f32 101 us, 5.3 TB/s read and written: what bounds it is
 // that a CU loads its rows, then stores them.  The same accesses without any arithmetic take 387 us of the first, a flat copy 328;
-// reading each row twice 520.
+// two workgroups a CU that hold half of their rows and read the rest twice 475.
 template <typename T, int S, int G, int NT>
 __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) void distill_held_kernel(
     uint32_t n, uint32_t rows, size_t stride, Scale sc, double inv_t, const T *x, Teacher t, const float *__restrict__ dy,
@@ -564,7 +564,7 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
   }
 }
 
-// The same for short rows, one wave a row.  Bound by the VALU: 65536 rows of 1000 bf16 115 us, where a copy takes 40; some 700 of a
+// The same for short rows, one wave a row.  Bound by the VALU: 65536 rows of 1000 bf16 115 us, where a copy takes 40; most of a
 // wave's 850 instructions are the slots'.
 template <typename T, int G, int NT>
 __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(4))) void distill_wave_kernel(
