@@ -702,15 +702,18 @@ uint32_t threads_for(uint32_t n, uint32_t k, uint32_t size) {
 // 54.8 against 52.0), below it THREADS apart (512 rows of bf16 30.8 against 33.4).
 constexpr uint64_t kNearBytes = uint64_t(192) << 20;
 
-// Parts of at least 8192 values, no more than bring the launch to eight waves a CU, and with room for three times k entries
-// each among those that are joined (a part leaves little more than k).
+// Rows of up to 65536 classes are not cut: the second launch costs more than what it saves (8 rows of 32768 floats 7.1 against 10.0
+// us in four parts, 200 of 50257 bf16 11.1 against 16.9, 8 of 65536 bf16 10.8 against 12.2).  Longer ones are, into parts of
+// at least 32768 values, no more than bring the launch to eight waves a CU (16 of 131072 bf16 14.0 against 17.2 us in two
+// parts and 14.5 in sixteen, 64 of them 14.7 and 16.2 in eight), and with room for three times k entries each among those that
+// are joined (a part leaves little more than k).
 Cut cut_row(uint32_t n, uint32_t rows, uint32_t k, uint32_t threads, uint32_t size) {
   const bool near = uint64_t(n) * rows * size >= kNearBytes;
   uint64_t parts = uint64_t(device_cu_count()) * (512u / threads) / rows;
-  if (parts > n / 8192u) parts = n / 8192u;
+  if (parts > n / 32768u) parts = n / 32768u;
   if (parts > 64u) parts = 64u;
   if (k != 0u && parts > kJoined / (3u * k)) parts = kJoined / (3u * k);
-  if (parts <= 1u) return Cut{1u, n, near};
+  if (parts <= 1u || n <= 65536u) return Cut{1u, n, near};
   const uint64_t per = ((uint64_t(n) + parts - 1u) / parts + 1023u) / 1024u * 1024u;
   return Cut{uint32_t((n + per - 1u) / per), uint32_t(per), near};
 }
