@@ -14,10 +14,11 @@ namespace {
 constexpr int kDrawThreads = 256;
 constexpr uint32_t kDrawWaves = kDrawThreads / kWave;
 constexpr uint32_t kBlockGroups = 512;  // 16-byte groups (2048 classes) of a row that are summed together: eight a lane
-// Rows of up to 16 blocks (32768 classes) are drawn from in one launch, a workgroup a sequence; longer rows are spread over the
-// GPU first and drawn from by a second kernel.  Measured at 32768 classes 9.4 against 11.7 us for 200 sequences and
-// 8.1 against 10.0 for 16; at 131072 classes 18.5 against 10.2 us for 16 and 153 against 136 us for 1024.
-constexpr uint32_t kMostHeld = 16;
+// Rows of up to 32 blocks (65536 classes) are drawn from in one launch, a workgroup a sequence; longer rows are spread over the
+// GPU first and drawn from by a second kernel.  At 32768 classes 9.4 against 11.7 us for 200 sequences and 8.1 against
+// 10.0 for 16, at 50257 14.6 against 17.0 and 11.2 against 11.3 for 64, at 65536 13.2 against 15.6 and 12.2 against 11.8;
+// at 131072 18.5 against 10.2 us for 16 and 153 against 136 us for 1024.
+constexpr uint32_t kMostHeld = 32;
 
 struct Drafts {
   uint32_t n, drafted;       // classes; drafted tokens of a sequence at most
