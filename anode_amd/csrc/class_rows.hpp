@@ -149,6 +149,11 @@ __device__ inline void unpack(const u32x4 &q, float (&v)[8], const f16_t *) {
   }
 }
 
+// One value.  (Of a conversion from bfloat16 the compiler takes it that no signalling NaN comes out, but it is a shift.)
+__device__ inline float widened(float x) { return x; }
+__device__ inline float widened(f16_t x) { return float(x); }
+__device__ inline float widened(bf16_t x) { return __uint_as_float(uint32_t(__builtin_bit_cast(uint16_t, x)) << 16); }
+
 // Rounding to the element type: to nearest, ties to even (the conversions of gfx950).
 __device__ inline u32x4 pack(const float (&v)[4], const float *) {
   return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
@@ -237,17 +242,21 @@ struct SoftmaxSum {
   float m, s;
 };
 
-// The largest of m and the values, two values an instruction; a NaN is passed over.  (fmaxf() costs two more instructions a
-// value to quiet signalling NaNs, which the maximum ignores here either way.)
+// The larger of two, and the largest of m and the values, two values an instruction; NaN where one of them is a NaN, of either
+// kind.  (fmaxf() passes over a quiet NaN only: it quiets a signalling one by an instruction a value, and not at all one that was
+// widened from bfloat16.  Of a signalling NaN and a number the hardware's maximum makes a quiet NaN, which the next one passes
+// over, and the number is lost.)
+__device__ inline float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 template <int COUNT>
 __device__ inline float max_of(float m, const float (&v)[COUNT]) {
   static_assert(COUNT == 2 || COUNT % 4 == 0, "values are taken four at a time");
+  // (written out, the two of a step side by side: left to the compiler the held rows of distill.hip spill three registers more)
   if constexpr (COUNT == 2) {
-    asm("v_max3_f32 %0, %0, %1, %2" : "+v"(m) : "v"(v[0]), "v"(v[1]));
+    asm("v_maximum3_f32 %0, %0, %1, %2" : "+v"(m) : "v"(v[0]), "v"(v[1]));
   } else {
 #pragma unroll
     for (int j = 0; j < COUNT; j += 4) {
-      asm("v_max3_f32 %0, %0, %1, %2\n\tv_max3_f32 %0, %0, %3, %4" : "+v"(m) : "v"(v[j]), "v"(v[j + 1]), "v"(v[j + 2]), "v"(v[j + 3]));
+      asm("v_maximum3_f32 %0, %0, %1, %2\n\tv_maximum3_f32 %0, %0, %3, %4" : "+v"(m) : "v"(v[j]), "v"(v[j + 1]), "v"(v[j + 2]), "v"(v[j + 3]));
     }
   }
   return m;
@@ -255,7 +264,7 @@ __device__ inline float max_of(float m, const float (&v)[COUNT]) {
 
 // The fast form.
 template <int COUNT>
-__device__ inline void fold_below(SoftmaxSum &t, float m, const float (&v)[COUNT], float c) {  // m: the new reference, >= t.m and all values
+__device__ inline void fold_below(SoftmaxSum &t, float m, const float (&v)[COUNT], float c) {  // m: the new reference, >= t.m and all values, or a NaN
   const float shift = m * c;
   if (m > t.m) {
     t.s *= __builtin_amdgcn_exp2f(t.m * c - shift);
@@ -325,6 +334,8 @@ __device__ inline SoftmaxSum block_merge(SoftmaxSum t, float c, SoftmaxSum *lds)
 }
 // Whether the fast form holds for a row of this maximum.
 __device__ inline bool measured(float m, Scale sc) { return fabsf(m) < sc.limit; }
+// The same of both: a row with a NaN has a sum that is one, and its maximum may lack values that lay beside the NaN.
+__device__ inline bool measured(SoftmaxSum t, Scale sc) { return measured(t.m, sc) && t.s == t.s; }
 // The reference's rounding taken out: S about m itself.
 __device__ inline float true_sum(SoftmaxSum t, float c) { return t.s * __builtin_amdgcn_exp2f(fmaf(-t.m, c, t.m * c)); }
 
@@ -339,8 +350,9 @@ __device__ inline SoftmaxSum plain_stats(const T *row, uint32_t n, float c, floa
     float v = pass == 0 ? kMinusInf : 0.0f;
 #pragma unroll 1
     for (uint64_t i = threadIdx.x; i < n; i += THREADS) {
-      const float x = float(row[i]);
-      v = pass == 0 ? fmaxf(v, x) : v + __builtin_amdgcn_exp2f((x - about) * c);
+      const float x = widened(row[i]);
+      // (a comparison that no NaN passes, of either kind: not a maximum)
+      v = pass == 0 ? (x > v ? x : v) : v + __builtin_amdgcn_exp2f((x - about) * c);
     }
 #pragma unroll 1
     for (int off = kWave / 2; off > 0; off >>= 1) {
@@ -456,7 +468,7 @@ __device__ inline SoftmaxSum stream_stats(const RowSpan<T> &span, const T *row, 
 template <typename T, int THREADS>
 __device__ inline SoftmaxSum finish_stats(SoftmaxSum t, const T *row, uint32_t n, Scale sc, SoftmaxSum *lds) {
   t = block_merge<THREADS / kWave>(t, sc.c, lds);
-  if (measured(t.m, sc)) return SoftmaxSum{t.m, true_sum(t, sc.c)};
+  if (measured(t, sc)) return SoftmaxSum{t.m, true_sum(t, sc.c)};
   return plain_stats<T, THREADS>(row, n, sc.c, reinterpret_cast<float *>(lds));
 }
 

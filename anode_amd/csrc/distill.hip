@@ -288,7 +288,7 @@ __device__ inline SoftmaxSum join_parts(const SoftmaxSum *partial, uint32_t part
   SoftmaxSum st = {-sc.limit, 0.0f};
   for (uint32_t i = threadIdx.x & (kWave - 1); i < parts; i += kWave) st = merge(st, partial[i], sc.c);
   st = wave_merge(st, sc.c);
-  if (measured(st.m, sc)) return SoftmaxSum{st.m, true_sum(st, sc.c)};
+  if (measured(st, sc)) return SoftmaxSum{st.m, true_sum(st, sc.c)};
   return plain_stats<T, THREADS>(row, n, sc.c, lds);
 }
 
@@ -473,7 +473,7 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
   // the row's statistics, by every wave alike
   auto joined = [&](const T *xr) {
     const SoftmaxSum st = lane_merge<WAVES>(parts, sc.c);
-    if (measured(st.m, sc)) return SoftmaxSum{st.m, true_sum(st, sc.c)};
+    if (measured(st, sc)) return SoftmaxSum{st.m, true_sum(st, sc.c)};
     return plain_stats<T, THREADS>(xr, n, sc.c, plain_lds);
   };
   if (threadIdx.x >= uint32_t(S)) {

@@ -444,7 +444,8 @@ __device__ inline uint32_t key_of_threads(const uint32_t *thread_key, uint32_t k
 // 16-byte group each, or as many groups as that takes) in LDS.  A threshold that k of the threads' largest values reach (of long
 // rows; of short ones every wave finds what its share of k reaches, the least of the waves counts; for large k the
 // segments count, not the threads) names the few segments that can hold one of the k largest; these are read again,
-// and of their values those that reach the threshold are ranked and written.  Rows for which there are too many
+// and of their values those that reach the threshold are ranked and written.  (A segment with a NaN has one as its largest
+// value and is always read again; its thread counts for nothing in the threshold.)  Rows for which there are too many
 // (thousands of ties at the threshold, the largest values all in few segments) are selected from with further passes.
 //
 // Bound by reading: [2048, 131072] bf16 with the norm 95 us (5.6 TB/s) for k = 1, 99 us (5.4) for k = 64, 228 us for k = 1000,
@@ -517,12 +518,12 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
             for (int j = 0; j < W; ++j) w[j] = v[u * W + j];
             const float group_top = max_of(kMinusInf, w);
             if (base / uint32_t(THREADS) + uint32_t(u) < uint32_t(kSegments)) own[u * THREADS] = group_top;
-            tile_top = fmaxf(tile_top, group_top);
+            tile_top = larger(tile_top, group_top);
           }
           own += U * THREADS;
         } else {
           tile_top = max_of(kMinusInf, v);
-          segment_top = fmaxf(segment_top, tile_top);
+          segment_top = larger(segment_top, tile_top);
           if (--left == 0u || !more) {
             own[0] = segment_top;
             own += THREADS;
@@ -530,7 +531,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
             left = span_tiles;
           }
         }
-        top = fmaxf(top, tile_top);
+        top = larger(top, tile_top);
         if constexpr (NORM) fold_below(st, fmaxf(top, -sc.limit), v, sc.c);
         if (!more) break;
 #pragma unroll
@@ -555,7 +556,8 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
     const float least = low < kLowestKey ? -__FLT_MAX__ : value_of(low);
     uint32_t marked = 0u;
 #pragma unroll 4
-    for (uint32_t j = 0; j < segments; ++j) marked |= uint32_t(segment[j * uint32_t(THREADS) + threadIdx.x] >= least) << j;
+    for (uint32_t j = 0; j < segments; ++j) marked |= uint32_t(!(segment[j * uint32_t(THREADS) + threadIdx.x] < least)) << j;
+    if (k == 0u) marked = 0u;  // (the norm alone)
     uint32_t place = reserve(&named, uint32_t(__popc(marked)));
     for (; marked != 0u && place < kShort; marked &= marked - 1u) {
       names[place++] = (uint32_t(__ffs(int(marked))) - 1u) * uint32_t(THREADS) + threadIdx.x;
