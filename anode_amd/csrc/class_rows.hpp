@@ -339,42 +339,6 @@ __device__ inline bool measured(SoftmaxSum t, Scale sc) { return measured(t.m, s
 // The reference's rounding taken out: S about m itself.
 __device__ inline float true_sum(SoftmaxSum t, float c) { return t.s * __builtin_amdgcn_exp2f(fmaf(-t.m, c, t.m * c)); }
 
-// The plain form, for rows that the fast one does not measure: two passes, one value at a time.  -inf only (or
-// nothing): m = -inf, S = 0.  A NaN is ignored by m and makes S NaN; so does +inf.
-template <typename T, int THREADS>
-__device__ inline SoftmaxSum plain_stats(const T *row, uint32_t n, float c, float *lds) {
-  SoftmaxSum t = {kMinusInf, 0.0f};
-#pragma unroll 1
-  for (int pass = 0; pass < 2; ++pass) {
-    const float about = t.m == kMinusInf ? 0.0f : t.m;
-    float v = pass == 0 ? kMinusInf : 0.0f;
-#pragma unroll 1
-    for (uint64_t i = threadIdx.x; i < n; i += THREADS) {
-      const float x = widened(row[i]);
-      // (a comparison that no NaN passes, of either kind: not a maximum)
-      v = pass == 0 ? (x > v ? x : v) : v + __builtin_amdgcn_exp2f((x - about) * c);
-    }
-#pragma unroll 1
-    for (int off = kWave / 2; off > 0; off >>= 1) {
-      const float o = __shfl_xor(v, off, kWave);
-      v = pass == 0 ? fmaxf(v, o) : v + o;
-    }
-    __syncthreads();
-    if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
-    __syncthreads();
-    v = lds[0];
-#pragma unroll 1
-    for (int w = 1; w < THREADS / kWave; ++w) v = pass == 0 ? fmaxf(v, lds[w]) : v + lds[w];
-    if (pass == 0) {
-      t.m = v;
-    } else {
-      t.s = v;
-    }
-  }
-  __syncthreads();
-  return t;
-}
-
 // A row, or a part of one, as it is streamed: `head` single values, `groups` 16-byte groups, `tail` single values.  The
 // single values are taken one a thread.  head = 0 for kernels that only read (a 16-byte load may start at any
 // element); a kernel that stores takes as many as bring its groups to a 128-byte line of the output.
@@ -437,6 +401,69 @@ __device__ inline void mask_tile(const RowSpan<T> &span, uint32_t g, float fill,
   }
 }
 
+// The plain form, for rows that the fast one does not measure: two passes, U groups of a thread on their way together (the loss
+// of 512 rows of 131072 bf16 at the type's lowest value 64 us, 26 of random values; value by value, and with one wave for
+// rows in parts, it took 1205 and, of 4 rows, 562 instead of 12).  -inf only
+// (or nothing): m = -inf, S = 0.  A NaN is ignored by m and makes S NaN; so does +inf.  A thread adds its groups' sums in
+// 64 bits: a long row of a mask's lowest value is nothing but ones, of which 32 bits hold 2^24.
+template <typename T, int THREADS, int U>
+__device__ inline SoftmaxSum plain_stats(const T *row, uint32_t n, float c, float *lds) {
+  constexpr int N = U * Group<T>::W;
+  const RowSpan<T> span(n, 0u);
+  SoftmaxSum t = {kMinusInf, 0.0f};
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+    const float about = t.m == kMinusInf ? 0.0f : t.m;
+    float top = kMinusInf;
+    double sum = 0.0;
+    if (span.single(threadIdx.x)) {  // (the tail: fewer than a group)
+      const float x = widened(row[span.single_at(threadIdx.x)]);
+      if (pass == 0) {
+        top = x > top ? x : top;
+      } else {
+        sum = double(__builtin_amdgcn_exp2f((x - about) * c));
+      }
+    }
+#pragma unroll 1
+    for (uint32_t g = threadIdx.x; g < span.groups; g += uint32_t(THREADS) * uint32_t(U)) {
+      u32x4 q[U];
+      float v[N];
+      load_tile<T, THREADS, U>(span, row, g, q);
+      unpack_tile<T, U>(q, v);
+      if (U > 1) mask_tile<T, THREADS, U>(span, g, kMinusInf, v);
+      if (pass == 0) {
+        // (a comparison that no NaN passes, of either kind: not a maximum)
+#pragma unroll
+        for (int j = 0; j < N; ++j) top = v[j] > top ? v[j] : top;
+      } else {
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) s += __builtin_amdgcn_exp2f((v[j] - about) * c);
+        sum += double(s);
+      }
+    }
+    float v = pass == 0 ? top : float(sum);
+#pragma unroll 1
+    for (int off = kWave / 2; off > 0; off >>= 1) {
+      const float o = __shfl_xor(v, off, kWave);
+      v = pass == 0 ? fmaxf(v, o) : v + o;
+    }
+    __syncthreads();
+    if ((threadIdx.x & (kWave - 1)) == 0) lds[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = lds[0];
+#pragma unroll 1
+    for (int w = 1; w < THREADS / kWave; ++w) v = pass == 0 ? fmaxf(v, lds[w]) : v + lds[w];
+    if (pass == 0) {
+      t.m = v;
+    } else {
+      t.s = v;
+    }
+  }
+  __syncthreads();
+  return t;
+}
+
 // A thread's running reference and sum over its part of a row (merge them with block_merge): tiles of U groups a thread,
 // the next tile on its way while one is folded.
 template <typename T, int THREADS, int U>
@@ -464,12 +491,23 @@ __device__ inline SoftmaxSum stream_stats(const RowSpan<T> &span, const T *row, 
   return st;
 }
 
-// A row's statistics from its threads' parts, by the whole workgroup.
-template <typename T, int THREADS>
+// The statistics of a row, or of a part of one, from its threads' parts, by the whole workgroup.  NORM: for a row's log-sum-exp
+// alone, which is NaN whatever the maximum of a row with a NaN.
+template <typename T, int THREADS, bool NORM>
 __device__ inline SoftmaxSum finish_stats(SoftmaxSum t, const T *row, uint32_t n, Scale sc, SoftmaxSum *lds) {
   t = block_merge<THREADS / kWave>(t, sc.c, lds);
-  if (measured(t, sc)) return SoftmaxSum{t.m, true_sum(t, sc.c)};
-  return plain_stats<T, THREADS>(row, n, sc.c, reinterpret_cast<float *>(lds));
+  if (NORM ? measured(t.m, sc) : measured(t, sc)) return SoftmaxSum{t.m, true_sum(t, sc.c)};
+  return plain_stats<T, THREADS, (THREADS > kWave ? 2 : 1)>(row, n, sc.c, reinterpret_cast<float *>(lds));
+}
+
+// The statistics of the lanes' parts of a row together, the same in every lane; they are finished, whichever form they took, so
+// no row is read again to join them.  (m = -inf, S = 0 for a lane that has none.)
+__device__ inline SoftmaxSum join_lanes(SoftmaxSum t, float c) {
+  SoftmaxSum r = {lanes_max(t.m), 0.0f};
+  const float about = r.m == kMinusInf ? 0.0f : r.m;
+  r.s = lanes_upto(t.s * __builtin_amdgcn_exp2f((t.m - about) * c));
+  r.s = __shfl(r.s, kWave - 1, kWave);
+  return r;
 }
 
 #endif  // __HIPCC__

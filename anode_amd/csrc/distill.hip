@@ -254,7 +254,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(uint32_t n, uint32_t r
     LaneSlot slot = {};
     if (threadIdx.x < uint32_t(kWave)) slot = lane_slot(t, r, xr, n, threadIdx.x);
     const SoftmaxSum st =
-        finish_stats<T, THREADS>(stream_stats<T, THREADS, U>(RowSpan<T>(n, 0u), xr, sc), xr, n, sc, lds);
+        finish_stats<T, THREADS, false>(stream_stats<T, THREADS, U>(RowSpan<T>(n, 0u), xr, sc), xr, n, sc, lds);
     if (threadIdx.x < uint32_t(kWave)) {
       const float l = row_loss(t, r, xr, n, st, inv_t, slot);
       if (threadIdx.x == 0) {
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(THREADS) void distill_kernel(uint32_t n, uint32_t r
   }
 }
 
-// One workgroup a part of a row: its statistics, to partial[row * parts + part].  24 rows of 131072 bf16 are 384 parts, 3.9 us, and
+// One workgroup a part of a row: its statistics, finished, to partial[row * parts + part].  24 rows of 131072 bf16 are 384 parts, 3.9 us, and
 // 3.7 for the kernel that joins them: latency.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void part_stats_kernel(uint32_t n, uint32_t rows, size_t stride, Scale sc, Parts ps,
@@ -275,21 +275,24 @@ __global__ __launch_bounds__(kBlock) void part_stats_kernel(uint32_t n, uint32_t
   const uint64_t items = uint64_t(rows) * ps.parts;
   for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
     const uint32_t r = uint32_t(i / ps.parts), part = uint32_t(i % ps.parts);
-    const RowSpan<T> span(ps.count(part, n), 0u);
-    const SoftmaxSum st = block_merge<kBlock / kWave>(
-        stream_stats<T, kBlock, kUnroll>(span, x + size_t(r) * stride + ps.first(part), sc), sc.c, lds);
+    const T *xp = x + size_t(r) * stride + ps.first(part);
+    const uint32_t count = ps.count(part, n);
+    const SoftmaxSum st =
+        finish_stats<T, kBlock, false>(stream_stats<T, kBlock, kUnroll>(RowSpan<T>(count, 0u), xp, sc), xp, count, sc, lds);
     if (threadIdx.x == 0) partial[i] = st;
   }
 }
 
-// The parts of a row merged, by a whole workgroup whose waves all do the same.
-template <typename T, int THREADS>
-__device__ inline SoftmaxSum join_parts(const SoftmaxSum *partial, uint32_t parts, const T *row, uint32_t n, Scale sc, float *lds) {
-  SoftmaxSum st = {-sc.limit, 0.0f};
-  for (uint32_t i = threadIdx.x & (kWave - 1); i < parts; i += kWave) st = merge(st, partial[i], sc.c);
-  st = wave_merge(st, sc.c);
-  if (measured(st, sc)) return SoftmaxSum{st.m, true_sum(st, sc.c)};
-  return plain_stats<T, THREADS>(row, n, sc.c, lds);
+// The parts of a row joined, by every wave alike: a lane takes every 64th of them, the lanes then meet.
+__device__ inline SoftmaxSum join_parts(const SoftmaxSum *partial, uint32_t parts, Scale sc) {
+  SoftmaxSum st = {kMinusInf, 0.0f};
+  for (uint32_t i = threadIdx.x & (kWave - 1); i < parts; i += kWave) {
+    const SoftmaxSum p = partial[i];
+    const float m = fmaxf(st.m, p.m), about = m == kMinusInf ? 0.0f : m;
+    st.s = st.s * __builtin_amdgcn_exp2f((st.m - about) * sc.c) + p.s * __builtin_amdgcn_exp2f((p.m - about) * sc.c);
+    st.m = m;
+  }
+  return join_lanes(st, sc.c);
 }
 
 // One wave a row: the parts' statistics joined, and the loss.
@@ -298,10 +301,9 @@ __global__ __launch_bounds__(kWave) void distill_join_kernel(uint32_t n, uint32_
                                                              uint32_t parts, const T *__restrict__ x, Teacher t,
                                                              const SoftmaxSum *__restrict__ partial, float *__restrict__ loss,
                                                              float *__restrict__ row_max, float *__restrict__ row_sum) {
-  __shared__ float lds[1];
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const LaneSlot slot = lane_slot(t, r, x + r * stride, n, threadIdx.x);
-    const SoftmaxSum st = join_parts<T, kWave>(partial + r * parts, parts, x + r * stride, n, sc, lds);
+    const SoftmaxSum st = join_parts(partial + r * parts, parts, sc);
     const float l = row_loss(t, r, x + r * stride, n, st, inv_t, slot);
     if (threadIdx.x == 0) {
       loss[r] = l;
@@ -404,7 +406,6 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32
                                                               Joined jn, T *dx) {
   extern __shared__ double slot_lds[];
   __shared__ RowShared rs;
-  __shared__ float plain_lds[THREADS / kWave];
   const Slots slots = slots_in(slot_lds, t.k, THREADS);
   const uint64_t items = uint64_t(rows) * ps.parts;
   for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
@@ -418,7 +419,7 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32
     if (span.groups != 0u) load_tile<T, THREADS, U>(span, xr + from, threadIdx.x, q);
     SoftmaxSum st;
     if (JOIN) {
-      st = join_parts<T, THREADS>(jn.partial + r * ps.parts, ps.parts, xr, n, sc, plain_lds);
+      st = join_parts(jn.partial + r * ps.parts, ps.parts, sc);
     } else {
       st = SoftmaxSum{jn.row_max[r], jn.row_sum[r]};
     }
@@ -474,7 +475,7 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
   auto joined = [&](const T *xr) {
     const SoftmaxSum st = lane_merge<WAVES>(parts, sc.c);
     if (measured(st, sc)) return SoftmaxSum{st.m, true_sum(st, sc.c)};
-    return plain_stats<T, THREADS>(xr, n, sc.c, plain_lds);
+    return plain_stats<T, THREADS, 1>(xr, n, sc.c, plain_lds);
   };
   if (threadIdx.x >= uint32_t(S)) {
     for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
@@ -591,7 +592,7 @@ __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(4))) void
       mask_tile<T, kWave, G>(span, threadIdx.x, kMinusInf, v);
       fold(st, v, sc.c);
     }
-    st = finish_stats<T, kWave>(st, xr, n, sc, lds);
+    st = finish_stats<T, kWave, false>(st, xr, n, sc, lds);
     const float l = slots_loss(t, r, st, inv_t, tr, slots);
     if (threadIdx.x == 0) {
       loss[r] = l;

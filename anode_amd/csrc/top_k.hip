@@ -620,14 +620,14 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
     if (cut.parts == 1u) {
       write_result<THREADS>(found, have, r, k, value, index);
       if constexpr (NORM) {
-        st = finish_stats<T, THREADS>(st, xr, n, sc, sums);
+        st = finish_stats<T, THREADS, true>(st, xr, n, sc, sums);
         if (threadIdx.x == 0) log_norm[r] = float(double(st.m) * inv_t + log(double(st.s)));
       }
     } else {
       for (uint32_t i = threadIdx.x; i < have; i += THREADS) pr.entries[item * pr.quota + i] = found[i];
       if (threadIdx.x == 0) pr.count[item] = have;
       if constexpr (NORM) {
-        st = block_merge<WAVES>(st, sc.c, sums);
+        st = finish_stats<T, THREADS, true>(st, xr, count, sc, sums);
         if (threadIdx.x == 0) pr.stats[item] = st;
       }
     }
@@ -638,8 +638,7 @@ __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS
 // One workgroup a row: its parts' entries together, thinned, ranked and written.  Latency: 4 to 5 us for some hundred entries.
 constexpr uint32_t kJoined = 4096;  // entries of a row's parts at most
 template <typename T, bool NORM>
-__global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc,
-                                                            double inv_t, uint32_t parts, const T *__restrict__ x,
+__global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t rows, uint32_t k, Scale sc, double inv_t, uint32_t parts,
                                                             float *__restrict__ value, uint32_t *__restrict__ index,
                                                             float *__restrict__ log_norm, PartResults pr) {
   constexpr uint32_t kShort = 2048;
@@ -648,9 +647,8 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
   __shared__ uint32_t first[65];
   __shared__ uint32_t wave_count[2 * kBlock / kWave];
   __shared__ uint32_t taken;
-  __shared__ float plain_lds[kBlock / kWave];
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    SoftmaxSum st = {-sc.limit, 0.0f};
+    SoftmaxSum st = {kMinusInf, 0.0f};
     if constexpr (NORM) {
       const uint32_t lane = threadIdx.x & (kWave - 1);
       if (lane < parts) st = pr.stats[r * parts + lane];
@@ -677,12 +675,7 @@ __global__ __launch_bounds__(kBlock) void top_k_join_kernel(uint32_t n, uint32_t
       write_result<kBlock>(list, have, r, k, value, index);
     }
     if constexpr (NORM) {
-      st = wave_merge(st, sc.c);
-      if (measured(st.m, sc)) {
-        st.s = true_sum(st, sc.c);
-      } else {
-        st = plain_stats<T, kBlock>(x + r * stride, n, sc.c, plain_lds);
-      }
+      st = join_lanes(st, sc.c);
       if (threadIdx.x == 0) log_norm[r] = float(double(st.m) * inv_t + log(double(st.s)));
     }
     __syncthreads();
@@ -747,8 +740,7 @@ int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, u
     pr.stats = reinterpret_cast<SoftmaxSum *>(at + bytes.entries);
     pr.count = reinterpret_cast<uint32_t *>(at + bytes.entries + bytes.stats);
     top_k_kernel<T, THREADS, SHORT, NORM><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
-    top_k_join_kernel<T, NORM><<<rows < most ? rows : most, kBlock, 0, st>>>(n, rows, stride, k, sc, inv_t, cut.parts, x, value,
-                                                                           index, log_norm, pr);
+    top_k_join_kernel<T, NORM><<<rows < most ? rows : most, kBlock, 0, st>>>(rows, k, sc, inv_t, cut.parts, value, index, log_norm, pr);
   }
   note_launch(symbol);
   return 0;
