@@ -5,6 +5,7 @@
 #include "common.hpp"
 
 #include <cmath>
+#include <tuple>
 
 namespace anode {
 
@@ -64,6 +65,18 @@ static inline bool misaligned(const T *p) {
 }
 
 #if defined(__HIPCC__)
+
+// Launches a kernel and returns how that went, which <<< >>> does not tell.
+template <typename... P, typename... A>
+static inline hipError_t launch(void (*kernel)(P...), uint32_t grid, uint32_t threads, size_t lds, hipStream_t stream, A... args) {
+  std::tuple<P...> values(args...);  // of the kernel's own parameter types
+  return std::apply(
+      [&](P &...p) {
+        void *at[] = {const_cast<void *>(static_cast<const void *>(&p))...};
+        return hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3(grid), dim3(threads), at, lds, stream);
+      },
+      values);
+}
 
 constexpr float kMinusInf = -__builtin_huge_valf();
 

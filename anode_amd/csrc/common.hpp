@@ -302,6 +302,9 @@ uint32_t checked_len(uint64_t a, uint64_t b, uint64_t c, const char *symbol);
 // Looks at the thread's HIP error state after a launch (hipPeekAtLastError: the state is left to the caller) and,
 // when an error has appeared, records it for anode_gpu_take_last_error() and prints it to stderr.
 void note_launch(const char *symbol);
+// The same of a launch whose own result is known: `e` is recorded and printed if it is an error, and returned.  (The thread's error
+// state may hold an error from before, or the same one from an earlier launch, so it does not tell how this one went.)
+int note_launched(const char *symbol, hipError_t e);
 // Records `e` for anode_gpu_take_last_error() and prints "<symbol>: <what>: <error string>".
 void note_error(const char *symbol, hipError_t e, const char *what);
 

@@ -714,43 +714,35 @@ int distill(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, f
     const RowsScratch scratch = rows_scratch(st, partial_bytes(s.rows, ps), symbol);
     if (scratch.error != 0) return scratch.error;
     SoftmaxSum *partial = static_cast<SoftmaxSum *>(scratch.lease.ptr);
-    part_stats_kernel<T><<<grid_for(uint64_t(s.rows) * ps.parts), kBlock, 0, st>>>(s.n, s.rows, s.stride, s.sc, ps, x, partial);
-    distill_join_kernel<T><<<grid_for(s.rows), kWave, 0, st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, ps.parts, x, t, partial, loss,
-                                                             row_max, row_sum);
-  } else {
-    auto go = [&](auto kernel, uint32_t threads) {
-      kernel<<<grid_for(s.rows), threads, 0, st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, loss, row_max, row_sum);
-    };
-    const size_t row = size_t(s.n) * sizeof(T);
-    if (row <= kShortRow) {
-      go(distill_kernel<T, kWave, 2>, kWave);
-    } else if (row <= kWaveRow) {
-      go(distill_kernel<T, kWave, kUnroll>, kWave);
-    } else {
-      go(distill_kernel<T, kBlock, kUnroll>, kBlock);
-    }
+    const hipError_t e =
+        launch(&part_stats_kernel<T>, grid_for(uint64_t(s.rows) * ps.parts), kBlock, 0, st, s.n, s.rows, s.stride, s.sc, ps, x, partial);
+    if (e != hipSuccess) return note_launched(symbol, e);
+    return note_launched(symbol, launch(&distill_join_kernel<T>, grid_for(s.rows), kWave, 0, st, s.n, s.rows, s.stride, s.sc, s.inv_t,
+                                        ps.parts, x, t, partial, loss, row_max, row_sum));
   }
-  note_launch(symbol);
-  return 0;
+  auto go = [&](auto *kernel, uint32_t threads) {
+    return note_launched(symbol, launch(kernel, grid_for(s.rows), threads, 0, st, s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, loss, row_max,
+                                        row_sum));
+  };
+  const size_t row = size_t(s.n) * sizeof(T);
+  if (row <= kShortRow) return go(&distill_kernel<T, kWave, 2>, kWave);
+  if (row <= kWaveRow) return go(&distill_kernel<T, kWave, kUnroll>, kWave);
+  return go(&distill_kernel<T, kBlock, kUnroll>, kBlock);
 }
 
 template <typename T, bool ACC, int NT>
-void launch_bwd(const Shape &s, const float *dy, const T *x, const Teacher &t, const float *row_max, const float *row_sum, T *dx,
+hipError_t launch_bwd(const Shape &s, const float *dy, const T *x, const Teacher &t, const float *row_max, const float *row_sum, T *dx,
                 hipStream_t st) {
   const Parts ps = cut_rows<T>(s);
   const uint32_t grid = grid_for(uint64_t(s.rows) * ps.parts);
   const Joined jn = {nullptr, nullptr, const_cast<float *>(row_max), const_cast<float *>(row_sum)};  // (read only)
-  auto go = [&](auto kernel, uint32_t threads) {
-    kernel<<<grid, threads, slot_bytes(t.k, threads), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, ps, dy, x, t, jn, dx);
+  auto go = [&](auto *kernel, uint32_t threads) {
+    return launch(kernel, grid, threads, slot_bytes(t.k, threads), st, s.n, s.rows, s.stride, s.sc, s.inv_t, ps, dy, x, t, jn, dx);
   };
   const size_t row = size_t(s.n) * sizeof(T);
-  if (row <= kShortRow) {
-    go(distill_bwd_kernel<T, kWave, 2, ACC, false, NT>, kWave);
-  } else if (row <= kWaveRow && s.rows > kWanted) {
-    go(distill_bwd_kernel<T, kWave, kUnroll, ACC, false, NT>, kWave);
-  } else {
-    go(distill_bwd_kernel<T, kBlock, kUnroll, ACC, false, NT>, kBlock);
-  }
+  if (row <= kShortRow) return go(&distill_bwd_kernel<T, kWave, 2, ACC, false, NT>, kWave);
+  if (row <= kWaveRow && s.rows > kWanted) return go(&distill_bwd_kernel<T, kWave, kUnroll, ACC, false, NT>, kWave);
+  return go(&distill_bwd_kernel<T, kBlock, kUnroll, ACC, false, NT>, kBlock);
 }
 
 template <typename T, bool ACC>
@@ -762,41 +754,28 @@ int distill_bwd(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t strid
   if (const int e = check_arrays(symbol, s, x, t, {dy, row_max, row_sum, dx})) return e;
   if (misaligned(dx)) return refuse(symbol, "the gradient is not aligned to its type");
   if (tangled<T>(x, dx, s)) return refuse(symbol, "the gradient's rows lie across the logits'");
-  if (stream_policy(s.bytes(sizeof(T)), tuning().nontemporal) & kNtStore) {
-    launch_bwd<T, ACC, kNtStore>(s, dy, x, t, row_max, row_sum, dx, as_stream(stream));
-  } else {
-    launch_bwd<T, ACC, 0>(s, dy, x, t, row_max, row_sum, dx, as_stream(stream));
-  }
-  note_launch(symbol);
-  return 0;
+  const bool nt = (stream_policy(s.bytes(sizeof(T)), tuning().nontemporal) & kNtStore) != 0;
+  auto *go = nt ? &launch_bwd<T, ACC, kNtStore> : &launch_bwd<T, ACC, 0>;
+  return note_launched(symbol, go(s, dy, x, t, row_max, row_sum, dx, as_stream(stream)));
 }
 
 template <typename T, int NT>
-void launch_fused(const Shape &s, const T *x, const Teacher &t, const float *dy, float *loss, float *row_max, float *row_sum,
+hipError_t launch_fused(const Shape &s, const T *x, const Teacher &t, const float *dy, float *loss, float *row_max, float *row_sum,
                   T *dx, hipStream_t st) {
   const size_t row = size_t(s.n) * sizeof(T);
-  auto go = [&](auto kernel, uint32_t threads) {
+  auto go = [&](auto *kernel, uint32_t threads) {
     const uint32_t streaming = threads > uint32_t(kWave) ? threads - uint32_t(kWave) : threads;
-    kernel<<<grid_for(s.rows), threads, slot_bytes(t.k, streaming), st>>>(s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, dy, loss, row_max,
-                                                              row_sum, dx);
+    return launch(kernel, grid_for(s.rows), threads, slot_bytes(t.k, streaming), st, s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, dy, loss,
+                  row_max, row_sum, dx);
   };
-  if (row <= kHeldByWave / 2u) {
-    go(distill_wave_kernel<T, 2, NT>, kWave);
-  } else if (row <= kHeldByWave) {
-    go(distill_wave_kernel<T, 4, NT>, kWave);
-  } else if (row <= kHeldBy64) {
-    go(distill_held_kernel<T, 64, 12, NT>, 128u);
-  } else if (row <= kHeldBy192) {
-    go(distill_held_kernel<T, 192, 6, NT>, 256u);
-  } else if (row <= kHeldBy448[0]) {
-    go(distill_held_kernel<T, 448, 6, NT>, 512u);
-  } else if (row <= kHeldBy448[1]) {
-    go(distill_held_kernel<T, 448, 10, NT>, 512u);
-  } else if (row <= kHeldBy448[2]) {
-    go(distill_held_kernel<T, 448, 20, NT>, 512u);
-  } else {
-    go(distill_held_kernel<T, 960, 18, NT>, 1024u);
-  }
+  if (row <= kHeldByWave / 2u) return go(&distill_wave_kernel<T, 2, NT>, kWave);
+  if (row <= kHeldByWave) return go(&distill_wave_kernel<T, 4, NT>, kWave);
+  if (row <= kHeldBy64) return go(&distill_held_kernel<T, 64, 12, NT>, 128u);
+  if (row <= kHeldBy192) return go(&distill_held_kernel<T, 192, 6, NT>, 256u);
+  if (row <= kHeldBy448[0]) return go(&distill_held_kernel<T, 448, 6, NT>, 512u);
+  if (row <= kHeldBy448[1]) return go(&distill_held_kernel<T, 448, 10, NT>, 512u);
+  if (row <= kHeldBy448[2]) return go(&distill_held_kernel<T, 448, 20, NT>, 512u);
+  return go(&distill_held_kernel<T, 960, 18, NT>, 1024u);
 }
 
 template <typename T>
@@ -821,19 +800,14 @@ int distill_fused(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t str
     if (scratch.error != 0) return scratch.error;
     SoftmaxSum *partial = static_cast<SoftmaxSum *>(scratch.lease.ptr);
     const uint32_t grid = grid_for(uint64_t(s.rows) * ps.parts);
-    part_stats_kernel<T><<<grid, kBlock, 0, st>>>(s.n, s.rows, s.stride, s.sc, ps, x, partial);
-    distill_bwd_kernel<T, kBlock, kUnroll, false, true, 0><<<grid, kBlock, slot_bytes(t.k, kBlock), st>>>(
-        s.n, s.rows, s.stride, s.sc, s.inv_t, ps, dy, x, t, Joined{partial, loss, row_max, row_sum}, dx);
-    note_launch(symbol);
-    return 0;
+    const hipError_t e = launch(&part_stats_kernel<T>, grid, kBlock, 0, st, s.n, s.rows, s.stride, s.sc, ps, x, partial);
+    if (e != hipSuccess) return note_launched(symbol, e);
+    return note_launched(symbol, launch(&distill_bwd_kernel<T, kBlock, kUnroll, false, true, 0>, grid, kBlock, slot_bytes(t.k, kBlock), st,
+                                        s.n, s.rows, s.stride, s.sc, s.inv_t, ps, dy, x, t, Joined{partial, loss, row_max, row_sum}, dx));
   }
-  if (stream_policy(s.bytes(sizeof(T)), tuning().nontemporal) & kNtStore) {
-    launch_fused<T, kNtStore>(s, x, t, dy, loss, row_max, row_sum, dx, as_stream(stream));
-  } else {
-    launch_fused<T, 0>(s, x, t, dy, loss, row_max, row_sum, dx, as_stream(stream));
-  }
-  note_launch(symbol);
-  return 0;
+  const bool nt = (stream_policy(s.bytes(sizeof(T)), tuning().nontemporal) & kNtStore) != 0;
+  auto *go = nt ? &launch_fused<T, kNtStore> : &launch_fused<T, 0>;
+  return note_launched(symbol, go(s, x, t, dy, loss, row_max, row_sum, dx, as_stream(stream)));
 }
 
 }  // namespace

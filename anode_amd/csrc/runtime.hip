@@ -112,17 +112,29 @@ uint32_t checked_len(uint64_t a, uint64_t b, uint64_t c, const char *symbol) {
   return uint32_t(ab * c);
 }
 
+namespace {
+// The error that was pending at this thread's previous check: it is not reported again.
+thread_local hipError_t g_pending = hipSuccess;
+}  // namespace
+
 void note_launch(const char *symbol) {
   // Peek, never take: the thread's HIP error state belongs to the caller (the reference's kernels never touch
-  // the CUDA error state, so the host framework's own checks must keep seeing what they see today).  An error
-  // that was already pending at this thread's previous check is not reported again.
-  static thread_local hipError_t pending = hipSuccess;
+  // the CUDA error state, so the host framework's own checks must keep seeing what they see today).
   const hipError_t e = hipPeekAtLastError();
-  if (e != hipSuccess && e != pending) {
+  if (e != hipSuccess && e != g_pending) {
     g_last_error.store(int(e), std::memory_order_relaxed);
     std::fprintf(stderr, "%s: HIP error pending after the launch: %s\n", symbol, hipGetErrorString(e));
   }
-  pending = e;
+  g_pending = e;
+}
+
+int note_launched(const char *symbol, hipError_t e) {
+  if (e != hipSuccess) {
+    g_last_error.store(int(e), std::memory_order_relaxed);
+    std::fprintf(stderr, "%s: the launch failed: %s\n", symbol, hipGetErrorString(e));
+    g_pending = hipPeekAtLastError();
+  }
+  return int(e);
 }
 
 int recorded_error() { return g_last_error.load(std::memory_order_relaxed); }

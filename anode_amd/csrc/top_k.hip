@@ -729,21 +729,21 @@ int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, u
   const Scale sc = scale_for(temperature);
   const double inv_t = 1.0 / double(temperature);
   PartResults pr = {nullptr, nullptr, nullptr, kJoined / cut.parts};
+  auto *kernel = &top_k_kernel<T, THREADS, SHORT, NORM>;
   if (cut.parts == 1u) {
-    top_k_kernel<T, THREADS, SHORT, NORM><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
-  } else {
-    const PartBytes bytes = part_bytes(rows, cut);
-    const RowsScratch scratch = rows_scratch(st, bytes.entries + bytes.stats + bytes.counts, symbol);
-    if (scratch.error != 0) return scratch.error;
-    char *at = static_cast<char *>(scratch.lease.ptr);
-    pr.entries = reinterpret_cast<uint64_t *>(at);
-    pr.stats = reinterpret_cast<SoftmaxSum *>(at + bytes.entries);
-    pr.count = reinterpret_cast<uint32_t *>(at + bytes.entries + bytes.stats);
-    top_k_kernel<T, THREADS, SHORT, NORM><<<grid, THREADS, 0, st>>>(n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
-    top_k_join_kernel<T, NORM><<<rows < most ? rows : most, kBlock, 0, st>>>(rows, k, sc, inv_t, cut.parts, value, index, log_norm, pr);
+    return note_launched(symbol, launch(kernel, grid, THREADS, 0, st, n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr));
   }
-  note_launch(symbol);
-  return 0;
+  const PartBytes bytes = part_bytes(rows, cut);
+  const RowsScratch scratch = rows_scratch(st, bytes.entries + bytes.stats + bytes.counts, symbol);
+  if (scratch.error != 0) return scratch.error;
+  char *at = static_cast<char *>(scratch.lease.ptr);
+  pr.entries = reinterpret_cast<uint64_t *>(at);
+  pr.stats = reinterpret_cast<SoftmaxSum *>(at + bytes.entries);
+  pr.count = reinterpret_cast<uint32_t *>(at + bytes.entries + bytes.stats);
+  const hipError_t e = launch(kernel, grid, THREADS, 0, st, n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
+  if (e != hipSuccess) return note_launched(symbol, e);
+  return note_launched(symbol, launch(&top_k_join_kernel<T, NORM>, rows < most ? rows : most, kBlock, 0, st, rows, k, sc, inv_t, cut.parts,
+                                      value, index, log_norm, pr));
 }
 
 template <typename T>

@@ -320,11 +320,12 @@ ANODE_EXPORT int anode_gpu_verify_draft_packed_f32(uint32_t dim0, uint32_t dim1,
                                                    const float *accept, const float *pick, uint32_t *token, uint32_t *accepted,
                                                    const KernelConfig *, CUstream_st *stream) {
   using namespace anode;
+  const char *const symbol = __func__;
   if (dim2 == 0u) return 0;
-  if (dim0 != 0u && target == nullptr) return refuse(__func__, "the target's probabilities are missing");
-  if (dim1 != 0u && (draft_token == nullptr || accept == nullptr)) return refuse(__func__, "the drafted tokens are missing");
-  if (pick == nullptr || token == nullptr || accepted == nullptr) return refuse(__func__, "an array is missing");
-  if (dim1 >= kRefused) return refuse(__func__, "more drafted tokens than 2^31 - 1");
+  if (dim0 != 0u && target == nullptr) return refuse(symbol, "the target's probabilities are missing");
+  if (dim1 != 0u && (draft_token == nullptr || accept == nullptr)) return refuse(symbol, "the drafted tokens are missing");
+  if (pick == nullptr || token == nullptr || accepted == nullptr) return refuse(symbol, "an array is missing");
+  if (dim1 >= kRefused) return refuse(symbol, "more drafted tokens than 2^31 - 1");
   const hipStream_t st = as_stream(stream);
   const uint32_t blocks = blocks_of(dim0);
   const Drafts d = {dim0, dim1, target, draft, draft_token, draft_length, accept};
@@ -335,24 +336,20 @@ ANODE_EXPORT int anode_gpu_verify_draft_packed_f32(uint32_t dim0, uint32_t dim1,
   const uint32_t cus = uint32_t(device_cu_count());
   if (blocks <= kMostHeld) {
     // one launch, a workgroup a sequence, as wide as lets all of them run at once
-    auto go = [&](auto kernel, uint32_t threads) { kernel<<<grid, threads, 0, st>>>(d, dim2, blocks, pick, token, accepted); };
-    if (blocks <= 4u || dim2 > 2u * cus) {
-      nt ? go(verify_kernel<256, kNtLoad>, 256u) : go(verify_kernel<256, 0>, 256u);
-    } else if (dim2 > cus) {
-      nt ? go(verify_kernel<512, kNtLoad>, 512u) : go(verify_kernel<512, 0>, 512u);
-    } else {
-      nt ? go(verify_kernel<1024, kNtLoad>, 1024u) : go(verify_kernel<1024, 0>, 1024u);
-    }
-  } else {
-    const RowsScratch scratch = rows_scratch(st, verify_scratch(dim0, dim2), __func__);
-    if (scratch.error != 0) return scratch.error;
-    char *at = static_cast<char *>(scratch.lease.ptr);
-    const Sums sums = {reinterpret_cast<BlockSum *>(at), reinterpret_cast<uint32_t *>(at + size_t(dim2) * blocks * sizeof(BlockSum))};
-    const uint64_t items = (uint64_t(dim2) * blocks + kDrawWaves - 1u) / kDrawWaves;
-    auto go = [&](auto kernel) { kernel<<<uint32_t(items < most ? items : most), kDrawThreads, 0, st>>>(d, dim2, blocks, sums); };
-    nt ? go(draw_sums_kernel<kNtLoad>) : go(draw_sums_kernel<0>);
-    draw_kernel<<<grid, kWave, 0, st>>>(d, dim2, blocks, sums, pick, token, accepted);
+    auto go = [&](auto *kernel, uint32_t threads) {
+      return note_launched(symbol, launch(kernel, grid, threads, 0, st, d, dim2, blocks, pick, token, accepted));
+    };
+    if (blocks <= 4u || dim2 > 2u * cus) return nt ? go(&verify_kernel<256, kNtLoad>, 256u) : go(&verify_kernel<256, 0>, 256u);
+    if (dim2 > cus) return nt ? go(&verify_kernel<512, kNtLoad>, 512u) : go(&verify_kernel<512, 0>, 512u);
+    return nt ? go(&verify_kernel<1024, kNtLoad>, 1024u) : go(&verify_kernel<1024, 0>, 1024u);
   }
-  note_launch(__func__);
-  return 0;
+  const RowsScratch scratch = rows_scratch(st, verify_scratch(dim0, dim2), symbol);
+  if (scratch.error != 0) return scratch.error;
+  char *at = static_cast<char *>(scratch.lease.ptr);
+  const Sums sums = {reinterpret_cast<BlockSum *>(at), reinterpret_cast<uint32_t *>(at + size_t(dim2) * blocks * sizeof(BlockSum))};
+  const uint64_t items = (uint64_t(dim2) * blocks + kDrawWaves - 1u) / kDrawWaves;
+  const hipError_t e = launch(nt ? &draw_sums_kernel<kNtLoad> : &draw_sums_kernel<0>, uint32_t(items < most ? items : most), kDrawThreads,
+                              0, st, d, dim2, blocks, sums);
+  if (e != hipSuccess) return note_launched(symbol, e);
+  return note_launched(symbol, launch(&draw_kernel, grid, kWave, 0, st, d, dim2, blocks, sums, pick, token, accepted));
 }

@@ -289,7 +289,8 @@ void anode_gpu_softmax_nd_cat_nll_bwd_ignore_packed_accumulate_f32(uint32_t pref
  * These entry points check their arguments before they touch the device: they return 0, or an error code that is also
  * recorded for anode_gpu_take_last_error(), with the reason on stderr and nothing enqueued: hipErrorInvalidValue (1)
  * for stride < dim0 (unless 0), k > 1024, a temperature that is not positive and finite (or so small that its
- * reciprocal is not), missing arrays and logits that are not aligned to their type.  Few long rows are cut into parts,
+ * reciprocal is not), missing arrays and logits that are not aligned to their type.  A launch that fails gives its own
+ * code in the same way (no device, a stream that is none).  Few long rows are cut into parts,
  * whose results meet in the stream's scratch (below): a stream that is captured needs
  * anode_gpu_class_rows_scratch_bytes() of it reserved first, or the call returns hipErrorStreamCaptureUnsupported (900). ---- */
 
