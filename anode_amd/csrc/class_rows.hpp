@@ -23,9 +23,6 @@ static inline int refuse(const char *symbol, const char *what) {
   return int(hipErrorInvalidValue);
 }
 
-// The code of the error recorded last (runtime.hip).
-int recorded_error();
-
 // The stream's scratch (runtime.hip) for these entry points, which return an error code and let no exception out: ptr is
 // null when it cannot be had, and `error` then what the entry point returns.
 struct RowsScratch {
@@ -36,11 +33,11 @@ static inline RowsScratch rows_scratch(hipStream_t stream, size_t bytes, const c
   RowsScratch s = {ScratchLease{}, 0};
   try {
     s.lease = acquire_scratch(stream, bytes, symbol);
-    if (s.lease.ptr == nullptr) s.error = recorded_error();
+    s.error = s.lease.error;
   } catch (...) {
     note_error(symbol, hipErrorOutOfMemory, "cannot keep account of the scratch");
+    s.error = int(hipErrorOutOfMemory);
   }
-  if (s.lease.ptr == nullptr && s.error == 0) s.error = int(hipErrorOutOfMemory);
   return s;
 }
 // The scratch that each of them needs for [classes, rows] (distill.hip, top_k.hip, verify_draft.hip).

@@ -315,11 +315,12 @@ void note_error(const char *symbol, hipError_t e, const char *what);
 // interleave their launches; threads on other streams or devices are not held up.
 // When the buffer cannot be provided (allocation failure, or the stream is being
 // captured and would have to allocate) the error is recorded under `symbol`, ptr
-// is null and the lock is not held: the caller skips its launch.
+// is null, the lock is not held and `error` is this call's code: the caller skips its launch.
 struct ScratchLease {
   void *ptr;
   std::unique_lock<std::mutex> lock;
   std::shared_ptr<void> owner;  // keeps the cache entry (and with it the mutex) alive while the lease is
+  int error = 0;
 };
 ScratchLease acquire_scratch(hipStream_t stream, size_t bytes, const char *symbol);
 

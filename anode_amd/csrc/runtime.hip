@@ -137,8 +137,6 @@ int note_launched(const char *symbol, hipError_t e) {
   return int(e);
 }
 
-int recorded_error() { return g_last_error.load(std::memory_order_relaxed); }
-
 void note_error(const char *symbol, hipError_t e, const char *what) {
   g_last_error.store(int(e), std::memory_order_relaxed);
   std::fprintf(stderr, "%s: %s: %s; nothing was enqueued\n", symbol, what, hipGetErrorString(e));
@@ -331,6 +329,11 @@ ScratchLease acquire_scratch(hipStream_t stream, size_t bytes, const char *symbo
   }
   ScratchLease lease{nullptr, std::unique_lock<std::mutex>(entry->mu), entry};
   ScratchBuf &buf = *entry;
+  auto refuse = [&](hipError_t e, const char *what) {
+    note_error(symbol, e, what);
+    lease.error = int(e);
+    lease.lock.unlock();
+  };
   if (buf.cap < bytes) {
     // Growing means hipMalloc, which a stream under capture cannot take (it would fail and could invalidate the
     // capture): refuse instead, and tell the caller how to avoid it.  A query that itself fails (no device; the
@@ -339,15 +342,13 @@ ScratchLease acquire_scratch(hipStream_t stream, size_t bytes, const char *symbo
     hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
     const hipError_t q = hipStreamIsCapturing(stream, &capturing);
     if (q != hipSuccess) {
-      note_error(symbol, q, "cannot read the capture state of the stream, so the reduction scratch is not allocated");
-      lease.lock.unlock();
+      refuse(q, "cannot read the capture state of the stream, so the reduction scratch is not allocated");
       return lease;
     }
     if (capturing != hipStreamCaptureStatusNone) {
-      note_error(symbol, hipErrorStreamCaptureUnsupported,
-                 "the stream is being captured and has no reduction scratch yet (call anode_gpu_reserve_scratch "
-                 "or run the entry point once on this stream before capturing)");
-      lease.lock.unlock();
+      refuse(hipErrorStreamCaptureUnsupported,
+             "the stream is being captured and has no reduction scratch yet (call anode_gpu_reserve_scratch "
+             "or run the entry point once on this stream before capturing)");
       return lease;
     }
     // Grow geometrically.  The previous buffer may still be read by kernels in flight on this stream, so it is
@@ -358,8 +359,7 @@ ScratchLease acquire_scratch(hipStream_t stream, size_t bytes, const char *symbo
     void *p = nullptr;
     const hipError_t e = hipMalloc(&p, cap);
     if (e != hipSuccess || !p) {
-      note_error(symbol, e != hipSuccess ? e : hipErrorOutOfMemory, "cannot allocate the reduction scratch");
-      lease.lock.unlock();
+      refuse(e != hipSuccess ? e : hipErrorOutOfMemory, "cannot allocate the reduction scratch");
       return lease;
     }
     if (buf.ptr) buf.outgrown.push_back(buf.ptr);
@@ -397,8 +397,7 @@ ANODE_EXPORT size_t anode_gpu_reduce_scratch_bytes(uint32_t S, uint32_t C, uint3
 ANODE_EXPORT int anode_gpu_reserve_scratch(CUstream_st *stream, size_t bytes) {
   anode::ScratchLease lease = anode::acquire_scratch(anode::as_stream(stream), bytes, __func__);
   if (lease.ptr || bytes == 0) return 0;
-  const int e = anode::g_last_error.load(std::memory_order_relaxed);
-  return e ? e : int(hipErrorOutOfMemory);
+  return lease.error;
 }
 
 // Frees every scratch buffer held for `stream` on the current device.  The caller must have synchronised the

@@ -49,3 +49,32 @@ assert rc != 0 and rc == err, (rc, err)
 print("done")
 """)
     assert r.stderr.count("anode_gpu_softmax_distill_fused_fwd_bwd_rows_bf16") == 1, r.stderr
+
+
+def test_scratch_that_cannot_be_had_is_the_code_of_this_call():
+    # other threads' errors come and go in the process-wide record meanwhile: calls on shapes with scratch return their own
+    run_without_device("""
+import ctypes, threading
+from anode_amd import _lib
+lib = _lib.load()
+cfg = ctypes.byref(_lib.KernelConfig(1024, 1024))
+def call(**change):
+    values = dict({"dim0": 131072, "dim1": 2, "stride": 0, "k": 5, "temperature": 1.0}, **change)
+    return lib.symbol("anode_gpu_top_k_rows_f32")(*[values.get(n, t.P) for n in t.CALLS["top_k_rows"][1]], cfg, None)
+want = call()
+assert want not in (0, 1), want
+stop = threading.Event()
+def others():
+    while not stop.is_set():
+        call(k=2000)                                        # refused: another code
+        lib.symbol("anode_gpu_take_last_error")()           # and taken
+threads = [threading.Thread(target=others) for _ in range(3)]
+for thread in threads:
+    thread.start()
+got = {call() for _ in range(4000)} | {lib.symbol("anode_gpu_reserve_scratch")(None, 1 << 20) for _ in range(4000)}
+stop.set()
+for thread in threads:
+    thread.join()
+assert got == {want}, got
+print("done")
+""")
