@@ -63,9 +63,12 @@ static inline bool misaligned(const T *p) {
 
 #if defined(__HIPCC__)
 
-// Launches a kernel and returns how that went, which <<< >>> does not tell.
+// Launches a kernel with a workgroup an item, or as many as a launch takes, and returns how that went, which <<< >>> does not tell.
+// (HIP refuses 2^32 work-items and more: 2^24 workgroups of 256.  The kernels here take the further items in turn.)
 template <typename... P, typename... A>
-static inline hipError_t launch(void (*kernel)(P...), uint32_t grid, uint32_t threads, size_t lds, hipStream_t stream, A... args) {
+static inline hipError_t launch(void (*kernel)(P...), uint64_t items, uint32_t threads, size_t lds, hipStream_t stream, A... args) {
+  const uint64_t most = (uint64_t(1) << 31) / threads;
+  const uint32_t grid = uint32_t(items < most ? items : most);
   std::tuple<P...> values(args...);  // of the kernel's own parameter types
   return std::apply(
       [&](P &...p) {

@@ -677,8 +677,6 @@ constexpr size_t kHeldBy448[3] = {448u * 6u * 16u, 448u * 10u * 16u, 448u * 20u 
 // rows of 32768: 13.7 against 11.2 us).
 constexpr uint32_t kFewRows = 32;
 
-uint32_t grid_for(uint64_t items) { return items < (1u << 24) ? uint32_t(items) : (1u << 24); }
-
 // Parts of at least one tile of a workgroup (kBlock * kUnroll groups), no more than bring the launch to kWanted workgroups:
 // four a CU (1001 rows of 50257 halves: loss and gradient 58.6 us whole, 66.3 us in two and three parts).
 constexpr uint32_t kWanted = 1024;
@@ -715,13 +713,13 @@ int distill(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t stride, f
     if (scratch.error != 0) return scratch.error;
     SoftmaxSum *partial = static_cast<SoftmaxSum *>(scratch.lease.ptr);
     const hipError_t e =
-        launch(&part_stats_kernel<T>, grid_for(uint64_t(s.rows) * ps.parts), kBlock, 0, st, s.n, s.rows, s.stride, s.sc, ps, x, partial);
+        launch(&part_stats_kernel<T>, uint64_t(s.rows) * ps.parts, kBlock, 0, st, s.n, s.rows, s.stride, s.sc, ps, x, partial);
     if (e != hipSuccess) return note_launched(symbol, e);
-    return note_launched(symbol, launch(&distill_join_kernel<T>, grid_for(s.rows), kWave, 0, st, s.n, s.rows, s.stride, s.sc, s.inv_t,
+    return note_launched(symbol, launch(&distill_join_kernel<T>, s.rows, kWave, 0, st, s.n, s.rows, s.stride, s.sc, s.inv_t,
                                         ps.parts, x, t, partial, loss, row_max, row_sum));
   }
   auto go = [&](auto *kernel, uint32_t threads) {
-    return note_launched(symbol, launch(kernel, grid_for(s.rows), threads, 0, st, s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, loss, row_max,
+    return note_launched(symbol, launch(kernel, s.rows, threads, 0, st, s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, loss, row_max,
                                         row_sum));
   };
   const size_t row = size_t(s.n) * sizeof(T);
@@ -734,10 +732,10 @@ template <typename T, bool ACC, int NT>
 hipError_t launch_bwd(const Shape &s, const float *dy, const T *x, const Teacher &t, const float *row_max, const float *row_sum, T *dx,
                 hipStream_t st) {
   const Parts ps = cut_rows<T>(s);
-  const uint32_t grid = grid_for(uint64_t(s.rows) * ps.parts);
+  const uint64_t items = uint64_t(s.rows) * ps.parts;
   const Joined jn = {nullptr, nullptr, const_cast<float *>(row_max), const_cast<float *>(row_sum)};  // (read only)
   auto go = [&](auto *kernel, uint32_t threads) {
-    return launch(kernel, grid, threads, slot_bytes(t.k, threads), st, s.n, s.rows, s.stride, s.sc, s.inv_t, ps, dy, x, t, jn, dx);
+    return launch(kernel, items, threads, slot_bytes(t.k, threads), st, s.n, s.rows, s.stride, s.sc, s.inv_t, ps, dy, x, t, jn, dx);
   };
   const size_t row = size_t(s.n) * sizeof(T);
   if (row <= kShortRow) return go(&distill_bwd_kernel<T, kWave, 2, ACC, false, NT>, kWave);
@@ -765,7 +763,7 @@ hipError_t launch_fused(const Shape &s, const T *x, const Teacher &t, const floa
   const size_t row = size_t(s.n) * sizeof(T);
   auto go = [&](auto *kernel, uint32_t threads) {
     const uint32_t streaming = threads > uint32_t(kWave) ? threads - uint32_t(kWave) : threads;
-    return launch(kernel, grid_for(s.rows), threads, slot_bytes(t.k, streaming), st, s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, dy, loss,
+    return launch(kernel, s.rows, threads, slot_bytes(t.k, streaming), st, s.n, s.rows, s.stride, s.sc, s.inv_t, x, t, dy, loss,
                   row_max, row_sum, dx);
   };
   if (row <= kHeldByWave / 2u) return go(&distill_wave_kernel<T, 2, NT>, kWave);
@@ -799,10 +797,10 @@ int distill_fused(const char *symbol, uint32_t dim0, uint32_t dim1, uint32_t str
     const RowsScratch scratch = rows_scratch(st, partial_bytes(s.rows, ps), symbol);
     if (scratch.error != 0) return scratch.error;
     SoftmaxSum *partial = static_cast<SoftmaxSum *>(scratch.lease.ptr);
-    const uint32_t grid = grid_for(uint64_t(s.rows) * ps.parts);
-    const hipError_t e = launch(&part_stats_kernel<T>, grid, kBlock, 0, st, s.n, s.rows, s.stride, s.sc, ps, x, partial);
+    const uint64_t items = uint64_t(s.rows) * ps.parts;
+    const hipError_t e = launch(&part_stats_kernel<T>, items, kBlock, 0, st, s.n, s.rows, s.stride, s.sc, ps, x, partial);
     if (e != hipSuccess) return note_launched(symbol, e);
-    return note_launched(symbol, launch(&distill_bwd_kernel<T, kBlock, kUnroll, false, true, 0>, grid, kBlock, slot_bytes(t.k, kBlock), st,
+    return note_launched(symbol, launch(&distill_bwd_kernel<T, kBlock, kUnroll, false, true, 0>, items, kBlock, slot_bytes(t.k, kBlock), st,
                                         s.n, s.rows, s.stride, s.sc, s.inv_t, ps, dy, x, t, Joined{partial, loss, row_max, row_sum}, dx));
   }
   const bool nt = (stream_policy(s.bytes(sizeof(T)), tuning().nontemporal) & kNtStore) != 0;

@@ -725,13 +725,12 @@ int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, u
                  float *value, uint32_t *index, float *log_norm, hipStream_t st) {
   const Cut cut = cut_row(n, rows, k, THREADS, uint32_t(sizeof(T)));
   const uint64_t items = uint64_t(rows) * cut.parts;
-  const uint32_t most = 1u << 24, grid = items < most ? uint32_t(items) : most;
   const Scale sc = scale_for(temperature);
   const double inv_t = 1.0 / double(temperature);
   PartResults pr = {nullptr, nullptr, nullptr, kJoined / cut.parts};
   auto *kernel = &top_k_kernel<T, THREADS, SHORT, NORM>;
   if (cut.parts == 1u) {
-    return note_launched(symbol, launch(kernel, grid, THREADS, 0, st, n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr));
+    return note_launched(symbol, launch(kernel, items, THREADS, 0, st, n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr));
   }
   const PartBytes bytes = part_bytes(rows, cut);
   const RowsScratch scratch = rows_scratch(st, bytes.entries + bytes.stats + bytes.counts, symbol);
@@ -740,9 +739,9 @@ int launch_top_k(const char *symbol, uint32_t n, uint32_t rows, size_t stride, u
   pr.entries = reinterpret_cast<uint64_t *>(at);
   pr.stats = reinterpret_cast<SoftmaxSum *>(at + bytes.entries);
   pr.count = reinterpret_cast<uint32_t *>(at + bytes.entries + bytes.stats);
-  const hipError_t e = launch(kernel, grid, THREADS, 0, st, n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
+  const hipError_t e = launch(kernel, items, THREADS, 0, st, n, rows, stride, k, sc, inv_t, cut, x, value, index, log_norm, pr);
   if (e != hipSuccess) return note_launched(symbol, e);
-  return note_launched(symbol, launch(&top_k_join_kernel<T, NORM>, rows < most ? rows : most, kBlock, 0, st, rows, k, sc, inv_t, cut.parts,
+  return note_launched(symbol, launch(&top_k_join_kernel<T, NORM>, rows, kBlock, 0, st, rows, k, sc, inv_t, cut.parts,
                                       value, index, log_norm, pr));
 }
 

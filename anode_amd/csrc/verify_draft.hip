@@ -329,15 +329,13 @@ ANODE_EXPORT int anode_gpu_verify_draft_packed_f32(uint32_t dim0, uint32_t dim1,
   const hipStream_t st = as_stream(stream);
   const uint32_t blocks = blocks_of(dim0);
   const Drafts d = {dim0, dim1, target, draft, draft_token, draft_length, accept};
-  const uint64_t most = 1u << 24;
-  const uint32_t grid = dim2 < most ? dim2 : uint32_t(most);
   // a token's rows are read once, past the caches where they are large (the model's other rows are not read at all)
   const bool nt = (stream_policy(size_t(dim2) * dim0 * 2u * sizeof(float), tuning().reduce_nontemporal) & kNtLoad) != 0;
   const uint32_t cus = uint32_t(device_cu_count());
   if (blocks <= kMostHeld) {
     // one launch, a workgroup a sequence, as wide as lets all of them run at once
     auto go = [&](auto *kernel, uint32_t threads) {
-      return note_launched(symbol, launch(kernel, grid, threads, 0, st, d, dim2, blocks, pick, token, accepted));
+      return note_launched(symbol, launch(kernel, dim2, threads, 0, st, d, dim2, blocks, pick, token, accepted));
     };
     if (blocks <= 4u || dim2 > 2u * cus) return nt ? go(&verify_kernel<256, kNtLoad>, 256u) : go(&verify_kernel<256, 0>, 256u);
     if (dim2 > cus) return nt ? go(&verify_kernel<512, kNtLoad>, 512u) : go(&verify_kernel<512, 0>, 512u);
@@ -348,8 +346,8 @@ ANODE_EXPORT int anode_gpu_verify_draft_packed_f32(uint32_t dim0, uint32_t dim1,
   char *at = static_cast<char *>(scratch.lease.ptr);
   const Sums sums = {reinterpret_cast<BlockSum *>(at), reinterpret_cast<uint32_t *>(at + size_t(dim2) * blocks * sizeof(BlockSum))};
   const uint64_t items = (uint64_t(dim2) * blocks + kDrawWaves - 1u) / kDrawWaves;
-  const hipError_t e = launch(nt ? &draw_sums_kernel<kNtLoad> : &draw_sums_kernel<0>, uint32_t(items < most ? items : most), kDrawThreads,
-                              0, st, d, dim2, blocks, sums);
+  const hipError_t e = launch(nt ? &draw_sums_kernel<kNtLoad> : &draw_sums_kernel<0>, items, kDrawThreads, 0,
+                              st, d, dim2, blocks, sums);
   if (e != hipSuccess) return note_launched(symbol, e);
-  return note_launched(symbol, launch(&draw_kernel, grid, kWave, 0, st, d, dim2, blocks, sums, pick, token, accepted));
+  return note_launched(symbol, launch(&draw_kernel, dim2, kWave, 0, st, d, dim2, blocks, sums, pick, token, accepted));
 }
