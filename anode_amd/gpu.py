@@ -48,15 +48,18 @@ def call(name: str, *args, cfg: Optional[KernelConfig] = None, stream: Optional[
     fn, count = _entries.get(name) or _entry(name)
     if len(args) != count:
         raise TypeError(f"{name} takes {count} arguments before (cfg, stream): {load().prototypes[name][2][:-2]}")
-    device = torch.cuda.current_device()
+    device = None
     values = []
     for a in args:
         if isinstance(a, torch.Tensor):
+            if device is None and a.is_cuda:  # (a tensor that is not on a GPU is refused before a device is asked for)
+                device = torch.cuda.current_device()
             if a.get_device() != device or not a.is_contiguous():
                 _refuse(a, device)
             a = a.data_ptr()
         values.append(a)
     if stream is None:
+        device = torch.cuda.current_device() if device is None else device
         stream = torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device)
     return fn(*values, ctypes.byref(DEFAULT_CONFIG if cfg is None else cfg), stream)
 
