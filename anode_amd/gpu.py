@@ -19,11 +19,9 @@ from ._lib import KernelConfig, load
 DEFAULT_CONFIG = KernelConfig(1024, 1024)
 
 
-def _refuse(a: torch.Tensor, device: int):
+def _refuse(a: torch.Tensor):
     if not a.is_cuda:
         raise ValueError("the ABI takes device pointers: tensor is not on the GPU")
-    if a.get_device() != device:
-        raise ValueError(f"the ABI works on the current device ({device}): tensor is on device {a.get_device()}")
     raise ValueError("the ABI takes packed arrays: tensor is not contiguous")
 
 
@@ -42,9 +40,17 @@ def _entry(name: str):
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def _current_stream(device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device)
+
+
 def call(name: str, *args, cfg: Optional[KernelConfig] = None, stream: Optional[int] = None):
     """Invoke entry point `name`; `args` are everything before (cfg, stream).  Returns what the entry point returns:
-    None, or for those that can refuse their arguments 0 or an error code (nothing is enqueued then)."""
+    None, or for those that can refuse their arguments 0 or an error code (nothing is enqueued then).
+
+    Without a `stream` the call goes to the current stream of the device that its tensors are on, as torch's own operators
+    do; they have to be on one.  A `stream` is taken as it is, and so are the tensors: the caller answers for the device that
+    is current, and for what that device can reach."""
     fn, count = _entries.get(name) or _entry(name)
     if len(args) != count:
         raise TypeError(f"{name} takes {count} arguments before (cfg, stream): {load().prototypes[name][2][:-2]}")
@@ -52,16 +58,23 @@ def call(name: str, *args, cfg: Optional[KernelConfig] = None, stream: Optional[
     values = []
     for a in args:
         if isinstance(a, torch.Tensor):
-            if device is None and a.is_cuda:  # (a tensor that is not on a GPU is refused before a device is asked for)
-                device = torch.cuda.current_device()
-            if a.get_device() != device or not a.is_contiguous():
-                _refuse(a, device)
+            at = a.get_device()  # -1 on the host
+            if at < 0 or not a.is_contiguous():
+                _refuse(a)
+            if device is None:
+                device = at
+            elif at != device and stream is None:
+                raise ValueError(f"tensors on devices {device} and {at}: the call has no stream of its own to say where it runs")
             a = a.data_ptr()
         values.append(a)
-    if stream is None:
-        device = torch.cuda.current_device() if device is None else device
-        stream = torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device)
-    return fn(*values, ctypes.byref(DEFAULT_CONFIG if cfg is None else cfg), stream)
+    tail = ctypes.byref(DEFAULT_CONFIG if cfg is None else cfg)
+    if stream is not None:
+        return fn(*values, tail, stream)
+    current = torch.cuda.current_device()
+    if device is None or device == current:
+        return fn(*values, tail, _current_stream(current))
+    with torch.cuda.device(device):
+        return fn(*values, tail, _current_stream(device))
 
 
 def take_last_error() -> int:
