@@ -9,7 +9,7 @@
 //   loss = sum p_k (ln p_k - ln q_{i_k})
 //   d loss / d x_j = (P q_j - sum of the p_k with i_k = j) / T,   P = sum p_k
 // The k terms of a row are computed in 64 bits: the loss is a small difference of large terms where the student is
-// close, and they are few.
+// close, and they are few.  Where the gradient is asked for too their factors p_k are those of the gradient, rounded to 32 bits.
 #include "class_rows.hpp"
 
 namespace anode {
@@ -177,10 +177,16 @@ __device__ inline float slots_loss(const Teacher &t, size_t row, SoftmaxSum st, 
   const double logs = log(double(st.s) * tr.scale);  // ln S and the logarithm of the probabilities' scale
   double loss = 0.0;
   for (uint32_t j = threadIdx.x & (kWave - 1); j < t.k; j += kWave) {
-    const float p = s.p[j];
-    if (s.index[j] == kNoClass || p == 0.0f) continue;  // (a slot without mass adds nothing, whatever the student says)
+    if (s.index[j] == kNoClass) continue;
     const double lp = double(t.value[row * t.k + j]) * inv_t - tr.shift;
-    loss += double(p) * (lp - (double(s.x[j]) - double(st.m)) * inv_t + logs);
+    double p = double(s.p[j]);
+    if (p == 0.0 && lp > -746.0) {
+      // 32 bits hold none below 2^-149; the student may rule its class out all the same.  (A factor to 32 bits, its exponent in 64:
+      // another exp() costs the kernels registers.)
+      const double bits = lp * 1.4426950408889634, whole = rint(bits);
+      p = ldexp(double(__builtin_amdgcn_exp2f(float(bits - whole))), int(whole)) * tr.scale;
+    }
+    if (p != 0.0) loss += p * (lp - (double(s.x[j]) - double(st.m)) * inv_t + logs);  // (a slot without mass adds nothing, whatever the student says)
   }
   return float(lanes_sum(loss));
 }
