@@ -241,7 +241,7 @@ __device__ inline void store_group(void *p, V v) {
 // end.  b starts at -limit, limit = 65536 / c: while it stays inside (-limit, limit) R is off by less than 2^-8 and
 // nothing overflows, whatever single values hold (-inf and the lowest value of a type add 0, a NaN shows in S).  A
 // row whose maximum lies outside -- nothing but -inf or a mask's lowest values, +inf, or values without measure --
-// is summed again in the plain form, exp2((x - m) * c).  Rows in earnest never do.
+// is summed again in the plain form, exp2((x - m) * c); of rows in earnest those are the positions that a mask empties.
 struct Scale {
   float c, limit;
 };
@@ -296,15 +296,8 @@ __device__ inline void fold_one(SoftmaxSum &t, float x, float c) {
   const float v[2] = {x, kMinusInf};
   fold(t, v, c);
 }
-__device__ inline SoftmaxSum merge(SoftmaxSum a, SoftmaxSum b, float c) {
-  SoftmaxSum r;
-  r.m = fmaxf(a.m, b.m);
-  const float shift = r.m * c;
-  r.s = a.s * __builtin_amdgcn_exp2f(a.m * c - shift) + b.s * __builtin_amdgcn_exp2f(b.m * c - shift);
-  return r;
-}
-// The same in every lane of the wave, added in a fixed order: first the maximum of all, then each lane's sum about it.  (Merging
-// pairs at every step takes two exponentials each.)
+// The lanes' parts together, the same in every lane of the wave, added in a fixed order: first the maximum of all, then each lane's
+// sum about it.  (Merging pairs at every step takes two exponentials each.)
 __device__ inline SoftmaxSum wave_merge(SoftmaxSum t, float c) {
   SoftmaxSum r = {lanes_max(t.m), 0.0f};
   r.s = lanes_upto(t.s * __builtin_amdgcn_exp2f(t.m * c - r.m * c));

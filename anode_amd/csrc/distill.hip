@@ -247,8 +247,8 @@ struct Parts {
   __device__ uint32_t count(uint32_t part, uint32_t n) const { return min(per, n - part * per); }
 };
 
-// One workgroup a row: statistics and loss.  Long rows are bound by reading: 4096 of 131072 bf16 5.9 TB/s, 1001 of 50257 halves 21.8
-// us (4.6 TB/s; 3 of them are the launch's beginning and end).  Short ones by the VALU, half of it the slots' 64-bit
+// One workgroup a row: statistics and loss.  Long rows are bound by reading: 4096 of 131072 bf16 6.0 TB/s, 1001 of 50257 halves 21.4
+// us (4.7 TB/s; 3 of them are the launch's beginning and end).  Short ones by the VALU, half of it the slots' 64-bit
 // terms: 65536 of 1000 bf16 57 us.
 template <typename T, int THREADS, int U>
 __global__ __launch_bounds__(THREADS) void distill_kernel(uint32_t n, uint32_t rows, size_t stride, Scale sc, double inv_t,
@@ -404,7 +404,7 @@ struct Joined {
 };
 
 // One workgroup a part of a row.  JOIN: the row's statistics are put together from its parts by every workgroup for itself, and
-// the first part's writes them and the loss.  Bound by memory: 1001 rows of 50257 halves 35.8 us (5.6 TB/s read and
+// the first part's writes them and the loss.  Bound by memory: 1001 rows of 50257 halves 36.2 us (5.6 TB/s read and
 // written), 512 of 131072 floats 95 us.
 template <typename T, int THREADS, int U, bool ACC, bool JOIN, int NT>
 __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32_t rows, size_t stride, Scale sc, double inv_t,
@@ -460,7 +460,7 @@ __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32
 // Loss and gradient, one workgroup a row: the first G groups of each streaming thread stay in registers from the statistics
 // to the gradient, so that x is read once (what lies behind them is streamed a second time).  The slots belong to a wave of
 // their own: their 64-bit exponentials and logarithms would spill the held registers of a wave that streams, and take
-// about as long as a small row.  [4096, 131072] bf16 402 us, [2048, 32768] f32 101 us, 5.3 TB/s read and written: what bounds it is
+// about as long as a small row.  [4096, 131072] bf16 407 us, [2048, 32768] f32 100 us, 5.3 TB/s read and written: what bounds it is
 // that a CU loads its rows, then stores them.  The same accesses without any arithmetic take 387 us of the first, a flat copy 328;
 // two workgroups a CU that hold half of their rows and read the rest twice 475.
 template <typename T, int S, int G, int NT>
@@ -571,8 +571,8 @@ __global__ __launch_bounds__(S + kWave) __attribute__((amdgpu_waves_per_eu(4))) 
   }
 }
 
-// The same for short rows, one wave a row.  Bound by the VALU: 65536 rows of 1000 bf16 115 us, where a copy takes 40; most of a
-// wave's 850 instructions are the slots'.
+// The same for short rows, one wave a row.  Bound by the VALU: 65536 rows of 1000 bf16 116 us, where a copy takes 40; most of a
+// wave's 900 instructions are the slots'.
 template <typename T, int G, int NT>
 __global__ __launch_bounds__(kWave) __attribute__((amdgpu_waves_per_eu(4))) void distill_wave_kernel(
     uint32_t n, uint32_t rows, size_t stride, Scale sc, double inv_t, const T *x, Teacher t, const float *__restrict__ dy,

@@ -448,13 +448,13 @@ __device__ inline uint32_t key_of_threads(const uint32_t *thread_key, uint32_t k
 // value and is always read again; its thread counts for nothing in the threshold.)  Rows for which there are too many
 // (thousands of ties at the threshold, the largest values all in few segments) are selected from with further passes.
 //
-// Bound by reading: [2048, 131072] bf16 with the norm 95 us (5.6 TB/s) for k = 1, 99 us (5.4) for k = 64, 228 us for k = 1000,
+// Bound by reading: [2048, 131072] bf16 with the norm 96 us (5.6 TB/s) for k = 1, 99 us (5.4) for k = 64, 231 us for k = 1000,
 // whose 1200 candidates are sorted.  A threshold held while the row streams, with a list of what reaches it, took 114 us:
 // its branches, barriers and LDS additions cost more than the 75 segments that are read again here.  With 8 segments a
 // thread the 64 take 111 us and the 1000 1742, with 32 103 and 294; with two groups of a thread on their way together
 // instead of four the 64 take 114.  The threads' threshold instead of the waves' is as quick for random values and eight
-// times as quick for rows in falling order.  [512, 131072] f32 47 us of random values, 111 of zeros, 79 in rising order;
-// bf16 29, 75 and 46.
+// times as quick for rows in falling order.  [512, 131072], k = 64 with the norm, three arrays in turn: f32 62 us of random
+// values (44 where one array stays in the last cache), 124 of zeros, 60 in rising order; bf16 33, 79 and 41.
 template <typename T, int THREADS, int SHORT, bool NORM>
 __global__ __launch_bounds__(THREADS) __attribute__((amdgpu_waves_per_eu(THREADS <= 128 && sizeof(T) == 4 ? 5 : 4))) void top_k_kernel(
     uint32_t n, uint32_t rows, size_t stride, uint32_t k, Scale sc, double inv_t, Cut cut, const T *__restrict__ x,

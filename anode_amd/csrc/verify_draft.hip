@@ -261,7 +261,7 @@ struct Sums {
 constexpr uint32_t kRefused = 0x80000000u;
 
 // One wave a block of a sequence's row (every wave finds out for itself which row that is).  Bound by reading: 1024 sequences of
-// 131072 classes, half of them with a refusal, 127 us (6.6 TB/s).  64-bit sums are free there: a wave waits 72 % of its time.
+// 131072 classes, half of them with a refusal, 128 us (6.5 TB/s).  64-bit sums are free there: a wave waits 72 % of its time.
 template <int NT>
 __global__ __launch_bounds__(kDrawThreads) void draw_sums_kernel(Drafts d, uint32_t sequences, uint32_t blocks, Sums out) {
   const RowGroups<float> rg(d.n);

@@ -309,7 +309,7 @@ int anode_gpu_top_k_rows_f16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint
  *   q    = softmax(x / t), row_max = max x, row_sum = sum exp((x - row_max) / t);
  *   loss = sum_k p_k (ln p_k - ln q[teacher_index[k]]), a term with p_k = 0 being 0.
  * A row without a slot has loss 0 whatever x holds (ignored positions).  A row of x that holds NaN or +inf, or -inf
- * only, gives NaN as its softmax does.  One slot holding the label is softmax_cat_nll. */
+ * only, gives NaN as its softmax does (row_max passes over NaN).  One slot holding the label is softmax_cat_nll. */
 int anode_gpu_softmax_distill_rows_f32(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const float *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, float *loss, float *row_max, float *row_sum, ANODE_LAUNCH_TAIL);
 int anode_gpu_softmax_distill_rows_bf16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, float *loss, float *row_max, float *row_sum, ANODE_LAUNCH_TAIL);
 int anode_gpu_softmax_distill_rows_f16(uint32_t dim0, uint32_t dim1, uint32_t stride, uint32_t k, float temperature, const uint16_t *x, const float *teacher_value, const uint32_t *teacher_index, const float *teacher_log_norm, float *loss, float *row_max, float *row_sum, ANODE_LAUNCH_TAIL);
@@ -398,7 +398,7 @@ size_t anode_host_arg_max_f32(const float *xs, size_t len);
  * buffer that is large enough -- the reduction entry point enqueues nothing, reports on stderr and records the
  * hipError_t for anode_gpu_take_last_error().  A HIP graph keeps the buffer of the stream it was captured on: graphs
  * captured on one stream must not be replayed concurrently with each other or with eager reduction calls on that
- * stream. */
+ * stream.  The entry points over rows of classes keep what few long rows leave in the same buffer, under the same rules. */
 /* Upper bound of the scratch bytes any reduction entry point needs for a [dim0, dim1, dim2] array, for either
  * alignment of its arrays.  The bound holds for the library's tiling as it is when the function is called: the
  * tiling is fixed for a build and only moves through the library's undeclared measurement hook, after which the
@@ -420,7 +420,8 @@ int anode_gpu_release_scratch(struct CUstream_st *stream);
  * (the reference's kernels leave it to the caller, whose own checks must keep seeing what they see today): a failed
  * launch is noticed by peeking at that state, so while the caller leaves an error pending there (no
  * hipGetLastError()), a later launch that fails with the same hipError_t cannot be told from the pending one and is
- * not recorded again.  Refusals (scratch unavailable, stream under capture) are always recorded. */
+ * not recorded again.  Refusals (scratch unavailable, stream under capture) are always recorded, and so are the failed
+ * launches of the entry points over rows of classes, which also return their own code. */
 int anode_gpu_take_last_error(void);
 /* Number of entry points of Part 1 (46). */
 uint32_t anode_gpu_reference_symbol_count(void);
