@@ -9,7 +9,7 @@
 //   loss = sum p_k (ln p_k - ln q_{i_k})
 //   d loss / d x_j = (P q_j - sum of the p_k with i_k = j) / T,   P = sum p_k
 // The k terms of a row are computed in 64 bits: the loss is a small difference of large terms where the student is
-// close, and they are few.  Where the gradient is asked for too their factors p_k are those of the gradient, rounded to 32 bits.
+// close, and they are few.
 #include "class_rows.hpp"
 
 namespace anode {
@@ -32,10 +32,10 @@ struct TeacherRow {
 // The slots of a row in LDS.  A streaming thread finds those that lie in its groups by a list of its own, and the turns of its
 // that have one by a bit mask, so that it takes their part off the values while it still has them in registers.
 struct Slots {
+  double *p;        // [k]: the probability
   double *sum;      // [k]: where a class is named twice, the probabilities of a leader and of the slots that follow it
-  float *p;         // [k]: the probability
   float *x;         // [k]: the student's logit
-  float *off;       // [k]: what is taken off the gradient of its class
+  float *off;       // [k]: the teacher's logit; then what is taken off the gradient of its class
   uint32_t *index;  // [k]: the class; kNoClass for a slot that does not count
   uint32_t *next;   // [k]: a slot's leader; then the next slot of the same thread, or kNoClass
   uint32_t *head;   // [threads]: a thread's first slot, or kNoClass
@@ -44,11 +44,11 @@ struct Slots {
 };
 constexpr uint32_t kSeen = 2048;  // (the leading 11 bits of a product)
 __device__ inline Slots slots_in(double *lds, uint32_t k, uint32_t threads) {
-  float *f = reinterpret_cast<float *>(lds + k);
-  uint32_t *u = reinterpret_cast<uint32_t *>(f + 3u * k), *t = u + 2u * k;
-  return Slots{lds, f, f + k, f + 2u * k, u, u + k, t, t + threads, reinterpret_cast<volatile uint16_t *>(t + 2u * threads)};
+  float *f = reinterpret_cast<float *>(lds + 2u * k);
+  uint32_t *u = reinterpret_cast<uint32_t *>(f + 2u * k), *t = u + 2u * k;
+  return Slots{lds, lds + k, f, f + k, u, u + k, t, t + threads, reinterpret_cast<volatile uint16_t *>(t + 2u * threads)};
 }
-uint32_t slot_bytes(uint32_t k, uint32_t threads) { return 28u * k + 8u * threads + 2u * kSeen; }
+uint32_t slot_bytes(uint32_t k, uint32_t threads) { return 32u * k + 8u * threads + 2u * kSeen; }
 
 // Reads the slots of a row, by one whole wave: x is the row, n its length.  LOSS: the student's logits too, which the loss asks for
 // and the gradient does not.
@@ -63,7 +63,7 @@ __device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x
     const float v = t.value[first + j];
     const bool counts = at < n && v > kMinusInf;
     s.index[j] = counts ? at : kNoClass;
-    s.p[j] = v;
+    s.off[j] = v;
     if (LOSS) s.x[j] = counts ? float(x[at]) : 0.0f;
     if (counts) top = fmaxf(top, v);
   }
@@ -73,15 +73,15 @@ __device__ inline TeacherRow read_slots(const Teacher &t, size_t row, const T *x
   r.shift = t.log_norm != nullptr ? double(t.log_norm[row]) : double(top) * inv_t;
   double sum = 0.0;
   for (uint32_t j = lane; j < t.k; j += kWave) {
-    const double e = s.index[j] != kNoClass ? exp(double(s.p[j]) * inv_t - r.shift) : 0.0;
-    s.p[j] = float(e);
+    const double e = s.index[j] != kNoClass ? exp(double(s.off[j]) * inv_t - r.shift) : 0.0;
+    s.p[j] = e;
     sum += e;
   }
   sum = lanes_sum(sum);
   r.mass = sum;
   if (t.log_norm == nullptr) {
     r.scale = 1.0 / sum;
-    for (uint32_t j = lane; j < t.k; j += kWave) s.p[j] *= float(r.scale);
+    for (uint32_t j = lane; j < t.k; j += kWave) s.p[j] *= r.scale;
     r.mass = 1.0;
   }
   return r;
@@ -118,7 +118,7 @@ __device__ inline bool find_leaders(uint32_t k, const Slots &s) {
 // The probabilities of a class that is named more than once, at its leader; added one follower after the other, in slot order.
 __device__ inline void add_followers(uint32_t k, const Slots &s) {
   const uint32_t lane = threadIdx.x & (kWave - 1);
-  for (uint32_t j = lane; j < k; j += kWave) s.sum[j] = double(s.p[j]);
+  for (uint32_t j = lane; j < k; j += kWave) s.sum[j] = s.p[j];
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   for (uint32_t base = 0; base < k; base += kWave) {
     const uint32_t j = base + lane;
@@ -127,7 +127,7 @@ __device__ inline void add_followers(uint32_t k, const Slots &s) {
     for (uint64_t rest = __ballot(leader != j); rest != 0u; rest &= rest - 1u) {
       const int at = __ffsll((unsigned long long)rest) - 1;
       const uint32_t to = from_lane(leader, at);
-      if (lane == 0u) s.sum[to] += double(s.p[base + uint32_t(at)]);
+      if (lane == 0u) s.sum[to] += s.p[base + uint32_t(at)];
     }
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -150,7 +150,7 @@ __device__ inline void deal_slots(uint32_t k, bool any, const RowSpan<T> &span, 
     const uint32_t at = s.index[j] - from;
     const bool mine = s.index[j] != kNoClass && at < end + span.tail && s.next[j] == j;  // (a class below `from` wraps)
     s.next[j] = kNoClass;
-    s.off[j] = float(w * (repeated ? s.sum[j] : double(s.p[j])));
+    s.off[j] = float(w * (repeated ? s.sum[j] : s.p[j]));
     if (!mine) continue;
     const bool single = at < span.head || at >= end;
     const uint32_t place = single ? (at < span.head ? at : at - end + span.head) : (at - span.head) / uint32_t(RowSpan<T>::W);
@@ -177,16 +177,10 @@ __device__ inline float slots_loss(const Teacher &t, size_t row, SoftmaxSum st, 
   const double logs = log(double(st.s) * tr.scale);  // ln S and the logarithm of the probabilities' scale
   double loss = 0.0;
   for (uint32_t j = threadIdx.x & (kWave - 1); j < t.k; j += kWave) {
-    if (s.index[j] == kNoClass) continue;
+    const double p = s.p[j];
+    if (s.index[j] == kNoClass || p == 0.0) continue;  // (a slot without mass adds nothing, whatever the student says)
     const double lp = double(t.value[row * t.k + j]) * inv_t - tr.shift;
-    double p = double(s.p[j]);
-    if (p == 0.0 && lp > -746.0) {
-      // 32 bits hold none below 2^-149; the student may rule its class out all the same.  (A factor to 32 bits, its exponent in 64:
-      // another exp() costs the kernels registers.)
-      const double bits = lp * 1.4426950408889634, whole = rint(bits);
-      p = ldexp(double(__builtin_amdgcn_exp2f(float(bits - whole))), int(whole)) * tr.scale;
-    }
-    if (p != 0.0) loss += p * (lp - (double(s.x[j]) - double(st.m)) * inv_t + logs);  // (a slot without mass adds nothing, whatever the student says)
+    loss += p * (lp - (double(s.x[j]) - double(st.m)) * inv_t + logs);
   }
   return float(lanes_sum(loss));
 }

@@ -1,10 +1,10 @@
-"""The loss of distillation where a slot's probability is smaller than 32 bits hold, on the GPU: the loss alone and the call that
-also gives the gradient agree on it."""
+"""The loss of distillation on the GPU where its terms need the 64 bits that they are computed in: probabilities smaller than 32
+bits hold, and losses of hundreds.  The loss alone and the call that also gives the gradient agree on it."""
 import numpy as np
 import pytest
 
 from gpu_util import F32
-from test_gpu_class_rows import TYPES, check_distill, logits
+from test_gpu_class_rows import TYPES, check_distill, logits, rounded, slots
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +26,17 @@ def test_classes_that_the_student_rules_out(kind, mode, n, rows):
     check_distill(kind, x, value, index, 1.0, dy, None, mode, what="ruled out")
     check_distill(kind, x, value, index, 1.0, dy, np.full(rows, 3.0, F32), mode, what="ruled out, norm")
     check_distill(kind, x, value, index, 0.5, dy, None, mode, n + 3, 1, what="ruled out, sharp")
+
+
+@pytest.mark.parametrize("kind", TYPES)
+@pytest.mark.parametrize("mode", ["fused", "apart"])
+@pytest.mark.parametrize("n,k", [(13, 8), (40, 9), (700, 64), (3000, 30)])
+def test_large_losses(kind, mode, n, k):
+    # logits far apart: a loss of hundreds to thousands, of which the bound leaves little more than its own rounding
+    g = np.random.default_rng(n + k)
+    rows = 60
+    x = rounded(800.0 * g.standard_normal((rows, n)), kind)
+    value, index = slots(g, rows, n, k, absent=0.1)
+    dy = g.standard_normal(rows).astype(F32)
+    for t in (1.0, 0.5):
+        check_distill(kind, x, value, index, t, dy, None, mode, what="large losses")
