@@ -122,3 +122,35 @@ def test_distill_row_max_passes_over_nans(kind, n, rows):
             bad = np.flatnonzero(host(top) != want)
             assert bad.size == 0, (what, bad[:4], host(top)[bad[:4]], want[bad[:4]])
             assert np.array_equal(np.isnan(host(loss)), has) and np.array_equal(np.isnan(host(total)), has), what
+
+
+@pytest.mark.parametrize("kind", TYPES)
+def test_top_k_beside_nans_of_large_arrays(kind):
+    # more than the last cache holds: a thread's groups lie side by side there
+    n, rows, k = 131071, 800 if kind != "f32" else 400, 64
+    g = torch.Generator("cuda").manual_seed(5)
+    x = torch.randn(rows, n, generator=g, device="cuda").mul_(3.0).to(TYPES[kind])
+    seen = x.float().clone()                          # (float() of a float array is the array itself)
+    word, unsigned, _ = WORD[kind]
+    bits = x.view(word)
+    place = torch.randint(100, n - 100, (rows,), generator=g, device="cuda")
+    row = torch.arange(rows, device="cuda")
+    for d in (-12, -5, -1, 1, 4, 12):                 # the largest values round the NaN
+        seen[row, place + d] = 30.0 + d
+    x.copy_(seen.to(TYPES[kind]))
+    seen.copy_(x)
+    for i, b in enumerate(BITS[kind]):
+        at = row[i::len(BITS[kind]) + 1]              # (every fifth row has none)
+        bits[at, place[at]] = torch.from_numpy(np.array([b], unsigned).view(WORD[kind][2])).cuda()
+        seen[at, place[at]] = -float("inf")
+    value, check_v = guarded(rows * k)
+    index, check_i = guarded(rows * k, torch.int32)
+    norm, check_n = guarded(rows)
+    call("anode_gpu_top_k_rows_" + kind, n, rows, 0, k, 1.0, x, value, index, norm)
+    for c in (check_v, check_i, check_n):
+        c("large array with NaN")
+    v, i = value.view(rows, k), index.view(rows, k)
+    assert bool((v == torch.sort(seen, dim=1, descending=True)[0][:, :k]).all())
+    assert bool((seen.gather(1, i.long()) == v).all())
+    has = row % (len(BITS[kind]) + 1) < len(BITS[kind])
+    assert bool((torch.isnan(norm) == has).all())
