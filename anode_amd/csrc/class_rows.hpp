@@ -23,6 +23,13 @@ static inline int refuse(const char *symbol, const char *what) {
   return int(hipErrorInvalidValue);
 }
 
+// acquire_scratch() with the code of its own failure, 0 if there was none (runtime.hip).  (What the process recorded last may be
+// another thread's error, or taken by it.)
+ScratchLease acquire_scratch(hipStream_t stream, size_t bytes, const char *symbol, int &error);
+// What note_launch() does, of a launch whose own result is known: `e` is recorded and printed if it is an error, and returned.
+// (The thread's error state may hold an error from before, or the same one from an earlier launch.)
+int note_launched(const char *symbol, hipError_t e);
+
 // The stream's scratch (runtime.hip) for these entry points, which return an error code and let no exception out: ptr is
 // null when it cannot be had, and `error` then what the entry point returns.
 struct RowsScratch {
@@ -32,8 +39,7 @@ struct RowsScratch {
 static inline RowsScratch rows_scratch(hipStream_t stream, size_t bytes, const char *symbol) {
   RowsScratch s = {ScratchLease{}, 0};
   try {
-    s.lease = acquire_scratch(stream, bytes, symbol);
-    s.error = s.lease.error;
+    s.lease = acquire_scratch(stream, bytes, symbol, s.error);
   } catch (...) {
     note_error(symbol, hipErrorOutOfMemory, "cannot keep account of the scratch");
     s.error = int(hipErrorOutOfMemory);

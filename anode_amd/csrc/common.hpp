@@ -302,9 +302,6 @@ uint32_t checked_len(uint64_t a, uint64_t b, uint64_t c, const char *symbol);
 // Looks at the thread's HIP error state after a launch (hipPeekAtLastError: the state is left to the caller) and,
 // when an error has appeared, records it for anode_gpu_take_last_error() and prints it to stderr.
 void note_launch(const char *symbol);
-// The same of a launch whose own result is known: `e` is recorded and printed if it is an error, and returned.  (The thread's error
-// state may hold an error from before, or the same one from an earlier launch, so it does not tell how this one went.)
-int note_launched(const char *symbol, hipError_t e);
 // Records `e` for anode_gpu_take_last_error() and prints "<symbol>: <what>: <error string>".
 void note_error(const char *symbol, hipError_t e, const char *what);
 
@@ -315,12 +312,11 @@ void note_error(const char *symbol, hipError_t e, const char *what);
 // interleave their launches; threads on other streams or devices are not held up.
 // When the buffer cannot be provided (allocation failure, or the stream is being
 // captured and would have to allocate) the error is recorded under `symbol`, ptr
-// is null, the lock is not held and `error` is this call's code: the caller skips its launch.
+// is null and the lock is not held: the caller skips its launch.
 struct ScratchLease {
   void *ptr;
   std::unique_lock<std::mutex> lock;
   std::shared_ptr<void> owner;  // keeps the cache entry (and with it the mutex) alive while the lease is
-  int error = 0;
 };
 ScratchLease acquire_scratch(hipStream_t stream, size_t bytes, const char *symbol);
 

@@ -1,6 +1,7 @@
 // Host-side runtime shared by all entry points: device queries, launch
 // geometry, the per-(device, stream) scratch cache and error bookkeeping.
 #include "chan_reduce.hpp"
+#include "class_rows.hpp"
 #include "common.hpp"
 
 #include <atomic>
@@ -318,6 +319,12 @@ ReducePlan plan_chan_reduce(uint32_t S, uint32_t C, uint32_t N, bool ptrs_aligne
 }
 
 ScratchLease acquire_scratch(hipStream_t stream, size_t bytes, const char *symbol) {
+  int error;
+  return acquire_scratch(stream, bytes, symbol, error);
+}
+
+ScratchLease acquire_scratch(hipStream_t stream, size_t bytes, const char *symbol, int &error) {
+  error = 0;
   int dev = 0;
   (void)hipGetDevice(&dev);
   std::shared_ptr<ScratchBuf> entry;
@@ -329,9 +336,9 @@ ScratchLease acquire_scratch(hipStream_t stream, size_t bytes, const char *symbo
   }
   ScratchLease lease{nullptr, std::unique_lock<std::mutex>(entry->mu), entry};
   ScratchBuf &buf = *entry;
-  auto refuse = [&](hipError_t e, const char *what) {
+  auto give_up = [&](hipError_t e, const char *what) {
     note_error(symbol, e, what);
-    lease.error = int(e);
+    error = int(e);
     lease.lock.unlock();
   };
   if (buf.cap < bytes) {
@@ -342,13 +349,13 @@ ScratchLease acquire_scratch(hipStream_t stream, size_t bytes, const char *symbo
     hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
     const hipError_t q = hipStreamIsCapturing(stream, &capturing);
     if (q != hipSuccess) {
-      refuse(q, "cannot read the capture state of the stream, so the reduction scratch is not allocated");
+      give_up(q, "cannot read the capture state of the stream, so the reduction scratch is not allocated");
       return lease;
     }
     if (capturing != hipStreamCaptureStatusNone) {
-      refuse(hipErrorStreamCaptureUnsupported,
-             "the stream is being captured and has no reduction scratch yet (call anode_gpu_reserve_scratch "
-             "or run the entry point once on this stream before capturing)");
+      give_up(hipErrorStreamCaptureUnsupported,
+              "the stream is being captured and has no reduction scratch yet (call anode_gpu_reserve_scratch "
+              "or run the entry point once on this stream before capturing)");
       return lease;
     }
     // Grow geometrically.  The previous buffer may still be read by kernels in flight on this stream, so it is
@@ -359,7 +366,7 @@ ScratchLease acquire_scratch(hipStream_t stream, size_t bytes, const char *symbo
     void *p = nullptr;
     const hipError_t e = hipMalloc(&p, cap);
     if (e != hipSuccess || !p) {
-      refuse(e != hipSuccess ? e : hipErrorOutOfMemory, "cannot allocate the reduction scratch");
+      give_up(e != hipSuccess ? e : hipErrorOutOfMemory, "cannot allocate the reduction scratch");
       return lease;
     }
     if (buf.ptr) buf.outgrown.push_back(buf.ptr);
@@ -395,9 +402,9 @@ ANODE_EXPORT size_t anode_gpu_reduce_scratch_bytes(uint32_t S, uint32_t C, uint3
 // current device, so that later calls on that stream allocate nothing (needed before the stream is captured into a
 // HIP graph).  Returns 0 or the hipError_t of the failed allocation.
 ANODE_EXPORT int anode_gpu_reserve_scratch(CUstream_st *stream, size_t bytes) {
-  anode::ScratchLease lease = anode::acquire_scratch(anode::as_stream(stream), bytes, __func__);
-  if (lease.ptr || bytes == 0) return 0;
-  return lease.error;
+  int error = 0;
+  anode::ScratchLease lease = anode::acquire_scratch(anode::as_stream(stream), bytes, __func__, error);
+  return lease.ptr || bytes == 0 ? 0 : error;
 }
 
 // Frees every scratch buffer held for `stream` on the current device.  The caller must have synchronised the
