@@ -241,7 +241,7 @@ struct Parts {
   __device__ uint32_t count(uint32_t part, uint32_t n) const { return min(per, n - part * per); }
 };
 
-// One workgroup a row: statistics and loss.  Long rows are bound by reading: 4096 of 131072 bf16 6.0 TB/s, 1001 of 50257 halves 21.4
+// One workgroup a row: statistics and loss.  Long rows are bound by reading: 4096 of 131072 bf16 6.0 TB/s, 1001 of 50257 halves 21.6
 // us (4.7 TB/s; 3 of them are the launch's beginning and end).  Short ones by the VALU, half of it the slots' 64-bit
 // terms: 65536 of 1000 bf16 57 us.
 template <typename T, int THREADS, int U>
@@ -398,7 +398,7 @@ struct Joined {
 };
 
 // One workgroup a part of a row.  JOIN: the row's statistics are put together from its parts by every workgroup for itself, and
-// the first part's writes them and the loss.  Bound by memory: 1001 rows of 50257 halves 36.2 us (5.6 TB/s read and
+// the first part's writes them and the loss.  Bound by memory: 1001 rows of 50257 halves 36.0 us (5.6 TB/s read and
 // written), 512 of 131072 floats 95 us.
 template <typename T, int THREADS, int U, bool ACC, bool JOIN, int NT>
 __global__ __launch_bounds__(THREADS) void distill_bwd_kernel(uint32_t n, uint32_t rows, size_t stride, Scale sc, double inv_t,
