@@ -340,7 +340,7 @@ int anode_gpu_softmax_distill_fused_fwd_bwd_rows_f16(uint32_t dim0, uint32_t dim
  * of 1 or more, or NaN, draws the last class that weighs; weights that are not greater than zero, NaN among them, do not
  * weigh; where none weighs the token is 0xffffffff.)  draft may be null: each drafted token is then a point mass (it was
  * looked up, or chosen greedily), taken with probability target[token].  token[., b] gets the taken tokens, the drawn one
- * and 0xffffffff behind it.  dim1 = 0 draws one token of each target row. */
+ * and 0xffffffff behind it.  dim1 = 0 draws one token of each target row; dim1 of 2^31 and more is refused (1). */
 int anode_gpu_verify_draft_packed_f32(uint32_t dim0, uint32_t dim1, uint32_t dim2, const float *target, const float *draft, const uint32_t *draft_token, const uint32_t *draft_length, const float *accept, const float *pick, uint32_t *token, uint32_t *accepted, ANODE_LAUNCH_TAIL);
 
 /* ---- the neighbours anode takes from its sibling library gpudevicemem (source not part of the reference tree) ----
